@@ -4,10 +4,12 @@
     box-convolutions_b200/box_convolution/_torch_binding.<ABI>.so
 
 The library: plain nvcc, no torch headers; its surface is the C ABI in include/boxconv_b200.h.
-nvcc cross-compiles without a GPU.  The binding (csrc/torch_binding.cpp): g++ with torch's headers,
-linked against the library beside it.  Usage: python box-convolutions_b200/build.py [--force] [-v]
+nvcc cross-compiles without a GPU.  Every source becomes an object under build/ of its own, made again when it
+or a header that it includes has changed.  The binding (csrc/*.cpp): g++ with torch's headers, linked against
+the library beside it.  Usage: python box-convolutions_b200/build.py [--force] [-v]
 """
 import argparse
+import concurrent.futures
 import glob
 import os
 import subprocess
@@ -20,22 +22,16 @@ OUT = os.path.join(HERE, "box_convolution", "libboxconv_b200.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
-    "-O3", "-lineinfo", "-std=c++17", "--threads", "0", "-Xcompiler", "-fPIC", "-shared",
+    "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC",
 ]
+OBJECTS = os.path.join(HERE, "build")
 
-
-BINDING_SRC = os.path.join(CSRC, "torch_binding.cpp")
 BINDING = os.path.join(HERE, "box_convolution", "_torch_binding" + sysconfig.get_config_var("EXT_SUFFIX"))
 CXX = os.environ.get("CXX", "g++")
 
 
 def sources():
     return sorted(glob.glob(os.path.join(CSRC, "*.cu")))
-
-
-def headers():
-    return sorted(glob.glob(os.path.join(CSRC, "*.cuh"))) + [
-        os.path.join(os.path.dirname(HERE), "include", "boxconv_b200.h")]
 
 
 def newer(out, inputs):
@@ -52,23 +48,49 @@ def run(cmd, out, verbose):
     os.replace(out + ".tmp", out)
 
 
+def compile_object(compiler, src, force, verbose):
+    """One source's object, and whether it had to be made; what it includes is read from the compiler's list."""
+    obj = os.path.join(OBJECTS, os.path.basename(src) + ".o")
+    deps = obj + ".d"
+    inputs = [src]
+    if os.path.exists(deps):
+        listed = open(deps).read().replace("\\\n", " ").split(":", 1)[1].split()
+        inputs += [f for f in listed if os.path.abspath(f).startswith(os.path.dirname(HERE) + os.sep)]
+    if not force and os.path.exists(deps) and all(map(os.path.exists, inputs)) and newer(obj, inputs):
+        return obj, False
+    run(compiler + ["-MMD", "-MF", deps, "-MT", obj, "-c", "-o", obj + ".tmp", src], obj, verbose)
+    return obj, True
+
+
+def compile_all(compiler, srcs, force, verbose):
+    os.makedirs(OBJECTS, exist_ok=True)
+    with concurrent.futures.ThreadPoolExecutor(max(1, os.cpu_count() or 1)) as pool:
+        made = list(pool.map(lambda s: compile_object(compiler, s, force, verbose), srcs))
+    return [o for o, _ in made], any(new for _, new in made)
+
+
 def build_library(force=False, verbose=False):
-    if force or not newer(OUT, sources() + headers()):
-        run([NVCC] + FLAGS + (["-Xptxas", "-v"] if verbose else []) + ["-o", OUT + ".tmp"] + sources(), OUT, verbose)
+    # (the largest sources first: they take minutes)
+    srcs = sorted(sources(), key=os.path.getsize, reverse=True)
+    objs, new = compile_all([NVCC] + FLAGS + (["-Xptxas", "-v"] if verbose else []), srcs, force, verbose)
+    if new or not newer(OUT, objs):
+        run([NVCC] + FLAGS + ["-shared", "-o", OUT + ".tmp"] + objs, OUT, verbose)
     return OUT
 
 
 def build_binding(force=False, verbose=False):
-    if force or not newer(BINDING, [BINDING_SRC, headers()[-1]]):
-        import torch
-        root = os.path.dirname(torch.__file__)
-        cuda = os.path.dirname(os.path.dirname(NVCC))
-        dirs = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
-                sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
-        libs = os.path.join(root, "lib")
-        run([CXX, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-             "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI] + ["-isystem" + d for d in dirs] +
-            ["-o", BINDING + ".tmp", BINDING_SRC, "-L" + os.path.dirname(OUT), "-lboxconv_b200", "-L" + libs, "-lc10", "-lc10_cuda",
+    import torch
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(NVCC))
+    dirs = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+            sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
+    libs = os.path.join(root, "lib")
+    objs, new = compile_all([CXX, "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden",
+                             "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI] + ["-isystem" + d for d in dirs],
+                            sorted(glob.glob(os.path.join(CSRC, "*.cpp"))), force, verbose)
+    if new or not newer(BINDING, objs):
+        run([CXX, "-shared", "-o", BINDING + ".tmp"] + objs +
+            ["-L" + os.path.dirname(OUT), "-lboxconv_b200", "-L" + libs, "-lc10", "-lc10_cuda",
              "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python", "-Wl,-rpath,$ORIGIN", "-Wl,-rpath," + libs],
             BINDING, verbose)
     return BINDING
