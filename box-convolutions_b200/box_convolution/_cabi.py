@@ -51,6 +51,13 @@ SIGNATURES = {
     "bc_pack_parameters": (_i, [_vp] * 4 + [_i, _i, _vp, _vp, _i, _vp]),
     "bc_boxconv2d_host_step_workspace": (_sz, [_i] * 6),
     "bc_boxconv2d_host_step": (_i, [_vp] * 9 + [_f, _f, _d, _d] + [_i] * 9 + [_vp, _sz, _vp, _vp, _vp]),
+    "bc_pointwise_forward": (_i, [_vp] * 5 + [_i] * 4 + [_i64, _i, _i, _vp]),
+    "bc_pointwise_backward_workspace": (_sz, [_i] * 4 + [_i64] + [_i] * 3),
+    "bc_pointwise_backward": (_i, [_vp] * 5 + [_i] * 4 + [_i64] + [_i] * 3 + [_vp] * 5 + [_sz, _vp]),
+    "bc_group_norm_forward_workspace": (_sz, [_i] * 3 + [_i64, _i, _i]),
+    "bc_group_norm_forward": (_i, [_vp] * 5 + [_i] * 3 + [_i64, _i, _f, _i, _i, _vp, _sz, _vp]),
+    "bc_group_norm_backward_workspace": (_sz, [_i] * 3 + [_i64, _i, _i]),
+    "bc_group_norm_backward": (_i, [_vp] * 5 + [_i] * 3 + [_i64] + [_i] * 4 + [_vp] * 4 + [_sz, _vp]),
     "bc_launch_count": (ctypes.c_uint64, []),
     "bc_wait_timeouts": (_i, [ctypes.POINTER(_i)]),
     "bc_profile_start": (_i, [_i]),

@@ -804,6 +804,12 @@ const char *bc_kernel_name(int kernel_id)
         case KID_BACKWARD_QUAD_PAIR: return "backward_quad_pair_kernel";
         case KID_BACKWARD_SQUARE: return "backward_square_kernel";
         case KID_FORWARD_FLAT: return "forward_flat_kernel";
+        case KID_POINTWISE: return "pointwise_kernel";
+        case KID_POINTWISE_WEIGHT: return "pointwise_weight_kernel";
+        case KID_POINTWISE_FINISH: return "pointwise_finish_kernel";
+        case KID_NORM_FORWARD: return "norm_forward_kernel";
+        case KID_NORM_BACKWARD: return "norm_backward_kernel";
+        case KID_NORM_FINISH: return "norm_finish_kernel";
         default: return "unknown";
     }
 }

@@ -250,6 +250,49 @@ int bc_clip_parameters_any(void *x_min, void *x_max, void *y_min, void *y_max, i
 int bc_pack_parameters(const void *x_min, const void *x_max, const void *y_min, const void *y_max, int io_kind, int count,
                        float *packed_out, unsigned *zeroed, int zeroed_count, bc_stream_t stream);
 
+/* ---- the layers around a box convolution ---------------------------------------------------
+ * A box convolution filters every plane by itself; what mixes planes and keeps their scale stands around it: in the
+ * reference's blocks a 1 x 1 convolution in front and normalisations with activations and a skip connection
+ * (examples/Cityscapes/models/ENet.py:282-304, examples/Cityscapes/models/ERFNet.py:117-137), PyTorch operators there.
+ *
+ * Tensors of N samples of `pixels` = h*w pixels: planes (N, C, pixels), or channels last (N, pixels, C) with
+ * channels_last nonzero, all tensors of a call alike; every array of type io_kind (BC_IO_*) unless stated.  Sums, statistics
+ * and products are float; results are rounded once.  activation: BC_ACT_*, GELU is the one with the error function.
+ * Workspaces: 256-byte aligned, may be NULL where the query says 0; calls that are not ordered by a stream need
+ * workspaces of their own.  Sums are taken in a fixed order: the same call gives the same bits. */
+enum { BC_ACT_NONE = 0, BC_ACT_RELU = 1, BC_ACT_SILU = 2, BC_ACT_GELU = 3 };
+
+/* out[n,o,p] = act( sum_i weight[o,i] * input[n,i,p] + bias[o] + residual[n,o,p] ): weight (out_planes, in_planes);
+ * bias (out_planes) or NULL; residual like out, or NULL.  out overlaps no input, except that it may be residual. */
+int bc_pointwise_forward(const void *input, const void *weight, const void *bias, const void *residual, void *out, int io_kind,
+                         int N, int in_planes, int out_planes, int64_t pixels, int channels_last, int activation, bc_stream_t stream);
+/* Gradients of the same; bits of need_mask as below, an array whose bit is clear may be NULL and is left untouched.
+ * What the activation's slope needs is computed again from input, weight, bias and residual.  grad_residual without an
+ * activation would be grad_output itself: the bit is then ignored. */
+enum { BC_NEED_PW_INPUT = 1, BC_NEED_PW_WEIGHT = 2, BC_NEED_PW_BIAS = 4, BC_NEED_PW_RESIDUAL = 8 };
+size_t bc_pointwise_backward_workspace(int io_kind, int N, int in_planes, int out_planes, int64_t pixels, int channels_last,
+                                       int activation, int need_mask);
+int bc_pointwise_backward(const void *input, const void *weight, const void *bias, const void *residual, const void *grad_output,
+                          int io_kind, int N, int in_planes, int out_planes, int64_t pixels, int channels_last, int activation,
+                          int need_mask, void *grad_input, void *grad_weight, void *grad_bias, void *grad_residual,
+                          void *workspace, size_t workspace_bytes, bc_stream_t stream);
+
+/* out = act( weight[c] * (input - mean) / sqrt(var + eps) + bias[c] ): mean and (biased) variance over the pixels of the
+ * C / groups adjacent channels of a sample's group; weight and bias (C), each or both NULL for 1 and 0.  stats, which may be
+ * NULL, receives 2 * N * groups floats, the mean and 1 / sqrt(var + eps) of every group: the backward pass reads them.
+ * out overlaps no input. */
+size_t bc_group_norm_forward_workspace(int io_kind, int N, int C, int64_t pixels, int groups, int channels_last);
+int bc_group_norm_forward(const void *input, const void *weight, const void *bias, void *out, float *stats, int io_kind, int N, int C,
+                          int64_t pixels, int groups, float eps, int channels_last, int activation, void *workspace,
+                          size_t workspace_bytes, bc_stream_t stream);
+/* bits of need_mask: input, weight, bias; an array whose bit is clear may be NULL and is left untouched */
+enum { BC_NEED_GN_INPUT = 1, BC_NEED_GN_WEIGHT = 2, BC_NEED_GN_BIAS = 4 };
+size_t bc_group_norm_backward_workspace(int io_kind, int N, int C, int64_t pixels, int groups, int channels_last);
+int bc_group_norm_backward(const void *input, const void *weight, const void *bias, const float *stats, const void *grad_output,
+                           int io_kind, int N, int C, int64_t pixels, int groups, int channels_last, int activation, int need_mask,
+                           void *grad_input, void *grad_weight, void *grad_bias, void *workspace, size_t workspace_bytes,
+                           bc_stream_t stream);
+
 /* ---- backward pass without caller-supplied scratch memory --------------------------------
  * This entry point has no counterpart in the reference (which allocates its temporaries with
  * at::empty on every call).  It is bc_boxconv2d_backward() for hosts that have no way to hand
