@@ -1,12 +1,15 @@
 // Group normalisation with an activation: out = act(weight * (x - mean) * rstd + bias), mean and variance over a sample's
 // group of D = C / G channels and P pixels, L = D * P values.
 //
-// Forward, one CTA a group: the mean, then the squares about it (a sum of squares minus a squared mean loses every digit
+// This file: which kernels serve a call (vectors of 16 bytes: group_norm_planes.cu, group_norm_last.cu), the general ones, and
+// the channels' sums over the samples.
+//
+// General forward, one CTA a group: the mean, then the squares about it (a sum of squares minus a squared mean loses every digit
 // where the mean is large), then the outputs.  Backward, with xhat = (x - mean) * rstd and dz = grad * act'(weight xhat + bias):
 //   S1 = sum dz and S2 = sum dz * xhat for each channel,
 //   grad_input = rstd * (weight dz - (sum_c weight S1 + xhat * sum_c weight S2) / L),
 //   grad_weight = sum_n S2,  grad_bias = sum_n S1.
-#include "bc_layers.cuh"
+#include "bc_norm.cuh"
 
 namespace bc {
 
@@ -113,25 +116,35 @@ __global__ void __launch_bounds__(kThreads) norm_backward_kernel(const T *__rest
     });
 }
 
-// Sums of the samples' S1 and S2, a warp a channel, in a fixed order.
+// The rows' S1 and S2 added up in a fixed order: a lane a channel, 32 rows at a time.
+constexpr int kFinish = 1024;
 template <typename T>
-__global__ void __launch_bounds__(kThreads) norm_finish_kernel(const float *__restrict__ sums, T *__restrict__ grad_weight,
-                                                               T *__restrict__ grad_bias, int N, int C)
+__global__ void __launch_bounds__(kFinish) norm_finish_kernel(const float *__restrict__ sums, T *__restrict__ grad_weight,
+                                                             T *__restrict__ grad_bias, int rows, int C)
 {
-    const int c = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    __shared__ float2 part[kFinish / 32][33];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
     grid_dependency_wait();
-    if (c >= C) return;
-    float s1 = 0, s2 = 0;
-    for (int n = lane; n < N; n += 32) {
-        const float2 v = reinterpret_cast<const float2 *>(sums)[(int64_t)n * C + c];
-        s1 += v.x;
-        s2 += v.y;
+    float2 t = make_float2(0.f, 0.f);
+    if (c < C) {
+        const float2 *from = reinterpret_cast<const float2 *>(sums) + c;
+#pragma unroll 8
+        for (int i = warp; i < rows; i += kFinish / 32) {
+            const float2 v = from[(int64_t)i * C];
+            t.x += v.x;
+            t.y += v.y;
+        }
     }
-    s1 = warp_sum(s1);
-    s2 = warp_sum(s2);
-    if (lane == 0) {
-        if (grad_bias) grad_bias[c] = from_float<T>(s1);
-        if (grad_weight) grad_weight[c] = from_float<T>(s2);
+    part[warp][lane] = t;
+    __syncthreads();
+    // a warp a channel
+    float2 v = part[lane][warp];
+    v.x = warp_sum(v.x);
+    v.y = warp_sum(v.y);
+    const int mine = blockIdx.x * 32 + warp;
+    if (lane == 0 && mine < C) {
+        if (grad_bias) grad_bias[mine] = from_float<T>(v.x);
+        if (grad_weight) grad_weight[mine] = from_float<T>(v.y);
     }
 }
 
@@ -146,15 +159,48 @@ int dispatch(const NormShape &s, F &&f)
     });
 }
 
+// How a call runs: planes of vectors, rows of vectors, or (channels last with more than 1024 places of a vector among the
+// channels; arrays off a vector's boundary) a CTA a group, value by value.
+struct Route {
+    bool planes = false, rows = false;
+    NormPlanes p{};
+    NormRows r{};
+    Route(const NormShape &s, bool aligned)
+    {
+        if (!aligned) return;
+        if (s.last) {
+            rows = plan_rows(s, &r);
+        } else {
+            plan_planes(s, &p);
+            planes = true;
+        }
+    }
+    int64_t sums(const NormShape &s) const { return (int64_t)s.N * (rows ? r.k : planes ? p.k : 1); }      // rows of S1, S2
+};
+
+bool aligned(const void *a, const void *b, const void *c = nullptr)
+{
+    return (((uintptr_t)a | (uintptr_t)b | (uintptr_t)c) & 15) == 0;
+}
+
 }  // namespace
 
-size_t group_norm_workspace(const NormShape &s, int need_mask) { return need_mask ? (size_t)s.N * s.C * 2 * sizeof(float) : 0; }
+size_t group_norm_workspace(const NormShape &s, int need_mask)
+{
+    // (the larger of the vectors' and the general way's: the query does not know the arrays)
+    const Route q(s, true);
+    const size_t general = need_mask ? (size_t)s.N * s.C * 8 : 0;
+    return std::max(general, q.rows ? rows_sums_bytes(s, q.r, need_mask != 0) : q.planes ? planes_sums_bytes(s, q.p, need_mask != 0) : 0);
+}
 
 int launch_group_norm_forward(const NormShape &s, const void *x, const void *weight, const void *bias, void *out, float *stats,
-                              void *, cudaStream_t stream)
+                              void *ws, cudaStream_t stream)
 {
     const int64_t groups = (int64_t)s.N * s.G;
     if (groups > INT32_MAX) return BC_ERR_BAD_SHAPE;
+    const Route q(s, aligned(x, out));
+    if (q.rows) return launch_norm_rows_forward(s, q.r, x, weight, bias, out, stats, ws, stream);
+    if (q.planes) return launch_norm_planes_forward(s, q.p, x, weight, bias, out, stats, ws, stream);
     return dispatch(s, [&](auto t, auto act, auto last) {
         using T = decltype(t);
         const LaunchScope scope(KID_NORM_FORWARD, stream);
@@ -170,21 +216,26 @@ int launch_group_norm_backward(const NormShape &s, const void *x, const void *we
 {
     const int64_t groups = (int64_t)s.N * s.G;
     if (groups > INT32_MAX) return BC_ERR_BAD_SHAPE;
-    const int e = dispatch(s, [&](auto t, auto act, auto last) {
+    void *gx = (need_mask & BC_NEED_GN_INPUT) ? grad_input : nullptr;
+    const Route q(s, aligned(x, grad, gx));
+    if (q.sums(s) > INT32_MAX) return BC_ERR_BAD_SHAPE;
+    int e;
+    if (q.rows) e = launch_norm_rows_backward(s, q.r, x, weight, bias, stats, grad, gx, (float *)ws, stream);
+    else if (q.planes) e = launch_norm_planes_backward(s, q.p, x, weight, bias, stats, grad, gx, (float *)ws, stream);
+    else e = dispatch(s, [&](auto t, auto act, auto last) {
         using T = decltype(t);
         const LaunchScope scope(KID_NORM_BACKWARD, stream);
         launch_overlapped(norm_backward_kernel<T, act(), last()>, (unsigned)groups, kThreads, 0, stream, (const T *)x, (const T *)weight,
-                          (const T *)bias, stats, (const T *)grad, (need_mask & BC_NEED_GN_INPUT) ? (T *)grad_input : nullptr,
-                          (float *)ws, s);
+                          (const T *)bias, stats, (const T *)grad, (T *)gx, (float *)ws, s);
         return check_launch("norm_backward_kernel");
     });
     if (e || !(need_mask & (BC_NEED_GN_WEIGHT | BC_NEED_GN_BIAS))) return e;
     return with_type(s.io_kind, [&](auto t) {
         using T = decltype(t);
         const LaunchScope scope(KID_NORM_FINISH, stream);
-        launch_overlapped(norm_finish_kernel<T>, (unsigned)((s.C + kThreads / 32 - 1) / (kThreads / 32)), kThreads, 0, stream,
-                          (const float *)ws, (need_mask & BC_NEED_GN_WEIGHT) ? (T *)grad_weight : nullptr,
-                          (need_mask & BC_NEED_GN_BIAS) ? (T *)grad_bias : nullptr, s.N, s.C);
+        launch_overlapped(norm_finish_kernel<T>, (unsigned)((s.C + 31) / 32), kFinish, 0, stream, (const float *)ws, 
+                          (need_mask & BC_NEED_GN_WEIGHT) ? (T *)grad_weight : nullptr,
+                          (need_mask & BC_NEED_GN_BIAS) ? (T *)grad_bias : nullptr, (int)q.sums(s), s.C);
         return check_launch("norm_finish_kernel");
     });
 }

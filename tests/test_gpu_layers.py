@@ -221,7 +221,7 @@ def check_norm(bc, x, G, w, b, g, act, eps=1e-5, train=True):
 NORM = [
     (1, 1, 1, 1, 1), (2, 6, 6, 1, 1), (3, 8, 2, 1, 1), (2, 32, 8, 32, 32), (1, 24, 1, 9, 11), (2, 60, 20, 31, 37), (2, 20, 4, 16, 24),
     (4, 128, 32, 16, 32), (1, 64, 16, 96, 128), (2, 7, 7, 13, 17), (1, 3, 1, 200, 301), (3, 96, 3, 5, 5), (64, 16, 4, 8, 8),
-    (1, 512, 32, 7, 9), (1, 1030, 10, 6, 7), (2, 1023, 1, 5, 4), (1, 8, 8, 128, 256), (2, 48, 6, 64, 64), (1, 2048, 32, 4, 5), (1, 8, 1, 250, 251),
+    (1, 512, 32, 7, 9), (1, 1030, 10, 6, 7), (2, 1035, 5, 5, 6), (3, 6144, 6144, 3, 3), (2, 1023, 1, 5, 4), (1, 8, 8, 128, 256), (2, 48, 6, 64, 64), (1, 2048, 32, 4, 5), (1, 8, 1, 250, 251),
 ]
 
 
