@@ -71,59 +71,136 @@ __device__ __forceinline__ uint4 pack(const float (&v)[kVec<T>])
         return make_uint4(narrow2(v[0], v[1], T()), narrow2(v[2], v[3], T()), narrow2(v[4], v[5], T()), narrow2(v[6], v[7], T()));
 }
 
-// ---- activations (BC_ACT_*).  A NaN stays one in all of them; the ReLU's slope at zero and at NaN is 0, as PyTorch's.
-// The exponential and the quotients are CUDA's own in full precision for float tensors.  16-bit tensors take the fast
-// forms: their errors, some 2^-21 for arguments that matter, are far below the rounding at the end (2^-9, 2^-12).
+// The same as pairs for the packed arithmetic of two floats an instruction.
 template <typename T>
-__device__ __forceinline__ float exp_of(float v) { return sizeof(T) == 4 ? expf(v) : __expf(v); }
+__device__ __forceinline__ void unpack_pairs(const uint4 &w, f2_t (&v)[kVec<T> / 2])
+{
+    float f[kVec<T>];
+    unpack<T>(w, f);
+#pragma unroll
+    for (int j = 0; j < kVec<T> / 2; ++j) v[j] = pack2(f[2 * j], f[2 * j + 1]);
+}
 template <typename T>
-__device__ __forceinline__ float quotient(float a, float b) { return sizeof(T) == 4 ? a / b : __fdividef(a, b); }
+__device__ __forceinline__ uint4 pack_pairs(const f2_t (&v)[kVec<T> / 2])
+{
+    float f[kVec<T>];
+#pragma unroll
+    for (int j = 0; j < kVec<T> / 2; ++j) unpack2(v[j], f[2 * j], f[2 * j + 1]);
+    return pack<T>(f);
+}
+__device__ __forceinline__ f2_t both(float v) { return pack2(v, v); }
 
-// The normal distribution function, and its density times sqrt(2 pi).  Float tensors: CUDA's error function.  16-bit ones:
-// Abramowitz and Stegun's 7.1.26, five terms of 1 / (1 + 0.3275911 |x|) times exp(-x^2), x = z / sqrt(2), off by 7.5e-8 at
-// most: a third of the instructions, and the exponential serves the density too.
+// ---- activations (BC_ACT_*), of two values at a time.  A NaN stays one in all of them; the ReLU's slope at zero and at NaN
+// is 0, as PyTorch's.  Exponentials and quotients are the hardware's powers of two and reciprocals (2^-22 and 2^-23): with
+// CUDA's own functions a normalisation of float planes with SiLU was bound by instructions, (256,32,64,128) forward 148 us.
+// Float tensors carry the rounding of the exponent along; 16-bit ones, whose results are rounded to 2^-9 or 2^-12, do not, and
+// take the normal distribution function from Abramowitz and Stegun's 7.1.26: five terms of 1 / (1 + 0.3275911 |x|) times
+// exp(-x^2), x = z / sqrt(2), off by 7.5e-8 at most.
+__device__ __forceinline__ float power_of_two(float v)
+{
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ float reciprocal(float v)
+{
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+template <typename F>
+__device__ __forceinline__ f2_t of_each(f2_t v, F &&f)
+{
+    float a, b;
+    unpack2(v, a, b);
+    return pack2(f(a), f(b));
+}
+// 1 / (1 + exp(-z)).  One reciprocal for two, 1 / a = b / (a b): reciprocals and powers of two are what 16-bit
+// normalisations wait for.  exp(-z) ends at 2^60, so that the product stays finite (and a NaN to itself); beyond, 0 is the result.
 template <typename T>
-__device__ __forceinline__ float normal(float z, float &density)
+__device__ __forceinline__ f2_t logistic2(f2_t z)
+{
+    float t0, t1;
+    // (float: infinities and NaN have no rounding to carry along)
+    if constexpr (sizeof(T) == 4) z = of_each(z, [](float v) { return fminf(fmaxf(v, -1e4f), 1e4f); });
+    unpack2(mul2(z, both(-1.44269504f)), t0, t1);
+    f2_t e = pack2(power_of_two(fminf(t0, 60.f)), power_of_two(fminf(t1, 60.f)));
+    if constexpr (sizeof(T) == 4) {      // the exponent's rounding, and what 1.44269504f lacks of log2(e)
+        const f2_t rest = fma2(z, both(-1.9259629911e-8f), fma2(z, both(-1.44269504f), pack2(-t0, -t1)));
+        e = fma2(e, mul2(rest, both(0.69314718f)), e);
+    }
+    float a, b;
+    unpack2(add2(e, both(1.f)), a, b);
+    const float r = reciprocal(a * b);
+    return pack2(t0 > 60.f ? 0.f : b * r, t1 > 60.f ? 0.f : a * r);
+}
+// The normal distribution function, and exp(-z^2 / 2).
+template <typename T>
+__device__ __forceinline__ f2_t normal2(f2_t z, f2_t &density)
 {
     if constexpr (sizeof(T) == 4) {
-        density = expf(-0.5f * z * z);
-        return 0.5f * (1.f + erff(z * 0.70710678118654752f));
-    } else {
-        density = __expf(-0.5f * z * z);
-        const float t = __fdividef(1.f, fmaf(0.3275911f * 0.70710678118654752f, fabsf(z), 1.f));
-        float p = fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
-        p = fmaf(p, t, 0.5f * 1.421413741f);
-        p = fmaf(p, t, 0.5f * -0.284496736f);
-        p = fmaf(p, t, 0.5f * 0.254829592f) * t * density;      // the smaller of the two tails
-        return z < 0.f ? p : 1.f - p;
+        density = of_each(z, [](float v) { return expf(-0.5f * v * v); });
+        return of_each(z, [](float v) { return 0.5f * (1.f + erff(v * 0.70710678118654752f)); });
     }
+    density = of_each(mul2(mul2(z, z), both(-0.5f * 1.4426950408889634f)), power_of_two);
+    const f2_t size = of_each(z, [](float v) { return fabsf(v); });
+    const f2_t t = of_each(fma2(size, both(0.3275911f * 0.70710678118654752f), both(1.f)), reciprocal);
+    f2_t p = fma2(both(0.5f * 1.061405429f), t, both(0.5f * -1.453152027f));
+    p = fma2(p, t, both(0.5f * 1.421413741f));
+    p = fma2(p, t, both(0.5f * -0.284496736f));
+    p = fma2(p, t, both(0.5f * 0.254829592f));
+    p = mul2(mul2(p, t), density);      // the smaller of the two tails
+    float z0, z1, p0, p1;
+    unpack2(z, z0, z1);
+    unpack2(p, p0, p1);
+    return pack2(z0 < 0.f ? p0 : 1.f - p0, z1 < 0.f ? p1 : 1.f - p1);
 }
 
 template <int ACT, typename T>
-__device__ __forceinline__ float activate(float z)
+__device__ __forceinline__ f2_t activate2(f2_t z)
 {
-    if constexpr (ACT == BC_ACT_RELU) return z <= 0.f ? 0.f : z;
-    if constexpr (ACT == BC_ACT_SILU) return quotient<T>(z, 1.f + exp_of<T>(-z));
+    if constexpr (ACT == BC_ACT_RELU) return of_each(z, [](float v) { return v <= 0.f ? 0.f : v; });
+    if constexpr (ACT == BC_ACT_SILU) return mul2(z, logistic2<T>(z));
     if constexpr (ACT == BC_ACT_GELU) {
-        float density;
-        return z * normal<T>(z, density);
+        f2_t density;
+        return mul2(z, normal2<T>(z, density));
     }
     return z;
 }
+// g times the activation's slope
 template <int ACT, typename T>
-__device__ __forceinline__ float slope(float z)
+__device__ __forceinline__ f2_t times_slope2(f2_t g, f2_t z)
 {
-    if constexpr (ACT == BC_ACT_RELU) return z > 0.f ? 1.f : 0.f;
+    if constexpr (ACT == BC_ACT_RELU) {
+        float g0, g1, z0, z1;
+        unpack2(g, g0, g1);
+        unpack2(z, z0, z1);
+        return pack2(z0 > 0.f ? g0 : 0.f, z1 > 0.f ? g1 : 0.f);
+    }
     if constexpr (ACT == BC_ACT_SILU) {
-        const float s = quotient<T>(1.f, 1.f + exp_of<T>(-z));
-        return s * (1.f + z * (1.f - s));
+        const f2_t s = logistic2<T>(z), u = fma2(s, both(-1.f), both(1.f));
+        return mul2(mul2(g, s), fma2(z, u, both(1.f)));
     }
     if constexpr (ACT == BC_ACT_GELU) {
-        float density;
-        const float p = normal<T>(z, density);
-        return fmaf(z * 0.39894228040143268f, density, p);
+        f2_t density;
+        const f2_t p = normal2<T>(z, density);
+        return mul2(g, fma2(mul2(z, both(0.39894228040143268f)), density, p));
     }
-    return 1.f;
+    return g;
+}
+template <int ACT, typename T>
+__device__ __forceinline__ float activate(float z)
+{
+    float a, b;
+    unpack2(activate2<ACT, T>(pack2(z, 0.f)), a, b);
+    return a;
+}
+template <int ACT, typename T>
+__device__ __forceinline__ float times_slope(float g, float z)
+{
+    float a, b;
+    unpack2(times_slope2<ACT, T>(pack2(g, 0.f), pack2(z, 0.f)), a, b);
+    return a;
 }
 
 // A runtime activation as a template argument: f(std::integral_constant<int, ACT>).

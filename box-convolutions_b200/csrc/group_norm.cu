@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(kThreads) norm_backward_kernel(const T *__rest
         double s1 = 0, s2 = 0;
         for (int64_t p = threadIdx.x; p < s.P; p += kThreads) {
             const int64_t at = LAST ? (n * s.P + p) * s.C + c : (n * s.C + c) * s.P + p;
-            const float unit = (to_float(x[at]) - mean) * rstd, dz = to_float(grad[at]) * slope<ACT, T>(unit * w + b);
+            const float unit = (to_float(x[at]) - mean) * rstd, dz = times_slope<ACT, T>(to_float(grad[at]), unit * w + b);
             s1 += dz;
             s2 += dz * unit;
         }
@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(kThreads) norm_backward_kernel(const T *__rest
     const float a1 = (float)(all1 / ((double)D * s.P)), a2 = (float)(all2 / ((double)D * s.P));
     walk<LAST>(n, g, D, s.C, s.P, [&](int64_t at, int d) {
         const float w = weight ? to_float(weight[g * D + d]) : 1.f, b = bias ? to_float(bias[g * D + d]) : 0.f;
-        const float unit = (to_float(x[at]) - mean) * rstd, dz = to_float(grad[at]) * slope<ACT, T>(unit * w + b);
+        const float unit = (to_float(x[at]) - mean) * rstd, dz = times_slope<ACT, T>(to_float(grad[at]), unit * w + b);
         grad_input[at] = from_float<T>(rstd * (w * dz - a1 - unit * a2));
     });
 }

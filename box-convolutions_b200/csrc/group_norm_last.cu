@@ -31,31 +31,29 @@ struct Rows {
         const int64_t p0 = min(s.P, (int64_t)rank * r.per), p1 = min(s.P, p0 + r.per);
         const int t = threadIdx.x;
         if (r.slabs > 1) {      // aligned vectors of a part of the channels
-            const int cols = r.width / V, row = t / cols, rows = r.active / cols;
+            const unsigned cols = r.width / V, row = (unsigned)t / cols, rows = (unsigned)r.active / cols;
             channel = (t - row * cols) * V;
             first = (n * s.P + p0 + row) * s.C + slab * r.width + channel;
             step = (int64_t)rows * s.C;
-            count = t < r.active && p0 + row < p1 ? (int)((p1 - p0 - row + rows - 1) / rows) : 0;
+            count = t < r.active && p0 + row < p1 ? (int)(((unsigned)(p1 - p0) - row + rows - 1) / rows) : 0;
             phase = edges = 0;
             e0 = e1 = v0 = v1 = 0;
         } else {
             e0 = (n * s.P + p0) * s.C;
             e1 = (n * s.P + p1) * s.C;
-            v0 = min((e0 + V - 1) / V * V, e1);
-            v1 = max(e1 / V * V, v0);
+            v0 = min((e0 + V - 1) & ~(int64_t)(V - 1), e1);
+            v1 = max(e1 & ~(int64_t)(V - 1), v0);
             edges = (int)(v0 - e0 + e1 - v1);
             first = v0 + (int64_t)t * V;
             step = (int64_t)r.active * V;
-            count = t < r.active && first < v1 ? (int)((v1 - first + step - 1) / step) : 0;
+            count = 0;
+            if (t < r.active && first < v1) {
+                const int64_t more = v1 - first + step - 1;
+                count = more >> 32 ? (int)(more / step) : (int)((unsigned)more / (unsigned)step);
+            }
             phase = (int)(v0 - e0) % s.C;
             channel = (phase + t * V) % s.C;
         }
-    }
-    __device__ __forceinline__ int channel_of(int j, int width) const      // of the thread's value j, in the unit
-    {
-        int c = channel + j;
-        while (c >= width) c -= width;
-        return c;
     }
     // The i-th single value and its channel (one slab).
     __device__ __forceinline__ int64_t edge(int i, int C, int &c) const
@@ -82,11 +80,34 @@ __device__ __forceinline__ void each(const Rows<T> &r, F &&f)
     for (; i < r.count; ++i, at += r.step) f(std::integral_constant<int, 1>(), at);
 }
 
+// Channels' factors in shared memory, made once a CTA: rows of `width` floats.
+struct Affine {
+    float *base;
+    int width;
+    __device__ __forceinline__ void put(int c, int row, float v) const { base[row * width + c] = v; }
+    __device__ __forceinline__ float at(int c, int row) const { return base[row * width + c]; }
+    // Those of a thread's vector.
+    template <int V, typename R>
+    __device__ __forceinline__ void get(int row, const R &r, f2_t (&v)[V / 2]) const
+    {
+        int c = r.channel;
+        const float *from = base + row * width;
+#pragma unroll
+        for (int j = 0; j < V / 2; ++j) {
+            const float a = from[c];
+            c = c + 1 < width ? c + 1 : 0;
+            const float b = from[c];
+            c = c + 1 < width ? c + 1 : 0;
+            v[j] = pack2(a, b);
+        }
+    }
+};
+
 // Shared memory: positions (pairs), counts of threads, groups' moments and results.
 struct Layout {
-    int active_v, threads, groups;
+    int active_v, threads, width, groups;
     __host__ __device__ size_t pairs() const { return 0; }
-    __host__ __device__ size_t counts() const { return (size_t)active_v * 8; }
+    __host__ __device__ size_t counts() const { return (size_t)(active_v > 2 * width ? active_v : 2 * width) * 8; }      // (or three rows of channels)
     __host__ __device__ size_t moments() const { return counts() + (size_t)threads * 4; }
     __host__ __device__ size_t results() const { return (moments() + (size_t)groups * 12 + 7) / 8 * 8; }
     __host__ __device__ size_t edges() const { return results() + (size_t)groups * 8; }
@@ -100,19 +121,23 @@ __global__ void __launch_bounds__(THREADS) norm_rows_forward_kernel(const T *__r
     constexpr int V = kVec<T>;
     extern __shared__ __align__(16) char smem[];
     const int D = s.C / s.G, groups = plan.width / D, warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const Layout lay{plan.active * V, (int)blockDim.x, groups};
+    const Layout lay{plan.active * V, (int)blockDim.x, plan.width, groups};
     float2 *pairs = reinterpret_cast<float2 *>(smem + lay.pairs());
     float *counts = reinterpret_cast<float *>(smem + lay.counts());
     float *moments = reinterpret_cast<float *>(smem + lay.moments());
     float2 *results = reinterpret_cast<float2 *>(smem + lay.results());
     float2 *edges = reinterpret_cast<float2 *>(smem + lay.edges());
-    const int64_t unit = blockIdx.x / plan.k, n = unit / plan.slabs;
-    const int rank = (int)(blockIdx.x - unit * plan.k), slab = (int)(unit - n * plan.slabs);
+    const unsigned index = blockIdx.x / (unsigned)plan.k, sample = index / (unsigned)plan.slabs;
+    const int64_t unit = index, n = sample;
+    const int rank = (int)(blockIdx.x - index * plan.k), slab = (int)(index - sample * plan.slabs);
     const Rows<T> r(s, plan, n, slab, rank);
     grid_dependency_wait();
 
     if (STEP != NORM_RESULTS) {
-        float mean[V] = {}, m2[V] = {}, have = 0.f;
+        f2_t mean[V / 2], m2[V / 2];
+        float have = 0.f;
+#pragma unroll
+        for (int j = 0; j < V / 2; ++j) mean[j] = m2[j] = both(0.f);
         each(r, [&](auto many, int64_t at) {
             constexpr int M = decltype(many)::value;
             uint4 raw[M];
@@ -120,21 +145,39 @@ __global__ void __launch_bounds__(THREADS) norm_rows_forward_kernel(const T *__r
             for (int u = 0; u < M; ++u) raw[u] = *reinterpret_cast<const uint4 *>(x + at + u * r.step);
 #pragma unroll
             for (int u = 0; u < M; ++u) {
-                float v[V];
-                unpack<T>(raw[u], v);
+                f2_t v[V / 2];
+                unpack_pairs<T>(raw[u], v);
                 have += 1.f;
-                const float share = __fdividef(1.f, have);
+                const f2_t share = both(reciprocal(have));
 #pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const float d = v[j] - mean[j];
-                    mean[j] = fmaf(d, share, mean[j]);
-                    m2[j] = fmaf(d, v[j] - mean[j], m2[j]);
+                for (int j = 0; j < V / 2; ++j) {
+                    const f2_t d = sub2(v[j], mean[j]);
+                    mean[j] = fma2(d, share, mean[j]);
+                    m2[j] = fma2(d, sub2(v[j], mean[j]), m2[j]);
                 }
             }
         });
+        // Neighbours of a group become one in the thread, where vectors and groups end together: their counts are equal.
+        const int run = s.C % V == 0 && (D % V == 0 || V % D == 0) ? min(D, V) : 1;
         if (threadIdx.x < plan.active) {
+            float mj[V], qj[V];
 #pragma unroll
-            for (int j = 0; j < V; ++j) pairs[threadIdx.x * V + j] = make_float2(mean[j], m2[j]);
+            for (int j = 0; j < V; j += 2) {
+                unpack2(mean[j / 2], mj[j], mj[j + 1]);
+                unpack2(m2[j / 2], qj[j], qj[j + 1]);
+            }
+#pragma unroll
+            for (int w = 1; w < V; w *= 2)
+                if (run > w)
+#pragma unroll
+                    for (int j = 0; j < V; j += 2 * w) {
+                        const float d = mj[j + w] - mj[j];
+                        mj[j] = fmaf(0.5f, d, mj[j]);
+                        qj[j] += fmaf(d * d, 0.5f * w * have, qj[j + w]);
+                    }
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                if (j % run == 0) pairs[(threadIdx.x * V + j) / (unsigned)run] = make_float2(mj[j], qj[j]);
             counts[threadIdx.x] = have;
         }
         if (threadIdx.x < r.edges) {
@@ -146,10 +189,12 @@ __global__ void __launch_bounds__(THREADS) norm_rows_forward_kernel(const T *__r
         const int repeats = plan.active * V / plan.width;
         for (int g = warp; g < groups; g += warps) {
             Moments m{0.f, 0.f, 0.f};
-            for (int i = lane; i < repeats * D; i += 32) {
-                const int pp = i / D, q = r.position(pp, g * D + i - pp * D, plan.width, plan.active);
-                const float2 v = pairs[q];
-                m = merged(m, {counts[q / V], v.x, v.y});
+            const int each = D / run;
+            for (int i = lane; i < repeats * each; i += 32) {
+                const int pp = (unsigned)i / (unsigned)each;
+                const int q = r.position(pp, g * D + (i - pp * each) * run, plan.width, plan.active);
+                const float2 v = pairs[(unsigned)q / (unsigned)run];
+                m = merged(m, {counts[q / V] * run, v.x, v.y});
             }
             m = warp_merged(m);
             for (int i = 0; i < r.edges; ++i)
@@ -167,14 +212,18 @@ __global__ void __launch_bounds__(THREADS) norm_rows_forward_kernel(const T *__r
     if (STEP == NORM_WHOLE) {
         if (plan.k > 1) cluster_sync();
         else __syncthreads();
-        for (int g = threadIdx.x; g < groups; g += blockDim.x) {
+        // a lane a CTA, k lanes a group
+        for (int i0 = 0; i0 < groups * plan.k; i0 += blockDim.x) {
+            const int i = i0 + threadIdx.x, g = (unsigned)i / (unsigned)plan.k;
             Moments m{0.f, 0.f, 0.f};
-            for (int i = 0; i < plan.k; ++i) {
-                const uint32_t at = cluster_map(smem_u32(moments + 3 * g), plan.k > 1 ? i : 0);
-                if (plan.k > 1) m = merged(m, {cluster_load(at), cluster_load(at + 4), cluster_load(at + 8)});
-                else m = {moments[3 * g], moments[3 * g + 1], moments[3 * g + 2]};
+            if (g < groups) {
+                const uint32_t at = plan.k > 1 ? cluster_map(smem_u32(moments + 3 * g), i - g * plan.k) : smem_u32(moments + 3 * g);
+                m = {cluster_load(at), cluster_load(at + 4), cluster_load(at + 8)};
             }
-            results[g] = make_float2(m.mean, rsqrtf(__fdiv_rn(m.m2, m.n) + s.eps));
+            for (int o = 1; o < plan.k; o *= 2)
+                m = merged(m, {__shfl_down_sync(0xffffffffu, m.n, o), __shfl_down_sync(0xffffffffu, m.mean, o),
+                               __shfl_down_sync(0xffffffffu, m.m2, o)});
+            if (g < groups && i == g * plan.k) results[g] = make_float2(m.mean, rsqrtf(__fdiv_rn(m.m2, m.n) + s.eps));
         }
         if (plan.k > 1) cluster_sync();      // (nobody leaves while its moments are read)
         else __syncthreads();
@@ -194,15 +243,19 @@ __global__ void __launch_bounds__(THREADS) norm_rows_forward_kernel(const T *__r
         for (int g = threadIdx.x; g < groups; g += blockDim.x)
             reinterpret_cast<float2 *>(stats)[n * s.G + slab * groups + g] = results[g];
 
-    float mean[V], a[V], b[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const int c = r.count ? r.channel_of(j, plan.width) : 0, all = slab * plan.width + c;
-        const float2 st = results[c / D];
-        mean[j] = st.x;
-        a[j] = weight ? st.y * to_float(weight[all]) : st.y;
-        b[j] = bias ? to_float(bias[all]) : 0.f;
+    const Affine table{reinterpret_cast<float *>(smem + lay.pairs()), plan.width};      // (the positions have been read)
+    __syncthreads();
+    for (int c = threadIdx.x; c < plan.width; c += blockDim.x) {
+        const float2 st = results[(unsigned)c / (unsigned)D];
+        table.put(c, 0, st.x);
+        table.put(c, 1, weight ? st.y * to_float(weight[slab * plan.width + c]) : st.y);
+        table.put(c, 2, bias ? to_float(bias[slab * plan.width + c]) : 0.f);
     }
+    __syncthreads();
+    f2_t mean[V / 2], a[V / 2], b[V / 2];
+    table.get<V>(0, r, mean);
+    table.get<V>(1, r, a);
+    table.get<V>(2, r, b);
     each(r, [&](auto many, int64_t at) {
         constexpr int M = decltype(many)::value;
         uint4 raw[M];
@@ -210,19 +263,17 @@ __global__ void __launch_bounds__(THREADS) norm_rows_forward_kernel(const T *__r
         for (int u = 0; u < M; ++u) raw[u] = *reinterpret_cast<const uint4 *>(x + at + u * r.step);
 #pragma unroll
         for (int u = 0; u < M; ++u) {
-            float v[V];
-            unpack<T>(raw[u], v);
+            f2_t v[V / 2];
+            unpack_pairs<T>(raw[u], v);
 #pragma unroll
-            for (int j = 0; j < V; ++j) v[j] = activate<ACT, T>(fmaf(v[j] - mean[j], a[j], b[j]));
-            *reinterpret_cast<uint4 *>(out + at + u * r.step) = pack<T>(v);
+            for (int j = 0; j < V / 2; ++j) v[j] = activate2<ACT, T>(fma2(sub2(v[j], mean[j]), a[j], b[j]));
+            *reinterpret_cast<uint4 *>(out + at + u * r.step) = pack_pairs<T>(v);
         }
     });
     if (threadIdx.x < r.edges) {
         int c;
         const int64_t at = r.edge(threadIdx.x, s.C, c);
-        const float2 st = results[c / D];
-        const float w = weight ? st.y * to_float(weight[c]) : st.y;
-        out[at] = from_float<T>(activate<ACT, T>(fmaf(to_float(x[at]) - st.x, w, bias ? to_float(bias[c]) : 0.f)));
+        out[at] = from_float<T>(activate<ACT, T>(fmaf(to_float(x[at]) - table.at(c, 0), table.at(c, 1), table.at(c, 2))));
     }
 }
 
@@ -230,7 +281,7 @@ __global__ void __launch_bounds__(THREADS) norm_rows_forward_kernel(const T *__r
 //   S1 = sum dz, S2 = rstd * sum dz d,   A1 = sum_c weight S1 / L, A2 = sum_c weight S2 / L over the group,
 //   grad_input = a dz - rstd A1 - d rstd^2 A2.
 // `sums`: a row of C pairs (S1, S2) per (sample, rank).
-// Shared memory: positions' pairs, partial sums of the channels, channels' pairs, groups' sums (twice), edges.
+// Shared memory: positions' pairs, partial sums of the channels, channels' pairs, groups' sums (twice), edges, channels' factors.
 struct BackLayout {
     int active_v, threads, width, groups;
     __host__ __device__ size_t pairs() const { return 0; }
@@ -239,7 +290,8 @@ struct BackLayout {
     __host__ __device__ size_t sums() const { return channels() + (size_t)width * 8; }
     __host__ __device__ size_t results() const { return sums() + (size_t)groups * 8; }
     __host__ __device__ size_t edges() const { return results() + (size_t)groups * 8; }
-    __host__ __device__ size_t bytes() const { return edges() + 16 * 12; }
+    __host__ __device__ size_t affine() const { return edges() + 16 * 12; }
+    __host__ __device__ size_t bytes() const { return affine() + (size_t)width * 20; }
 };
 
 template <typename T, int ACT, int STEP, int THREADS>
@@ -255,37 +307,41 @@ __global__ void __launch_bounds__(THREADS) norm_rows_backward_kernel(const T *__
     float2 *channels = reinterpret_cast<float2 *>(smem + lay.channels()), *own = reinterpret_cast<float2 *>(smem + lay.sums());
     float2 *results = reinterpret_cast<float2 *>(smem + lay.results());
     float *edges = reinterpret_cast<float *>(smem + lay.edges());
-    const int64_t unit = blockIdx.x / plan.k, n = unit / plan.slabs;
-    const int rank = (int)(blockIdx.x - unit * plan.k), slab = (int)(unit - n * plan.slabs);
+    const unsigned index = blockIdx.x / (unsigned)plan.k, sample = index / (unsigned)plan.slabs;
+    const int64_t n = sample;
+    const int rank = (int)(blockIdx.x - index * plan.k), slab = (int)(index - sample * plan.slabs);
     const Rows<T> r(s, plan, n, slab, rank);
     grid_dependency_wait();
 
     const float2 *of_group = reinterpret_cast<const float2 *>(stats) + n * s.G + slab * groups;
-    float mean[V], a[V], b[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const int c = r.count ? r.channel_of(j, plan.width) : 0, all = slab * plan.width + c;
-        const float2 st = of_group[c / D];
-        mean[j] = st.x;
-        a[j] = weight ? st.y * to_float(weight[all]) : st.y;
-        b[j] = ACT != BC_ACT_NONE && bias ? to_float(bias[all]) : 0.f;
+    const Affine table{reinterpret_cast<float *>(smem + lay.affine()), plan.width};
+    for (int c = threadIdx.x; c < plan.width; c += blockDim.x) {
+        const float2 st = of_group[(unsigned)c / (unsigned)D];
+        table.put(c, 0, st.x);
+        table.put(c, 1, weight ? st.y * to_float(weight[slab * plan.width + c]) : st.y);
+        table.put(c, 2, ACT != BC_ACT_NONE && bias ? to_float(bias[slab * plan.width + c]) : 0.f);
     }
-    auto both = [&](auto &&f) {      // U vectors of x and of grad at a time
+    __syncthreads();
+    f2_t mean[V / 2], a[V / 2], b[V / 2];
+    table.get<V>(0, r, mean);
+    table.get<V>(1, r, a);
+    table.get<V>(2, r, b);
+    auto each_both = [&](auto &&f) {      // U vectors of x and of grad at a time
         int64_t at = r.first;
         int i = 0;
         for (; i + U <= r.count; i += U, at += U * r.step) f(std::integral_constant<int, U>(), at);
         for (; i < r.count; ++i, at += r.step) f(std::integral_constant<int, 1>(), at);
     };
     auto edge_slope = [&](int64_t at, int c, float &d) {      // dz of a single value
-        const float2 st = of_group[c / D];
-        const float w = weight ? st.y * to_float(weight[c]) : st.y;
-        d = to_float(x[at]) - st.x;
-        return to_float(grad[at]) * slope<ACT, T>(fmaf(d, w, ACT != BC_ACT_NONE && bias ? to_float(bias[c]) : 0.f));
+        d = to_float(x[at]) - table.at(c, 0);
+        return times_slope<ACT, T>(to_float(grad[at]), fmaf(d, table.at(c, 1), table.at(c, 2)));
     };
 
     if (STEP != NORM_RESULTS) {
-        float s1[V] = {}, s2[V] = {};
-        both([&](auto many, int64_t at) {
+        f2_t s1[V / 2], s2[V / 2];
+#pragma unroll
+        for (int j = 0; j < V / 2; ++j) s1[j] = s2[j] = both(0.f);
+        each_both([&](auto many, int64_t at) {
             constexpr int M = decltype(many)::value;
             uint4 rx[M], rg[M];
 #pragma unroll
@@ -295,20 +351,25 @@ __global__ void __launch_bounds__(THREADS) norm_rows_backward_kernel(const T *__
             }
 #pragma unroll
             for (int u = 0; u < M; ++u) {
-                float v[V], g[V];
-                unpack<T>(rx[u], v);
-                unpack<T>(rg[u], g);
+                f2_t v[V / 2], g[V / 2];
+                unpack_pairs<T>(rx[u], v);
+                unpack_pairs<T>(rg[u], g);
 #pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const float d = v[j] - mean[j], dz = g[j] * slope<ACT, T>(fmaf(d, a[j], b[j]));
-                    s1[j] += dz;
-                    s2[j] = fmaf(dz, d, s2[j]);
+                for (int j = 0; j < V / 2; ++j) {
+                    const f2_t d = sub2(v[j], mean[j]), dz = times_slope2<ACT, T>(g[j], fma2(d, a[j], b[j]));
+                    s1[j] = add2(s1[j], dz);
+                    s2[j] = fma2(dz, d, s2[j]);
                 }
             }
         });
         if (threadIdx.x < plan.active)
 #pragma unroll
-            for (int j = 0; j < V; ++j) pairs[threadIdx.x * V + j] = make_float2(s1[j], s2[j]);
+            for (int j = 0; j < V; j += 2) {
+                float p, q, u, v;
+                unpack2(s1[j / 2], p, q);
+                unpack2(s2[j / 2], u, v);
+                *reinterpret_cast<float4 *>(pairs + threadIdx.x * V + j) = make_float4(p, u, q, v);
+            }
         if (threadIdx.x < r.edges) {
             int c;
             float d;
@@ -363,17 +424,18 @@ __global__ void __launch_bounds__(THREADS) norm_rows_backward_kernel(const T *__
         if (plan.k > 1) cluster_sync();
         else __syncthreads();
         const float count = (float)D * (float)s.P;
-        for (int g = threadIdx.x; g < groups; g += blockDim.x) {
-            float2 t = own[g];
-            if (plan.k > 1) {
-                t = make_float2(0.f, 0.f);
-                for (int i = 0; i < plan.k; ++i) {
-                    const uint32_t at = cluster_map(smem_u32(own + g), i);
-                    t.x += cluster_load(at);
-                    t.y += cluster_load(at + 4);
-                }
+        for (int i0 = 0; i0 < groups * plan.k; i0 += blockDim.x) {      // a lane a CTA, k lanes a group
+            const int i = i0 + threadIdx.x, g = (unsigned)i / (unsigned)plan.k;
+            float2 t = make_float2(0.f, 0.f);
+            if (g < groups) {
+                const uint32_t at = plan.k > 1 ? cluster_map(smem_u32(own + g), i - g * plan.k) : smem_u32(own + g);
+                t = make_float2(cluster_load(at), cluster_load(at + 4));
             }
-            results[g] = make_float2(__fdiv_rn(t.x, count), __fdiv_rn(t.y, count));
+            for (int o = 1; o < plan.k; o *= 2) {
+                t.x += __shfl_down_sync(0xffffffffu, t.x, o);
+                t.y += __shfl_down_sync(0xffffffffu, t.y, o);
+            }
+            if (g < groups && i == g * plan.k) results[g] = make_float2(__fdiv_rn(t.x, count), __fdiv_rn(t.y, count));
         }
         if (plan.k > 1) cluster_sync();
         else __syncthreads();
@@ -396,15 +458,17 @@ __global__ void __launch_bounds__(THREADS) norm_rows_backward_kernel(const T *__
         __syncthreads();
     }
 
-    float k1[V], k2[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const int g = (r.count ? r.channel_of(j, plan.width) : 0) / D;
+    for (int c = threadIdx.x; c < plan.width; c += blockDim.x) {
+        const int g = (unsigned)c / (unsigned)D;
         const float rstd = of_group[g].y;
-        k1[j] = rstd * results[g].x;
-        k2[j] = rstd * rstd * results[g].y;
+        table.put(c, 3, -rstd * results[g].x);
+        table.put(c, 4, -rstd * rstd * results[g].y);
     }
-    both([&](auto many, int64_t at) {
+    __syncthreads();
+    f2_t k1[V / 2], k2[V / 2];
+    table.get<V>(3, r, k1);
+    table.get<V>(4, r, k2);
+    each_both([&](auto many, int64_t at) {
         constexpr int M = decltype(many)::value;
         uint4 rx[M], rg[M];
 #pragma unroll
@@ -414,24 +478,23 @@ __global__ void __launch_bounds__(THREADS) norm_rows_backward_kernel(const T *__
         }
 #pragma unroll
         for (int u = 0; u < M; ++u) {
-            float v[V], g[V];
-            unpack<T>(rx[u], v);
-            unpack<T>(rg[u], g);
+            f2_t v[V / 2], g[V / 2];
+            unpack_pairs<T>(rx[u], v);
+            unpack_pairs<T>(rg[u], g);
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const float d = v[j] - mean[j], dz = g[j] * slope<ACT, T>(fmaf(d, a[j], b[j]));
-                v[j] = fmaf(-d, k2[j], fmaf(a[j], dz, -k1[j]));
+            for (int j = 0; j < V / 2; ++j) {
+                const f2_t d = sub2(v[j], mean[j]), dz = times_slope2<ACT, T>(g[j], fma2(d, a[j], b[j]));
+                v[j] = fma2(d, k2[j], fma2(a[j], dz, k1[j]));
             }
-            *reinterpret_cast<uint4 *>(grad_input + at + u * r.step) = pack<T>(v);
+            *reinterpret_cast<uint4 *>(grad_input + at + u * r.step) = pack_pairs<T>(v);
         }
     });
     if (threadIdx.x < r.edges) {
         int c;
         float d;
         const int64_t at = r.edge(threadIdx.x, s.C, c);
-        const float dz = edge_slope(at, c, d), rstd = of_group[c / D].y;
-        const float w = weight ? rstd * to_float(weight[c]) : rstd;
-        grad_input[at] = from_float<T>(fmaf(-d, rstd * rstd * results[c / D].y, fmaf(w, dz, -rstd * results[c / D].x)));
+        const float dz = edge_slope(at, c, d);
+        grad_input[at] = from_float<T>(fmaf(d, table.at(c, 4), fmaf(table.at(c, 1), dz, table.at(c, 3))));
     }
 }
 
@@ -464,15 +527,16 @@ bool plan_rows(const NormShape &s, NormRows *plan)
     r.width = s.C;
     r.slabs = 1;
     const int64_t sample = s.P * s.C * size;
-    // Few samples: parts of the channels as units of their own, down to two sectors of 32 bytes a pixel.
-    while ((s.N * r.slabs * kNormCluster < kNormFill || sample / r.slabs > kNormCluster * kNormSlice) && r.width % 2 == 0 &&
-           r.width / 2 % D == 0 && r.width / 2 * size % 64 == 0) {
+    // Parts of the channels as units of their own: down to 64 bytes a pixel where the GPU would not fill, to 128 where slices
+    // would be long ((16,128,64,128) bf16: forward 37 us at 64 bytes, 33 at 128; (1,64,256,512) f32 the other way round, 17 and 19).
+    while (r.width % 2 == 0 && r.width / 2 % D == 0 && r.width / 2 * size % 64 == 0 &&
+           (s.N * r.slabs * kNormCluster < 148 || (sample / r.slabs > kNormCluster * kNormSlice && r.width / 2 * size % 128 == 0))) {
         r.width /= 2;
         r.slabs *= 2;
     }
     const int period = r.slabs > 1 ? r.width / V : s.C / gcd(s.C, V);      // vectors after which the places repeat
     if (period > 1024) return false;
-    r.threads = period > 512 ? 1024 : 512;
+    r.threads = period > 512 ? 1024 : period > 256 ? 512 : 256;
     const int64_t units = (int64_t)s.N * r.slabs, bytes = sample / r.slabs;
     // slices that fill the GPU, of a vector a thread at least
     int64_t k = norm_ceil(bytes, kNormSlice);
@@ -492,7 +556,7 @@ bool plan_rows(const NormShape &s, NormRows *plan)
     r.k = (int)k;
     *plan = r;
     const int groups = r.width / D;
-    return std::max(Layout{r.active * V, r.threads, groups}.bytes(), BackLayout{r.active * V, r.threads, r.width, groups}.bytes()) <= kMostShared;
+    return std::max(Layout{r.active * V, r.threads, r.width, groups}.bytes(), BackLayout{r.active * V, r.threads, r.width, groups}.bytes()) <= kMostShared;
 }
 
 size_t rows_sums_bytes(const NormShape &s, const NormRows &plan, bool backward)
@@ -507,7 +571,7 @@ int launch_norm_rows_forward(const NormShape &s, const NormRows &plan, const voi
     return dispatch(s, [&](auto t, auto act) {
         using T = decltype(t);
         const int64_t grid = (int64_t)s.N * plan.slabs * plan.k;
-        const size_t smem = Layout{plan.active * kVec<T>, plan.threads, plan.width / (s.C / s.G)}.bytes();
+        const size_t smem = Layout{plan.active * kVec<T>, plan.threads, plan.width, plan.width / (s.C / s.G)}.bytes();
         auto go = [&](auto kernel, int cluster) {
             return launch(KID_NORM_FORWARD, "norm_rows_forward_kernel", kernel, grid, plan.threads, smem, cluster, stream, (const T *)x,
                           (const T *)weight, (const T *)bias, (T *)out, stats, (float *)ws, s, plan);

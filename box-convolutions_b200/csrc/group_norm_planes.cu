@@ -20,12 +20,12 @@ struct Piece {
     int channel;              // of the unit
     __device__ __forceinline__ Piece(const NormShape &s, const NormPlanes &plan, int64_t first_plane, int piece)
     {
-        channel = piece / plan.chunks;
+        channel = (unsigned)piece / (unsigned)plan.chunks;
         const int64_t from = (int64_t)(piece - channel * plan.chunks) * plan.chunk;
         a = (first_plane + channel) * s.P + from;
         b = a + min((int64_t)plan.chunk, s.P - from);
-        v0 = min((a + V - 1) / V * V, b);
-        v1 = max(b / V * V, v0);
+        v0 = min((a + V - 1) & ~(int64_t)(V - 1), b);
+        v1 = max(b & ~(int64_t)(V - 1), v0);
     }
     // The lane's single value, or -1.
     __device__ __forceinline__ int64_t edge(int lane) const
@@ -53,8 +53,9 @@ __global__ void __launch_bounds__(512, 2) norm_planes_forward_kernel(const T *__
     __shared__ float warp_moments[16][3], own[3];
     __shared__ float2 result;
     const int D = s.C / s.G, warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t unit = blockIdx.x / plan.k, first_plane = unit * D;
-    const int rank = (int)(blockIdx.x - unit * plan.k);
+    const unsigned index = blockIdx.x / (unsigned)plan.k;
+    const int64_t unit = index, first_plane = unit * D;
+    const int rank = (int)(blockIdx.x - index * plan.k);
     const int begin = rank * plan.per, end = min(D * plan.chunks, begin + plan.per);
     grid_dependency_wait();
 
@@ -69,14 +70,21 @@ __global__ void __launch_bounds__(512, 2) norm_planes_forward_kernel(const T *__
                 for (int u = 0; u < M; ++u) raw[u] = *reinterpret_cast<const uint4 *>(x + at + u * 32 * V);
 #pragma unroll
                 for (int u = 0; u < M; ++u) {
-                    float v[V], mean = 0.f, m2 = 0.f;
-                    unpack<T>(raw[u], v);
+                    f2_t v[V / 2], sum, squares = both(0.f);
+                    float a, b;
+                    unpack_pairs<T>(raw[u], v);
+                    sum = v[0];
 #pragma unroll
-                    for (int j = 0; j < V; ++j) mean += v[j];
-                    mean *= 1.f / V;
+                    for (int j = 1; j < V / 2; ++j) sum = add2(sum, v[j]);
+                    unpack2(sum, a, b);
+                    const float mean = (a + b) * (1.f / V);
 #pragma unroll
-                    for (int j = 0; j < V; ++j) m2 = fmaf(v[j] - mean, v[j] - mean, m2);
-                    m = merged(m, {(float)V, mean, m2});
+                    for (int j = 0; j < V / 2; ++j) {
+                        const f2_t d = sub2(v[j], both(mean));
+                        squares = fma2(d, d, squares);
+                    }
+                    unpack2(squares, a, b);
+                    m = merged(m, {(float)V, mean, a + b});
                 }
             });
             const int64_t at = piece.edge(lane);
@@ -127,7 +135,7 @@ __global__ void __launch_bounds__(512, 2) norm_planes_forward_kernel(const T *__
     }
     const float mean = result.x, rstd = result.y;
     if (stats && rank == 0 && threadIdx.x == 0) reinterpret_cast<float2 *>(stats)[unit] = make_float2(mean, rstd);
-    const int c0 = (int)(unit % s.G) * D;
+    const int c0 = (int)(index % (unsigned)s.G) * D;
     for (int i = begin + warp; i < end; i += warps) {
         const Piece<T> piece(s, plan, first_plane, i);
         const float a = weight ? rstd * to_float(weight[c0 + piece.channel]) : rstd, b = bias ? to_float(bias[c0 + piece.channel]) : 0.f;
@@ -138,11 +146,11 @@ __global__ void __launch_bounds__(512, 2) norm_planes_forward_kernel(const T *__
             for (int u = 0; u < M; ++u) raw[u] = *reinterpret_cast<const uint4 *>(x + at + u * 32 * V);
 #pragma unroll
             for (int u = 0; u < M; ++u) {
-                float v[V];
-                unpack<T>(raw[u], v);
+                f2_t v[V / 2];
+                unpack_pairs<T>(raw[u], v);
 #pragma unroll
-                for (int j = 0; j < V; ++j) v[j] = activate<ACT, T>(fmaf(v[j] - mean, a, b));
-                *reinterpret_cast<uint4 *>(out + at + u * 32 * V) = pack<T>(v);
+                for (int j = 0; j < V / 2; ++j) v[j] = activate2<ACT, T>(fma2(sub2(v[j], both(mean)), both(a), both(b)));
+                *reinterpret_cast<uint4 *>(out + at + u * 32 * V) = pack_pairs<T>(v);
             }
         });
         const int64_t at = piece.edge(lane);
@@ -161,8 +169,9 @@ __global__ void __launch_bounds__(512, 2) norm_planes_backward_kernel(const T *_
     __shared__ float2 pieces[kMostPieces];
     __shared__ float2 of_warp[16], own, result;
     const int D = s.C / s.G, warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t unit = blockIdx.x / plan.k, first_plane = unit * D, n = unit / s.G;
-    const int rank = (int)(blockIdx.x - unit * plan.k), c0 = (int)(unit - n * s.G) * D;
+    const unsigned index = blockIdx.x / (unsigned)plan.k, sample = index / (unsigned)s.G;
+    const int64_t unit = index, first_plane = unit * D, n = sample;
+    const int rank = (int)(blockIdx.x - index * plan.k), c0 = (int)(index - sample * s.G) * D;
     const int begin = rank * plan.per, end = min(D * plan.chunks, begin + plan.per);
     const float count = (float)D * (float)s.P;
     grid_dependency_wait();
@@ -175,7 +184,8 @@ __global__ void __launch_bounds__(512, 2) norm_planes_backward_kernel(const T *_
     if (STEP != NORM_RESULTS) {
         for (int i = begin + warp; i < end; i += warps) {
             const Piece<T> piece(s, plan, first_plane, i);
-            float a, b, s1 = 0.f, s2 = 0.f;
+            float a, b;
+            f2_t p1 = both(0.f), p2 = both(0.f);
             affine(piece.channel, a, b);
             piece.template each<U>(lane, [&](auto many, int64_t at) {
                 constexpr int M = decltype(many)::value;
@@ -187,20 +197,25 @@ __global__ void __launch_bounds__(512, 2) norm_planes_backward_kernel(const T *_
                 }
 #pragma unroll
                 for (int u = 0; u < M; ++u) {
-                    float v[V], g[V];
-                    unpack<T>(rx[u], v);
-                    unpack<T>(rg[u], g);
+                    f2_t v[V / 2], g[V / 2];
+                    unpack_pairs<T>(rx[u], v);
+                    unpack_pairs<T>(rg[u], g);
 #pragma unroll
-                    for (int j = 0; j < V; ++j) {
-                        const float d = v[j] - mean, dz = g[j] * slope<ACT, T>(fmaf(d, a, b));
-                        s1 += dz;
-                        s2 = fmaf(dz, d, s2);
+                    for (int j = 0; j < V / 2; ++j) {
+                        const f2_t d = sub2(v[j], both(mean)), dz = times_slope2<ACT, T>(g[j], fma2(d, both(a), both(b)));
+                        p1 = add2(p1, dz);
+                        p2 = fma2(dz, d, p2);
                     }
                 }
             });
+            float s1, s2, other;
+            unpack2(p1, s1, other);
+            s1 += other;
+            unpack2(p2, s2, other);
+            s2 += other;
             const int64_t at = piece.edge(lane);
             if (at >= 0) {
-                const float d = to_float(x[at]) - mean, dz = to_float(grad[at]) * slope<ACT, T>(fmaf(d, a, b));
+                const float d = to_float(x[at]) - mean, dz = times_slope<ACT, T>(to_float(grad[at]), fmaf(d, a, b));
                 s1 += dz;
                 s2 = fmaf(dz, d, s2);
             }
@@ -287,20 +302,20 @@ __global__ void __launch_bounds__(512, 2) norm_planes_backward_kernel(const T *_
             }
 #pragma unroll
             for (int u = 0; u < M; ++u) {
-                float v[V], g[V];
-                unpack<T>(rx[u], v);
-                unpack<T>(rg[u], g);
+                f2_t v[V / 2], g[V / 2];
+                unpack_pairs<T>(rx[u], v);
+                unpack_pairs<T>(rg[u], g);
 #pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const float d = v[j] - mean, dz = g[j] * slope<ACT, T>(fmaf(d, a, b));
-                    v[j] = fmaf(-d, k2, fmaf(a, dz, -k1));
+                for (int j = 0; j < V / 2; ++j) {
+                    const f2_t d = sub2(v[j], both(mean)), dz = times_slope2<ACT, T>(g[j], fma2(d, both(a), both(b)));
+                    v[j] = fma2(d, both(-k2), fma2(both(a), dz, both(-k1)));
                 }
-                *reinterpret_cast<uint4 *>(grad_input + at + u * 32 * V) = pack<T>(v);
+                *reinterpret_cast<uint4 *>(grad_input + at + u * 32 * V) = pack_pairs<T>(v);
             }
         });
         const int64_t at = piece.edge(lane);
         if (at >= 0) {
-            const float d = to_float(x[at]) - mean, dz = to_float(grad[at]) * slope<ACT, T>(fmaf(d, a, b));
+            const float d = to_float(x[at]) - mean, dz = times_slope<ACT, T>(to_float(grad[at]), fmaf(d, a, b));
             grad_input[at] = from_float<T>(fmaf(-d, k2, fmaf(a, dz, -k1)));
         }
     }

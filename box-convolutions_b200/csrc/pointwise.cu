@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(kThreads) pointwise_kernel(Product q)
             const int64_t at = base + (LAST ? (int64_t)m * q.Cn + n : n * q.P + m);
             float z = acc[i][j] + b;
             if (MODE != INPUT && residual) z += to_float(residual[at]);
-            out[at] = from_float<T>(MODE == FORWARD ? activate<ACT, T>(z) : MODE == SLOPE ? to_float(grad[at]) * slope<ACT, T>(z) : z);
+            out[at] = from_float<T>(MODE == FORWARD ? activate<ACT, T>(z) : MODE == SLOPE ? times_slope<ACT, T>(to_float(grad[at]), z) : z);
         }
     }
 }

@@ -387,15 +387,20 @@ def test_not_a_number_stays_where_it_belongs(bc):
         for last in (False, True):
             x = maps(torch.Generator(device="cuda").manual_seed(1), (3, 24, 9, 24), dtype, last)
             w = torch.randn(40, 24, device="cuda").to(dtype)
-            clean = bc.pointwise_conv2d(x, w, activation="relu")
-            for bad in (float("nan"), float("inf"), -float("inf")):
-                y = x.clone()
-                y[1, 3, 4, 5] = bad
-                out = bc.pointwise_conv2d(y, w, activation="relu")
-                touched = torch.zeros_like(out, dtype=torch.bool)
-                touched[1, :, 4, 5] = True
-                assert torch.equal(out[~touched], clean[~touched])
-                assert out[touched].isnan().all() if bad != bad else (out[touched].isinf() | (out[touched] == 0)).all()
+            for act in ("relu", "silu", "gelu"):
+                clean = bc.pointwise_conv2d(x, w, activation=act)
+                for bad in (float("nan"), float("inf"), -float("inf")):
+                    y = x.clone()
+                    y[1, 3, 4, 5] = bad
+                    out = bc.pointwise_conv2d(y, w, activation=act)
+                    touched = torch.zeros_like(out, dtype=torch.bool)
+                    touched[1, :, 4, 5] = True
+                    assert torch.equal(out[~touched], clean[~touched])
+                    if bad != bad:
+                        assert out[touched].isnan().all()
+                    else:
+                        want = act64(bad * torch.sign(w[:, 3]).double(), act)
+                        assert torch.equal(out[touched].double().nan_to_num(-1, posinf=1), want.nan_to_num(-1, posinf=1))
             clean = bc.group_norm(x, 6)
             for bad in (float("nan"), float("inf")):
                 y = x.clone()
