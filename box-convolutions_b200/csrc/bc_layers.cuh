@@ -250,6 +250,18 @@ struct PointwiseShape {
     bool last;
     int io_kind, act;
 };
+// The products on the tensor cores (pointwise_mma.cu): 16-bit types, rows and arrays on 16 bytes.
+bool pointwise_mma_suits(const PointwiseShape &s, bool input);
+bool pointwise_mma_aligned(const void *a, const void *b, const void *c = nullptr, const void *d = nullptr, const void *e = nullptr);
+int launch_pointwise_mma_forward(const PointwiseShape &s, const void *x, const void *weight, const void *bias, const void *residual,
+                                 void *out, cudaStream_t stream);
+// sums: pointwise_mma_sums_rows() rows of Co floats, sums of dz to be added, or null
+int pointwise_mma_sums_rows(const PointwiseShape &s);
+int launch_pointwise_mma_slope(const PointwiseShape &s, const void *x, const void *weight, const void *bias, const void *residual,
+                               const void *grad, void *dz, float *sums, cudaStream_t stream);
+int launch_pointwise_mma_input(const PointwiseShape &s, const void *dz, const void *weight, void *grad_input, cudaStream_t stream);
+int read_wait_timeouts_mma(int *count);
+
 size_t pointwise_workspace(const PointwiseShape &s, int need_mask);
 int launch_pointwise_forward(const PointwiseShape &s, const void *x, const void *weight, const void *bias, const void *residual, void *out,
                              cudaStream_t stream);

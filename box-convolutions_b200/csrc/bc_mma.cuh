@@ -1,0 +1,134 @@
+// tcgen05 products of 16-bit operands: shared-memory descriptors, issue, completion; tensor maps.
+//
+// Operands lie in shared memory as TMA's 128-byte swizzle leaves them.  K-major (k runs along memory): rows of 64 k, 8 rows of
+// 128 bytes a swizzle atom.  MN-major (the other index runs along memory): blocks of 64 m or n, a row of 128 bytes for each k.
+#pragma once
+#include <cuda.h>
+
+#include "bc_layers.cuh"
+#include "bc_tile_io.cuh"
+#include "bc_tmem.cuh"
+
+namespace bc {
+
+namespace {
+
+constexpr uint32_t kBlockBytes = 64 * 128;      // an MN-major block of 64 k
+
+// 14 bits each: start, leading and stride byte offsets in units of 16; version 1; 128-byte swizzle.
+__device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t leading, uint32_t stride)
+{
+    return (uint64_t)((addr & 0x3ffff) >> 4) | (uint64_t)(leading >> 4) << 16 | (uint64_t)(stride >> 4) << 32 | (uint64_t)1 << 46 |
+           (uint64_t)2 << 61;
+}
+// K-major: 16 k are 32 bytes on within the atoms' rows.
+__device__ __forceinline__ uint64_t k_major(uint32_t addr, int k) { return operand(addr + 2 * k, 16, 1024); }
+// MN-major: blocks `block` bytes apart; 8 k are an atom of 1024 bytes.
+__device__ __forceinline__ uint64_t mn_major(uint32_t addr, int k, uint32_t block) { return operand(addr + 128 * k, block, 1024); }
+
+// 16-bit operands of one type, float accumulators, M 128.
+__host__ __device__ inline uint32_t mma_instruction(bool bf16, bool a_mn, bool b_mn, int n)
+{
+    return 1u << 4 | (bf16 ? 1u << 7 | 1u << 10 : 0u) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 |
+           (uint32_t)(128 >> 4) << 24;
+}
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t instruction, bool add)
+{
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(instruction), "r"((uint32_t)add) : "memory");
+}
+// Arrives once everything issued so far by this thread is done (and has been read).
+__device__ __forceinline__ void mma_commit(uint32_t mbar)
+{
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(mbar) : "memory");
+}
+__device__ __forceinline__ void mbar_expect(uint32_t mbar, uint32_t bytes)
+{
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(mbar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t mbar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(mbar) : "memory"); }
+__device__ __forceinline__ void tile_load(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t mbar)
+{
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(mbar) : "memory");
+}
+__device__ __forceinline__ void tile_load(uint32_t dst, const CUtensorMap *map, int x, int y, int z, uint32_t mbar)
+{
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(mbar) : "memory");
+}
+__device__ __forceinline__ void map_prefetch(const CUtensorMap *map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
+
+// 32 accumulators of the warp's lanes.
+__device__ __forceinline__ void tmem_load32(uint32_t at, float (&v)[32])
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,"
+                 "%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n tcgen05.wait::ld.sync.aligned;"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]),
+                   "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]),
+                   "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]),
+                   "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+                 : "r"(at) : "memory");
+}
+
+// A wait whose expiry ends all further ones of the thread: a lost arrival is counted (bc_wait_timeouts), and nothing hangs.
+struct Waiter {
+    bool lost = false;
+    __device__ __forceinline__ bool operator()(uint32_t mbar, uint32_t parity)
+    {
+        if (lost) return false;
+        if (mbar_wait(mbar, parity)) return true;
+        atomicAdd(&g_wait_timeouts, 1);
+        lost = true;
+        return false;
+    }
+};
+// Before a CTA that has lost an arrival leaves: time for its copies in flight, far more than any takes.
+__device__ __forceinline__ void let_copies_land()
+{
+    for (const long long t0 = clock64(); clock64() - t0 < 20000000LL;) __nanosleep(1000);
+}
+
+}  // namespace
+
+// Tensor map of 16-bit values, 128-byte swizzle, zeros outside: `rank` sizes and boxes, innermost first, strides in values of
+// the second dimension on.
+inline int make_map(CUtensorMap *map, const void *base, bool bf16, int rank, const uint64_t *sizes, const uint64_t *strides,
+                    const uint32_t *box)
+{
+    typedef CUresult (*Encode)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                               const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                               CUtensorMapFloatOOBfill);
+    static const Encode encode = [] {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess) {
+            (void)cudaGetLastError();
+            f = nullptr;
+        }
+        return (Encode)f;
+    }();
+    if (!encode) return cuda_failed(cudaErrorNotSupported, "cuTensorMapEncodeTiled");
+    cuuint64_t bytes[4] = {};
+    const cuuint32_t steps[4] = {1, 1, 1, 1};
+    for (int i = 0; i + 1 < rank; ++i) bytes[i] = 2 * strides[i];
+    auto call = [&] {
+        return encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, const_cast<void *>(base), sizes, bytes,
+                      box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    CUresult r = call();
+    if (r != CUDA_SUCCESS) {
+        // A thread whose first call into CUDA this is (autograd's, say) has a device but no context yet, which the driver's
+        // function asks for and the runtime's provide.
+        int device = 0;
+        cudaError_t e = cudaGetDevice(&device);
+        if (e == cudaSuccess) e = cudaSetDevice(device);
+        if (e != cudaSuccess) return cuda_failed(e, "cuTensorMapEncodeTiled");
+        r = call();
+    }
+    return r == CUDA_SUCCESS ? BC_OK : cuda_failed(cudaErrorInvalidValue, "cuTensorMapEncodeTiled");
+}
+
+}  // namespace bc

@@ -8,7 +8,7 @@
 #include <vector>
 #include <string.h>
 
-#include "bc_common.cuh"
+#include "bc_layers.cuh"
 
 namespace bc {
 
@@ -738,7 +738,11 @@ uint64_t bc_launch_count(void) { return g_launches.load(); }
 int bc_wait_timeouts(int *count)
 {
     if (!count) return BC_ERR_NULL_POINTER;
-    return read_wait_timeouts(count);
+    int mma = 0;
+    if (const int e = read_wait_timeouts_mma(&mma)) return e;
+    const int e = read_wait_timeouts(count);
+    if (!e) *count += mma;
+    return e;
 }
 
 int bc_profile_start(int capacity)
@@ -807,6 +811,8 @@ const char *bc_kernel_name(int kernel_id)
         case KID_POINTWISE: return "pointwise_kernel";
         case KID_POINTWISE_WEIGHT: return "pointwise_weight_kernel";
         case KID_POINTWISE_FINISH: return "pointwise_finish_kernel";
+        case KID_POINTWISE_MMA: return "pointwise_mma_kernel";
+        case KID_POINTWISE_WEIGHT_MMA: return "pointwise_weight_mma_kernel";
         case KID_NORM_FORWARD: return "norm_forward_kernel";
         case KID_NORM_BACKWARD: return "norm_backward_kernel";
         case KID_NORM_FINISH: return "norm_finish_kernel";

@@ -194,18 +194,32 @@ __global__ void __launch_bounds__(kThreads) pointwise_weight_kernel(WeightProduc
     if (q.sums && i0 == 0 && tid < kBO && o0 + tid < q.Co) partial[(int64_t)q.Co * q.Ci + o0 + tid] = sum;
 }
 
-// The splits' sums, added in order, rounded once.
+// Rows of partial sums, added in a fixed order, rounded once: `count` columns, `stride` floats from row to row.
+struct Partials {
+    const float *from;
+    int64_t stride, count;
+    int rows;
+    void *to;
+};
+constexpr int kFinishRows = 8;
+// A lane a column; eight rows at a time, then those eight.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) pointwise_finish_kernel(const float *__restrict__ partial, int splits, int64_t weights, int Co,
-                                                                    T *__restrict__ grad_weight, T *__restrict__ grad_bias)
+__global__ void __launch_bounds__(32 * kFinishRows) pointwise_finish_kernel(Partials weights, Partials sums, unsigned blocks)
 {
-    const int64_t e = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    __shared__ float part[kFinishRows][32];
+    const Partials &q = blockIdx.x < blocks ? weights : sums;
+    const int64_t e = (int64_t)(blockIdx.x < blocks ? blockIdx.x : blockIdx.x - blocks) * 32 + threadIdx.x;
     grid_dependency_wait();
-    if (e >= weights + Co || (e < weights ? !grad_weight : !grad_bias)) return;
     float v = 0.f;
-    for (int s = 0; s < splits; ++s) v += partial[s * (weights + Co) + e];
-    if (e < weights) grad_weight[e] = from_float<T>(v);
-    else grad_bias[e - weights] = from_float<T>(v);
+    if (e < q.count) {
+#pragma unroll 8
+        for (int i = threadIdx.y; i < q.rows; i += kFinishRows) v += q.from[i * q.stride + e];
+    }
+    part[threadIdx.y][threadIdx.x] = v;
+    __syncthreads();
+    if (threadIdx.y || e >= q.count) return;
+    for (int i = 1; i < kFinishRows; ++i) v += part[i][threadIdx.x];
+    static_cast<T *>(q.to)[e] = from_float<T>(v);
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -257,6 +271,7 @@ size_t partial_bytes(const PointwiseShape &s)
 {
     return align_up((size_t)splits_of(s).splits * ((size_t)s.Co * s.Ci + s.Co) * sizeof(float));
 }
+size_t sums_bytes(const PointwiseShape &s) { return align_up((size_t)pointwise_mma_sums_rows(s) * s.Co * sizeof(float)); }
 // dz in memory, where it is neither grad_output itself nor asked for.
 bool own_dz(const PointwiseShape &s, int need_mask) { return s.act != BC_ACT_NONE && !(need_mask & BC_NEED_PW_RESIDUAL); }
 
@@ -265,6 +280,8 @@ bool own_dz(const PointwiseShape &s, int need_mask) { return s.act != BC_ACT_NON
 int launch_pointwise_forward(const PointwiseShape &s, const void *x, const void *weight, const void *bias, const void *residual, void *out,
                              cudaStream_t stream)
 {
+    if (pointwise_mma_suits(s, false) && pointwise_mma_aligned(x, weight, residual, out))
+        return launch_pointwise_mma_forward(s, x, weight, bias, residual, out, stream);
     return launch_product<FORWARD>(s, {x, weight, bias, residual, nullptr, out, s.Ci, s.Co, s.Ci, 1}, stream);
 }
 
@@ -272,6 +289,7 @@ size_t pointwise_workspace(const PointwiseShape &s, int need_mask)
 {
     size_t bytes = own_dz(s, need_mask) ? align_up((size_t)io_size(s.io_kind) * s.N * s.Co * s.P) : 0;
     if (need_mask & (BC_NEED_PW_WEIGHT | BC_NEED_PW_BIAS)) bytes += partial_bytes(s);
+    if ((need_mask & BC_NEED_PW_BIAS) && s.act != BC_ACT_NONE && pointwise_mma_suits(s, false)) bytes += sums_bytes(s);
     return bytes;
 }
 
@@ -279,38 +297,70 @@ int launch_pointwise_backward(const PointwiseShape &s, const void *x, const void
                               const void *grad, int need_mask, void *grad_input, void *grad_weight, void *grad_bias,
                               void *grad_residual, void *ws, cudaStream_t stream)
 {
+    char *free_ws = static_cast<char *>(ws);
+    auto take = [&](size_t bytes) {
+        void *p = free_ws;
+        free_ws += bytes;
+        return p;
+    };
+    const bool want_weight = need_mask & BC_NEED_PW_WEIGHT, want_bias = need_mask & BC_NEED_PW_BIAS;
     const void *dz = grad;
-    float *partial = static_cast<float *>(ws);
+    float *sums = nullptr;      // of dz as it was before its rounding
     if (s.act != BC_ACT_NONE) {
-        void *to = grad_residual;
-        if (own_dz(s, need_mask)) {
-            to = ws;
-            partial = reinterpret_cast<float *>(static_cast<char *>(ws) + align_up((size_t)io_size(s.io_kind) * s.N * s.Co * s.P));
+        void *to = own_dz(s, need_mask) ? take(align_up((size_t)io_size(s.io_kind) * s.N * s.Co * s.P)) : grad_residual;
+        int e;
+        if (pointwise_mma_suits(s, false) && pointwise_mma_aligned(x, weight, residual, grad, to)) {
+            if (want_bias) sums = static_cast<float *>(take(sums_bytes(s)));
+            e = launch_pointwise_mma_slope(s, x, weight, bias, residual, grad, to, sums, stream);
+        } else {
+            e = launch_product<SLOPE>(s, {x, weight, bias, residual, grad, to, s.Ci, s.Co, s.Ci, 1}, stream);
         }
-        if (const int e = launch_product<SLOPE>(s, {x, weight, bias, residual, grad, to, s.Ci, s.Co, s.Ci, 1}, stream)) return e;
+        if (e) return e;
         dz = to;
     }
-    if (need_mask & BC_NEED_PW_INPUT)
-        if (const int e = launch_product<INPUT>(s, {dz, weight, nullptr, nullptr, nullptr, grad_input, s.Co, s.Ci, 1, s.Ci}, stream)) return e;
-    if (!(need_mask & (BC_NEED_PW_WEIGHT | BC_NEED_PW_BIAS))) return BC_OK;
-    const Splits v = splits_of(s);
-    WeightProduct q{dz, x, partial, s.last ? 1 : s.N, s.Ci, s.Co, s.last ? s.N * s.P : s.P, (int)ceil_div(s.Co, kBO),
-                    (int)ceil_div(s.Ci ? s.Ci : 1, kBI), v.chunk, v.chunks, v.per, (need_mask & BC_NEED_PW_BIAS) != 0};
-    const int64_t ctas = (int64_t)v.splits * q.tiles_o * q.tiles_i;
-    if (ctas > INT32_MAX) return BC_ERR_BAD_SHAPE;
-    return with_type(s.io_kind, [&](auto t) {
-        using T = decltype(t);
-        {
+    if (need_mask & BC_NEED_PW_INPUT) {
+        const int e = pointwise_mma_suits(s, true) && pointwise_mma_aligned(dz, weight, grad_input)
+                          ? launch_pointwise_mma_input(s, dz, weight, grad_input, stream)
+                          : launch_product<INPUT>(s, {dz, weight, nullptr, nullptr, nullptr, grad_input, s.Co, s.Ci, 1, s.Ci}, stream);
+        if (e) return e;
+    }
+    if (!want_weight && !want_bias) return BC_OK;
+    const int64_t weights = (int64_t)s.Co * s.Ci;
+    Partials of_weights{}, of_sums{};
+    if (sums) of_sums = {sums, s.Co, s.Co, pointwise_mma_sums_rows(s), grad_bias};
+    if (want_weight || !sums) {
+        const Splits v = splits_of(s);
+        float *partial = static_cast<float *>(take(partial_bytes(s)));
+        WeightProduct q{dz, x, partial, s.last ? 1 : s.N, s.Ci, s.Co, s.last ? s.N * s.P : s.P, (int)ceil_div(s.Co, kBO),
+                        (int)ceil_div(s.Ci ? s.Ci : 1, kBI), v.chunk, v.chunks, v.per, want_bias && !sums};
+        const int64_t ctas = (int64_t)v.splits * q.tiles_o * q.tiles_i;
+        if (ctas > INT32_MAX) return BC_ERR_BAD_SHAPE;
+        const int e = with_type(s.io_kind, [&](auto t) {
+            using T = decltype(t);
             const LaunchScope scope(KID_POINTWISE_WEIGHT, stream);
             if (s.last) launch_overlapped(pointwise_weight_kernel<T, true>, (unsigned)ctas, kThreads, 0, stream, q);
             else launch_overlapped(pointwise_weight_kernel<T, false>, (unsigned)ctas, kThreads, 0, stream, q);
-            if (const int e = check_launch("pointwise_weight_kernel")) return e;
-        }
-        const int64_t weights = (int64_t)s.Co * s.Ci;
+            return check_launch("pointwise_weight_kernel");
+        });
+        if (e) return e;
+        if (want_weight) of_weights = {partial, weights + s.Co, weights, v.splits, grad_weight};
+        if (want_bias && !sums) of_sums = {partial + weights, weights + s.Co, s.Co, v.splits, grad_bias};
+    }
+    const int64_t blocks = ceil_div(of_weights.count, 32), more = ceil_div(of_sums.count, 32);
+    if (blocks + more > INT32_MAX) return BC_ERR_BAD_SHAPE;
+    return with_type(s.io_kind, [&](auto t) {
+        using T = decltype(t);
         const LaunchScope scope(KID_POINTWISE_FINISH, stream);
-        launch_overlapped(pointwise_finish_kernel<T>, (unsigned)ceil_div(weights + s.Co, kThreads), kThreads, 0, stream, (const float *)partial, v.splits,
-                          weights, s.Co, (need_mask & BC_NEED_PW_WEIGHT) ? (T *)grad_weight : nullptr,
-                          (need_mask & BC_NEED_PW_BIAS) ? (T *)grad_bias : nullptr);
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)(blocks + more));
+        cfg.blockDim = dim3(32, kFinishRows);
+        cfg.stream = stream;
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr.val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        cudaLaunchKernelEx(&cfg, pointwise_finish_kernel<T>, of_weights, of_sums, (unsigned)blocks);
         return check_launch("pointwise_finish_kernel");
     });
 }

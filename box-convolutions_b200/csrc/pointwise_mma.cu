@@ -1,0 +1,409 @@
+// Pointwise convolutions of 16-bit tensors on the tensor cores: the products of pointwise.cu where rows start on 16 bytes.
+//
+// pointwise_mma_kernel, the products with pixels in the rows: D[p, c] = sum_k A[p, k] B[c, k], tiles of 128 pixels x up to 256
+// channels.  The weights stay in shared memory; persistent CTAs walk over the pixels.  One thread brings slices of 64 k by
+// TMA into a ring, one issues tcgen05.mma into one of two sets of accumulators in tensor memory, eight warps take the other set
+// out.  Planes are an MN-major operand and channels last a K-major one: no transposition in either.
+// A warp of the epilogue passes 32 x 32 accumulators through shared memory (rows of 33 words: no bank conflicts), so that it
+// reads residuals and gradients and writes results 16 bytes a lane, along whichever index runs in memory.
+//
+// pointwise_weight_mma_kernel: grad_weight, D[o, i] = sum_p dz[o, p] x[i, p], 128 x up to 256 weights, split over the pixels.
+#include "bc_mma.cuh"
+
+namespace bc {
+
+namespace {
+
+enum { FORWARD, SLOPE, INPUT };
+constexpr int kEpilogue = 8, kThreads = 32 * (kEpilogue + 2);
+constexpr int kPitch = 33;
+constexpr uint32_t kStage = 16384;      // 128 pixels x 64 k
+constexpr size_t kMostShared = 227 << 10;
+
+struct MmaProduct {
+    CUtensorMap a, w;
+    const void *bias, *residual, *grad;
+    void *out;
+    float *sums;             // SLOPE: [CTA / tiles_n][Cn] sums of dz over the CTA's pixels, or null
+    int64_t P;               // pixels of a sample (of all of them together, channels last)
+    int K, Cn, samples;
+    int tiles_p, tiles_n;
+    int bn, stages, columns; // channels of a tile; slices in the ring; columns of tensor memory for one set
+    uint32_t instruction;
+};
+
+// Shared memory from a 1024-byte boundary on.
+struct MmaLayout {
+    int bn, stages, chunks;
+    bool input;
+    // of one slice of 64 k of the weights
+    __host__ __device__ uint32_t slice() const { return input ? (uint32_t)((bn + 63) / 64) * kBlockBytes : (uint32_t)bn * 128; }
+    __host__ __device__ uint32_t ring() const { return (chunks * slice() + 1023) / 1024 * 1024; }
+    __host__ __device__ uint32_t staging() const { return ring() + stages * kStage; }
+    __host__ __device__ uint32_t bias() const { return staging() + kEpilogue * 32 * kPitch * 4; }
+    __host__ __device__ uint32_t sums() const { return bias() + bn * 4; }
+    __host__ __device__ uint32_t barriers() const { return (sums() + 4 * bn * 4 + 7) / 8 * 8; }
+    __host__ __device__ uint32_t bytes() const { return barriers() + (2 * stages + 5) * 8 + 8 + 1024; }
+};
+
+template <typename T, int MODE, int ACT, bool LAST>
+__global__ void __launch_bounds__(kThreads, 2) pointwise_mma_kernel(const __grid_constant__ MmaProduct q)
+{
+    extern __shared__ char raw_smem[];
+    const uint32_t raw = smem_u32(raw_smem), base = (raw + 1023) & ~1023u;
+    char *smem = raw_smem + (base - raw);
+    const int chunks = (q.K + 63) / 64;
+    const MmaLayout lay{q.bn, q.stages, chunks, MODE == INPUT};
+    float *bias_smem = reinterpret_cast<float *>(smem + lay.bias()), *sums_smem = reinterpret_cast<float *>(smem + lay.sums());
+    const uint32_t full = base + lay.barriers(), empty = full + 8 * q.stages, ready = empty + 8 * q.stages, drained = ready + 16,
+                   weights_full = drained + 16;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + lay.barriers() + (2 * q.stages + 5) * 8);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const unsigned walkers = gridDim.x / (unsigned)q.tiles_n, walker = blockIdx.x / (unsigned)q.tiles_n;
+    const int n0 = (int)(blockIdx.x - walker * q.tiles_n) * q.bn;
+    const int64_t tiles = (int64_t)q.samples * q.tiles_p;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < q.stages; ++i) {
+            mbar_init(full + 8 * i, 1);
+            mbar_init(empty + 8 * i, 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(ready + 8 * i, 1);
+            mbar_init(drained + 8 * i, kEpilogue);
+        }
+        mbar_init(weights_full, 1);
+        fence_mbar_init();
+        map_prefetch(&q.a);
+        map_prefetch(&q.w);
+    }
+    grid_dependency_wait();
+    if (warp == kEpilogue + 1) tmem_alloc(tmem_slot, 2 * q.columns);
+    for (int i = threadIdx.x; i < q.bn; i += kThreads)
+        bias_smem[i] = MODE != INPUT && q.bias && n0 + i < q.Cn ? to_float(static_cast<const T *>(q.bias)[n0 + i]) : 0.f;
+    for (int i = threadIdx.x; i < 4 * q.bn; i += kThreads) sums_smem[i] = 0.f;
+    tmem_release();
+    __syncthreads();
+    tmem_acquire();
+    const uint32_t tmem = *tmem_slot;
+    Waiter wait;
+
+    if (warp == kEpilogue) {
+        if (lane == 0) {
+            mbar_expect(weights_full, chunks * lay.slice());
+            for (int c = 0; c < chunks; ++c) {
+                if (MODE == INPUT)
+                    for (int b = 0; b < (q.bn + 63) / 64; ++b)
+                        tile_load(base + c * lay.slice() + b * kBlockBytes, &q.w, n0 + 64 * b, 64 * c, weights_full);
+                else tile_load(base + c * lay.slice(), &q.w, 64 * c, n0, weights_full);
+            }
+            uint32_t stage = 0, phase = 0;
+            for (int64_t tile = walker; tile < tiles; tile += walkers) {
+                const int sample = (int)(tile / q.tiles_p);
+                const int64_t p0 = (tile - (int64_t)sample * q.tiles_p) * 128;
+                for (int c = 0; c < chunks; ++c) {
+                    if (!wait(empty + 8 * stage, phase ^ 1)) break;
+                    const uint32_t to = base + lay.ring() + stage * kStage, bar = full + 8 * stage;
+                    mbar_expect(bar, kStage);
+                    if (LAST) {
+                        tile_load(to, &q.a, 64 * c, (int)p0, bar);
+                    } else {
+                        tile_load(to, &q.a, (int)p0, 64 * c, sample, bar);
+                        tile_load(to + kBlockBytes, &q.a, (int)p0 + 64, 64 * c, sample, bar);
+                    }
+                    if (++stage == (uint32_t)q.stages) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                }
+                if (wait.lost) break;
+            }
+        }
+    } else if (warp == kEpilogue + 1) {
+        if (lane == 0) {
+            wait(weights_full, 0);
+            uint32_t stage = 0, phase = 0, set = 0, set_phase = 0;
+            for (int64_t tile = walker; tile < tiles; tile += walkers) {
+                if (!wait(drained + 8 * set, set_phase ^ 1)) break;
+                tmem_acquire();
+                for (int c = 0; c < chunks; ++c) {
+                    if (!wait(full + 8 * stage, phase)) break;
+                    tmem_acquire();
+                    const uint32_t a = base + lay.ring() + stage * kStage, w = base + c * lay.slice();
+                    const int steps = (min(64, q.K - 64 * c) + 15) / 16;
+                    for (int k = 0; k < 16 * steps; k += 16)
+                        mma(tmem + set * q.columns, LAST ? k_major(a, k) : mn_major(a, k, kBlockBytes),
+                            MODE == INPUT ? mn_major(w, k, kBlockBytes) : k_major(w, k), q.instruction, c || k);
+                    mma_commit(empty + 8 * stage);
+                    if (++stage == (uint32_t)q.stages) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                }
+                if (wait.lost) break;
+                mma_commit(ready + 8 * set);
+                if (set ^= 1; set == 0) set_phase ^= 1;
+            }
+        }
+    } else {
+        float *staging = reinterpret_cast<float *>(smem + lay.staging()) + warp * 32 * kPitch;
+        const int quarter = warp & 3, half = warp >> 2, blocks = (q.bn + 31) / 32;
+        const int row8 = lane >> 2, col8 = (lane & 3) * 8;
+        const T *residual = static_cast<const T *>(q.residual), *grad = static_cast<const T *>(q.grad);
+        T *out = static_cast<T *>(q.out);
+        uint32_t set = 0, set_phase = 0;
+        for (int64_t tile = walker; tile < tiles; tile += walkers) {
+            const int sample = (int)(tile / q.tiles_p);
+            const int64_t p0 = (tile - (int64_t)sample * q.tiles_p) * 128 + quarter * 32;
+            bool waited = false;
+            for (int b = half; b < blocks; b += 2) {
+                // the lane's four vectors: planes, channel 8 i + row8 and pixels from col8; last, pixel 8 i + row8 and channels
+                int64_t at[4];
+                bool there[4];
+                uint4 res[4], gr[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int64_t p = p0 + (LAST ? 8 * i + row8 : col8);
+                    const int c = n0 + 32 * b + (LAST ? col8 : 8 * i + row8);
+                    there[i] = p < q.P && c < q.Cn && 32 * b + (LAST ? col8 : 8 * i + row8) < q.bn;
+                    at[i] = LAST ? p * q.Cn + c : ((int64_t)sample * q.Cn + c) * q.P + p;
+                    if (MODE != INPUT && residual && there[i]) res[i] = *reinterpret_cast<const uint4 *>(residual + at[i]);
+                    if (MODE == SLOPE && there[i]) gr[i] = *reinterpret_cast<const uint4 *>(grad + at[i]);
+                }
+                if (!waited) {
+                    waited = true;
+                    wait(ready + 8 * set, set_phase);
+                    __syncwarp();
+                    tmem_acquire();
+                }
+                float v[32];
+                tmem_load32(tmem + set * q.columns + 32 * b + ((uint32_t)quarter << 21), v);
+                if (b + 2 >= blocks) {
+                    tmem_release();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(drained + 8 * set);
+                }
+#pragma unroll
+                for (int j = 0; j < 32; ++j) staging[lane * kPitch + j] = v[j];
+                __syncwarp();
+                float total[8] = {};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    f2_t z[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float *from = LAST ? staging + (8 * i + row8) * kPitch + col8 + 2 * j : staging + (col8 + 2 * j) * kPitch + 8 * i + row8;
+                        z[j] = pack2(from[0], from[LAST ? 1 : kPitch]);
+                    }
+                    if (MODE != INPUT) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int c = 32 * b + (LAST ? col8 + 2 * j : 8 * i + row8);
+                            if (there[i]) z[j] = add2(z[j], pack2(bias_smem[c], bias_smem[LAST ? c + 1 : c]));
+                        }
+                        if (residual && there[i]) {
+                            f2_t r[4];
+                            unpack_pairs<T>(res[i], r);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) z[j] = add2(z[j], r[j]);
+                        }
+                        if (MODE == SLOPE) {
+                            f2_t g[4];
+                            if (there[i]) {
+                                unpack_pairs<T>(gr[i], g);
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) z[j] = times_slope2<ACT, T>(g[j], z[j]);
+                            } else {
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) z[j] = both(0.f);
+                            }
+                            if (q.sums) {
+                                float s[8];
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) unpack2(z[j], s[2 * j], s[2 * j + 1]);
+                                if (LAST) {
+#pragma unroll
+                                    for (int j = 0; j < 8; ++j) total[j] += s[j];
+                                } else {
+                                    float t = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+                                    t += __shfl_xor_sync(0xffffffffu, t, 1);
+                                    t += __shfl_xor_sync(0xffffffffu, t, 2);
+                                    if ((lane & 3) == 0 && there[i]) sums_smem[quarter * q.bn + 32 * b + 8 * i + row8] += t;
+                                }
+                            }
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) z[j] = activate2<ACT, T>(z[j]);
+                        }
+                    }
+                    if (there[i]) *reinterpret_cast<uint4 *>(out + at[i]) = pack_pairs<T>(z);
+                }
+                if (MODE == SLOPE && LAST && q.sums) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        total[j] += __shfl_xor_sync(0xffffffffu, total[j], 4);
+                        total[j] += __shfl_xor_sync(0xffffffffu, total[j], 8);
+                        total[j] += __shfl_xor_sync(0xffffffffu, total[j], 16);
+                        if (row8 == j && 32 * b + col8 + j < q.bn) sums_smem[quarter * q.bn + 32 * b + col8 + j] += total[j];
+                    }
+                }
+                __syncwarp();
+            }
+            if (!waited) {      // (no columns for this half: it drains by arriving)
+                wait(ready + 8 * set, set_phase);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(drained + 8 * set);
+            }
+            if (wait.lost) break;
+            if (set ^= 1; set == 0) set_phase ^= 1;
+        }
+    }
+    if (wait.lost) let_copies_land();
+    __syncwarp();
+    tmem_release();
+    __syncthreads();
+    if (warp == kEpilogue + 1) tmem_free(tmem, 2 * q.columns);
+    if (MODE == SLOPE && q.sums)
+        for (int i = threadIdx.x; i < q.bn; i += kThreads)
+            if (n0 + i < q.Cn)
+                q.sums[(int64_t)walker * q.Cn + n0 + i] = (sums_smem[i] + sums_smem[q.bn + i]) + (sums_smem[2 * q.bn + i] + sums_smem[3 * q.bn + i]);
+}
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+// Tiles, ring and grid of a product; false where the weights do not fit.
+struct Plan {
+    int bn, tiles_n, stages, columns;
+    int64_t tiles_p;
+    unsigned walkers;
+    uint32_t smem;
+};
+bool plan_product(const PointwiseShape &s, int K, int Cn, bool input, Plan *plan)
+{
+    const int samples = s.last ? 1 : s.N, chunks = (int)ceil_div(K, 64);
+    const int64_t P = s.last ? s.N * s.P : s.P;
+    Plan r{};
+    // channels of a tile: all of them up to 256, with weights of at most 128 KB
+    const int64_t most = std::min<int64_t>(256, (int64_t)(128 << 10) / (chunks * 128) / 16 * 16);
+    if (most < 32) return false;
+    r.tiles_n = (int)ceil_div(Cn, most);
+    r.bn = (int)ceil_div(ceil_div(Cn, r.tiles_n), 16) * 16;
+    r.tiles_n = (int)ceil_div(Cn, r.bn);
+    r.columns = 32;
+    while (r.columns < r.bn) r.columns *= 2;
+    r.tiles_p = ceil_div(P, 128);
+    const int64_t tiles = r.tiles_p * samples;
+    for (r.stages = 4; r.stages >= 2; --r.stages) {
+        r.smem = MmaLayout{r.bn, r.stages, chunks, input}.bytes();
+        if (r.smem <= kMostShared) break;
+    }
+    // (coordinates of 32 bits, strides below 2^40 bytes)
+    if (r.stages < 2 || tiles > INT32_MAX || P > INT32_MAX - 256 || P * std::max(s.Ci, s.Co) >= (int64_t)1 << 38) return false;
+    const int per_sm = r.columns <= 128 && 2 * (r.smem + 1024) <= 228 << 10 ? 2 : 1;
+    r.walkers = (unsigned)std::min<int64_t>(tiles, std::max<int64_t>(1, 148 * per_sm / r.tiles_n));
+    *plan = r;
+    return true;
+}
+
+template <int MODE>
+int launch_mma(const PointwiseShape &s, const Plan &plan, MmaProduct q, const void *a, const void *w, cudaStream_t stream)
+{
+    const bool bf16 = s.io_kind == BC_IO_BF16;
+    q.samples = s.last ? 1 : s.N;
+    q.P = s.last ? s.N * s.P : s.P;
+    q.tiles_p = (int)plan.tiles_p;
+    q.tiles_n = plan.tiles_n;
+    q.bn = plan.bn;
+    q.stages = plan.stages;
+    q.columns = plan.columns;
+    q.instruction = mma_instruction(bf16, !s.last, MODE == INPUT, plan.bn);
+    {
+        const uint64_t last_sizes[2] = {(uint64_t)q.K, (uint64_t)q.P}, last_strides[1] = {(uint64_t)q.K};
+        const uint64_t sizes[3] = {(uint64_t)q.P, (uint64_t)q.K, (uint64_t)q.samples}, strides[2] = {(uint64_t)q.P, (uint64_t)q.P * q.K};
+        const uint32_t last_box[2] = {64, 128}, box[3] = {64, 64, 1};
+        if (const int e = s.last ? make_map(&q.a, a, bf16, 2, last_sizes, last_strides, last_box) : make_map(&q.a, a, bf16, 3, sizes, strides, box))
+            return e;
+        const uint64_t w_sizes[2] = {(uint64_t)s.Ci, (uint64_t)s.Co}, w_strides[1] = {(uint64_t)s.Ci};
+        const uint32_t w_box[2] = {64, MODE == INPUT ? 64u : (uint32_t)plan.bn};
+        if (const int e = make_map(&q.w, w, bf16, 2, w_sizes, w_strides, w_box)) return e;
+    }
+    return with_activation(MODE == INPUT ? BC_ACT_NONE : s.act, [&](auto act) {
+        constexpr int ACT = MODE == INPUT ? BC_ACT_NONE : act();
+        auto go = [&](auto kernel) {
+            if (const int e = raise_smem_limit((const void *)kernel, kMostShared)) return e;
+            const LaunchScope scope(KID_POINTWISE_MMA, stream);
+            launch_overlapped(kernel, plan.walkers * plan.tiles_n, kThreads, plan.smem, stream, q);
+            return check_launch("pointwise_mma_kernel");
+        };
+        if (bf16) return s.last ? go(pointwise_mma_kernel<__nv_bfloat16, MODE, ACT, true>) : go(pointwise_mma_kernel<__nv_bfloat16, MODE, ACT, false>);
+        return s.last ? go(pointwise_mma_kernel<__half, MODE, ACT, true>) : go(pointwise_mma_kernel<__half, MODE, ACT, false>);
+    });
+}
+
+// TMA wants rows that start on 16 bytes; the epilogue's vectors too.
+bool rows_aligned(const PointwiseShape &s)
+{
+    if (s.io_kind == BC_IO_F32 || s.Ci % 8 || s.Ci < 8) return false;
+    return s.last ? s.Co % 8 == 0 && s.Co >= 8 : s.P % 8 == 0;
+}
+
+}  // namespace
+
+// ---- the products with pixels in the rows; false: not for these kernels
+bool pointwise_mma_suits(const PointwiseShape &s, bool input)
+{
+    Plan plan;
+    return rows_aligned(s) && plan_product(s, input ? s.Co : s.Ci, input ? s.Ci : s.Co, input, &plan);
+}
+bool pointwise_mma_aligned(const void *a, const void *b, const void *c, const void *d, const void *e)
+{
+    return aligned16(a) && aligned16(b) && aligned16(c) && aligned16(d) && aligned16(e);
+}
+int pointwise_mma_sums_rows(const PointwiseShape &s)
+{
+    Plan plan;
+    return plan_product(s, s.Ci, s.Co, false, &plan) ? (int)plan.walkers : 0;
+}
+int launch_pointwise_mma_forward(const PointwiseShape &s, const void *x, const void *weight, const void *bias, const void *residual, void *out,
+                                 cudaStream_t stream)
+{
+    Plan plan;
+    plan_product(s, s.Ci, s.Co, false, &plan);
+    MmaProduct q{};
+    q.bias = bias;
+    q.residual = residual;
+    q.out = out;
+    q.K = s.Ci;
+    q.Cn = s.Co;
+    return launch_mma<FORWARD>(s, plan, q, x, weight, stream);
+}
+int launch_pointwise_mma_slope(const PointwiseShape &s, const void *x, const void *weight, const void *bias, const void *residual,
+                               const void *grad, void *dz, float *sums, cudaStream_t stream)
+{
+    Plan plan;
+    plan_product(s, s.Ci, s.Co, false, &plan);
+    MmaProduct q{};
+    q.bias = bias;
+    q.residual = residual;
+    q.grad = grad;
+    q.out = dz;
+    q.sums = sums;
+    q.K = s.Ci;
+    q.Cn = s.Co;
+    return launch_mma<SLOPE>(s, plan, q, x, weight, stream);
+}
+int launch_pointwise_mma_input(const PointwiseShape &s, const void *dz, const void *weight, void *grad_input, cudaStream_t stream)
+{
+    Plan plan;
+    plan_product(s, s.Co, s.Ci, true, &plan);
+    MmaProduct q{};
+    q.out = grad_input;
+    q.K = s.Co;
+    q.Cn = s.Ci;
+    return launch_mma<INPUT>(s, plan, q, dz, weight, stream);
+}
+
+int read_wait_timeouts_mma(int *count) { return read_wait_timeouts_here(count); }
+
+}  // namespace bc

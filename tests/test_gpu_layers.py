@@ -463,6 +463,27 @@ def test_two_captured_steps_replayed_at_once(bc):
                 assert all(torch.equal(a, b) for a, b in zip(out, want)), (name, turn)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_first_call_of_a_thread(bc, dtype):
+    """A thread that has not called into CUDA before, with memory at hand that needs no call either."""
+    import threading
+    x, g = torch.randn(2, 24, 16, 16, device="cuda").to(dtype), torch.randn(2, 40, 16, 16, device="cuda").to(dtype)
+    for name, f, params in _calls(bc):
+        params = [p.to(dtype) for p in params]
+        for what in (lambda: [f(x, *params)], lambda: _step(f, x, params, g)):
+            want, got = what(), []
+
+            def work():
+                got.extend(what())
+                torch.cuda.synchronize()
+
+            del want[1:]
+            t = threading.Thread(target=work)
+            t.start()
+            t.join()
+            assert got and torch.equal(got[0], want[0]), name
+
+
 def test_what_autograd_asks_for(bc):
     import torch.autograd.forward_ad as fwad
     for name, f, params in _calls(bc):
@@ -580,3 +601,8 @@ def test_the_layers_of_a_block_together(bc, dtype, last):
     assert rel(out, ref) < tol
     for k in want:
         assert rel(got[k], want[k]) < (10 * tol if k.startswith("box") else tol), k
+
+
+def test_no_wait_has_expired():
+    from box_convolution import _cabi
+    assert _cabi.wait_timeouts() == 0
