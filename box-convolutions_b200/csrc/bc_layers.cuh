@@ -260,6 +260,11 @@ int pointwise_mma_sums_rows(const PointwiseShape &s);
 int launch_pointwise_mma_slope(const PointwiseShape &s, const void *x, const void *weight, const void *bias, const void *residual,
                                const void *grad, void *dz, float *sums, cudaStream_t stream);
 int launch_pointwise_mma_input(const PointwiseShape &s, const void *dz, const void *weight, void *grad_input, cudaStream_t stream);
+// Floats of a row of partial sums of grad_weight, Co * Ci and the Co of grad_bias: whole vectors, so that every row starts on one.
+__host__ __device__ inline int64_t pointwise_partial_stride(int Co, int Ci) { return ((int64_t)Co * Ci + Co + 3) / 4 * 4; }
+// rows of partial sums (0: not for this kernel)
+int pointwise_mma_weight_splits(const PointwiseShape &s);
+int launch_pointwise_mma_weight(const PointwiseShape &s, const void *dz, const void *x, float *partial, bool sums, cudaStream_t stream);
 int read_wait_timeouts_mma(int *count);
 
 size_t pointwise_workspace(const PointwiseShape &s, int need_mask);

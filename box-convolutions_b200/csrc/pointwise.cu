@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(kThreads) pointwise_kernel(Product q)
 
 struct WeightProduct {
     const void *dz, *x;
-    float *partial;          // [split][Co * Ci, then Co sums of dz]
+    float *partial;          // a row a split: Co * Ci sums, then Co sums of dz
     int N, Ci, Co;           // (N 1, channels last)
     int64_t P;
     int tiles_o, tiles_i;
@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(kThreads) pointwise_weight_kernel(WeightProduc
             __syncthreads();
         }
     }
-    float *partial = q.partial + (int64_t)split * ((int64_t)q.Co * q.Ci + q.Co);
+    float *partial = q.partial + split * pointwise_partial_stride(q.Co, q.Ci);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const int o = o0 + 32 * (i / 4) + 4 * tm + i % 4;
@@ -269,7 +269,8 @@ Splits splits_of(const PointwiseShape &s)
 
 size_t partial_bytes(const PointwiseShape &s)
 {
-    return align_up((size_t)splits_of(s).splits * ((size_t)s.Co * s.Ci + s.Co) * sizeof(float));
+    // (either kernel's: the query does not know the arrays)
+    return align_up((size_t)std::max(splits_of(s).splits, pointwise_mma_weight_splits(s)) * pointwise_partial_stride(s.Co, s.Ci) * sizeof(float));
 }
 size_t sums_bytes(const PointwiseShape &s) { return align_up((size_t)pointwise_mma_sums_rows(s) * s.Co * sizeof(float)); }
 // dz in memory, where it is neither grad_output itself nor asked for.
@@ -329,22 +330,28 @@ int launch_pointwise_backward(const PointwiseShape &s, const void *x, const void
     Partials of_weights{}, of_sums{};
     if (sums) of_sums = {sums, s.Co, s.Co, pointwise_mma_sums_rows(s), grad_bias};
     if (want_weight || !sums) {
-        const Splits v = splits_of(s);
         float *partial = static_cast<float *>(take(partial_bytes(s)));
-        WeightProduct q{dz, x, partial, s.last ? 1 : s.N, s.Ci, s.Co, s.last ? s.N * s.P : s.P, (int)ceil_div(s.Co, kBO),
-                        (int)ceil_div(s.Ci ? s.Ci : 1, kBI), v.chunk, v.chunks, v.per, want_bias && !sums};
-        const int64_t ctas = (int64_t)v.splits * q.tiles_o * q.tiles_i;
-        if (ctas > INT32_MAX) return BC_ERR_BAD_SHAPE;
-        const int e = with_type(s.io_kind, [&](auto t) {
-            using T = decltype(t);
-            const LaunchScope scope(KID_POINTWISE_WEIGHT, stream);
-            if (s.last) launch_overlapped(pointwise_weight_kernel<T, true>, (unsigned)ctas, kThreads, 0, stream, q);
-            else launch_overlapped(pointwise_weight_kernel<T, false>, (unsigned)ctas, kThreads, 0, stream, q);
-            return check_launch("pointwise_weight_kernel");
-        });
+        int splits = pointwise_mma_weight_splits(s), e;
+        if (splits && pointwise_mma_aligned(dz, x)) {
+            e = launch_pointwise_mma_weight(s, dz, x, partial, want_bias && !sums, stream);
+        } else {
+            const Splits v = splits_of(s);
+            splits = v.splits;
+            WeightProduct q{dz, x, partial, s.last ? 1 : s.N, s.Ci, s.Co, s.last ? s.N * s.P : s.P, (int)ceil_div(s.Co, kBO),
+                            (int)ceil_div(s.Ci ? s.Ci : 1, kBI), v.chunk, v.chunks, v.per, want_bias && !sums};
+            const int64_t ctas = (int64_t)v.splits * q.tiles_o * q.tiles_i;
+            if (ctas > INT32_MAX) return BC_ERR_BAD_SHAPE;
+            e = with_type(s.io_kind, [&](auto t) {
+                using T = decltype(t);
+                const LaunchScope scope(KID_POINTWISE_WEIGHT, stream);
+                if (s.last) launch_overlapped(pointwise_weight_kernel<T, true>, (unsigned)ctas, kThreads, 0, stream, q);
+                else launch_overlapped(pointwise_weight_kernel<T, false>, (unsigned)ctas, kThreads, 0, stream, q);
+                return check_launch("pointwise_weight_kernel");
+            });
+        }
         if (e) return e;
-        if (want_weight) of_weights = {partial, weights + s.Co, weights, v.splits, grad_weight};
-        if (want_bias && !sums) of_sums = {partial + weights, weights + s.Co, s.Co, v.splits, grad_bias};
+        if (want_weight) of_weights = {partial, pointwise_partial_stride(s.Co, s.Ci), weights, splits, grad_weight};
+        if (want_bias && !sums) of_sums = {partial + weights, pointwise_partial_stride(s.Co, s.Ci), s.Co, splits, grad_bias};
     }
     const int64_t blocks = ceil_div(of_weights.count, 32), more = ceil_div(of_sums.count, 32);
     if (blocks + more > INT32_MAX) return BC_ERR_BAD_SHAPE;

@@ -269,6 +269,173 @@ __global__ void __launch_bounds__(kThreads, 2) pointwise_mma_kernel(const __grid
                 q.sums[(int64_t)walker * q.Cn + n0 + i] = (sums_smem[i] + sums_smem[q.bn + i]) + (sums_smem[2 * q.bn + i] + sums_smem[3 * q.bn + i]);
 }
 
+// ---- grad_weight
+
+constexpr int kWeightThreads = 32 * 6, kMostStages = 8;
+
+struct WeightMma {
+    CUtensorMap dz, x;
+    float *partial;          // a row a split: Co * Ci sums, then Co sums of dz
+    int64_t per;             // slices of 64 pixels of a split
+    int64_t slices;          // of a sample
+    int samples, Ci, Co;
+    int tiles_i;
+    int bn, rows, stages, columns;      // input channels of a tile; rows of dz that are loaded (planes); ring; tensor memory
+    bool sums;
+    uint32_t instruction;
+};
+
+// Shared memory from a 1024-byte boundary on: slices of dz (128 channels) and x (bn), then barriers.
+struct WeightLayout {
+    int bn, stages;
+    bool last;
+    __host__ __device__ uint32_t x_bytes() const { return last ? (uint32_t)((bn + 63) / 64) * kBlockBytes : (uint32_t)bn * 128; }
+    __host__ __device__ uint32_t stage() const { return 2 * kBlockBytes + x_bytes(); }
+    __host__ __device__ uint32_t barriers() const { return stages * stage(); }
+    __host__ __device__ uint32_t bytes() const { return barriers() + (2 * stages + 1) * 8 + 8 + 1024; }
+};
+
+// Four warps of the epilogue also add up dz, from the slices as they pass, for grad_bias.
+template <typename T, bool LAST>
+__global__ void __launch_bounds__(kWeightThreads) pointwise_weight_mma_kernel(const __grid_constant__ WeightMma q)
+{
+    extern __shared__ char raw_smem[];
+    __shared__ float part[128][9];
+    const uint32_t raw = smem_u32(raw_smem), base = (raw + 1023) & ~1023u;
+    char *smem = raw_smem + (base - raw);
+    const WeightLayout lay{q.bn, q.stages, LAST};
+    const uint32_t full = base + lay.barriers(), empty = full + 8 * q.stages, ready = empty + 8 * q.stages;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + lay.barriers() + (2 * q.stages + 1) * 8);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int tiles_o = (q.Co + 127) / 128, tiles = tiles_o * q.tiles_i;
+    const int split = (int)(blockIdx.x / (unsigned)tiles), t = (int)blockIdx.x - split * tiles;
+    const int o0 = t / q.tiles_i * 128, i0 = (t - t / q.tiles_i * q.tiles_i) * q.bn;
+    const int64_t first = split * q.per, last = min((int64_t)q.samples * q.slices, first + q.per);
+    const bool sums = q.sums && i0 == 0;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < q.stages; ++i) {
+            mbar_init(full + 8 * i, 1);
+            mbar_init(empty + 8 * i, sums ? 5 : 1);
+        }
+        mbar_init(ready, 1);
+        fence_mbar_init();
+        map_prefetch(&q.dz);
+        map_prefetch(&q.x);
+    }
+    grid_dependency_wait();
+    if (warp == 5) tmem_alloc(tmem_slot, q.columns);
+    tmem_release();
+    __syncthreads();
+    tmem_acquire();
+    const uint32_t tmem = *tmem_slot;
+    Waiter wait;
+
+    if (warp == 4) {
+        if (lane == 0) {
+            const int a_blocks = LAST ? (o0 + 64 < q.Co ? 2 : 1) : 0, b_blocks = (q.bn + 63) / 64;
+            const uint32_t bytes = (LAST ? a_blocks * kBlockBytes : (uint32_t)q.rows * 128) + lay.x_bytes();
+            uint32_t stage = 0, phase = 0;
+            for (int64_t slice = first; slice < last; ++slice) {
+                if (!wait(empty + 8 * stage, phase ^ 1)) break;
+                const int sample = (int)(slice / q.slices), p0 = (int)(slice - sample * q.slices) * 64;
+                const uint32_t a = base + stage * lay.stage(), b = a + 2 * kBlockBytes, bar = full + 8 * stage;
+                mbar_expect(bar, bytes);
+                if (LAST) {
+                    for (int i = 0; i < a_blocks; ++i) tile_load(a + i * kBlockBytes, &q.dz, o0 + 64 * i, p0, bar);
+                    for (int i = 0; i < b_blocks; ++i) tile_load(b + i * kBlockBytes, &q.x, i0 + 64 * i, p0, bar);
+                } else {
+                    tile_load(a, &q.dz, p0, o0, sample, bar);
+                    tile_load(b, &q.x, p0, i0, sample, bar);
+                }
+                if (++stage == (uint32_t)q.stages) {
+                    stage = 0;
+                    phase ^= 1;
+                }
+            }
+        }
+    } else if (warp == 5) {
+        if (lane == 0) {
+            uint32_t stage = 0, phase = 0;
+            for (int64_t slice = first; slice < last; ++slice) {
+                if (!wait(full + 8 * stage, phase)) break;
+                tmem_acquire();
+                const uint32_t a = base + stage * lay.stage(), b = a + 2 * kBlockBytes;
+#pragma unroll
+                for (int k = 0; k < 64; k += 16)
+                    mma(tmem, LAST ? mn_major(a, k, kBlockBytes) : k_major(a, k), LAST ? mn_major(b, k, kBlockBytes) : k_major(b, k), q.instruction,
+                        slice > first || k);
+                mma_commit(empty + 8 * stage);
+                if (++stage == (uint32_t)q.stages) {
+                    stage = 0;
+                    phase ^= 1;
+                }
+            }
+            if (!wait.lost) mma_commit(ready);
+        }
+    } else {
+        float *partial = q.partial + split * pointwise_partial_stride(q.Co, q.Ci);
+        if (sums) {
+            // planes: a thread a channel, its 64 pixels.  last: a thread 8 channels of 8 pixels.
+            float total[8] = {};
+            uint32_t stage = 0, phase = 0;
+            const int group = threadIdx.x & 15, pixel = threadIdx.x >> 4;
+            for (int64_t slice = first; slice < last; ++slice) {
+                if (!wait(full + 8 * stage, phase)) break;
+                const char *a = smem + stage * lay.stage();
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int k = 8 * j + pixel;
+                    const char *from = LAST ? a + (group >> 3) * kBlockBytes + k * 128 + (((group & 7) ^ (k & 7)) << 4)
+                                            : a + threadIdx.x * 128 + ((j ^ (threadIdx.x & 7)) << 4);
+                    if (LAST ? o0 + 8 * group < q.Co : o0 + (int)threadIdx.x < q.Co) {
+                        float v[8];
+                        unpack<T>(*reinterpret_cast<const uint4 *>(from), v);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) total[i] += v[i];
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(empty + 8 * stage);
+                if (++stage == (uint32_t)q.stages) {
+                    stage = 0;
+                    phase ^= 1;
+                }
+            }
+            if (LAST) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) part[8 * group + i][pixel] = total[i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) part[threadIdx.x][i] = total[i];
+            }
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            if (o0 + (int)threadIdx.x < q.Co) {
+                const float *v = part[threadIdx.x];
+                partial[(int64_t)q.Co * q.Ci + o0 + threadIdx.x] = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+            }
+        }
+        if (!wait.lost) wait(ready, 0);
+        __syncwarp();
+        tmem_acquire();
+        const int o = o0 + warp * 32 + lane;
+        if (!__any_sync(0xffffffffu, wait.lost))
+            for (int b = 0; b < q.bn; b += 32) {
+                float v[32];
+                tmem_load32(tmem + b + ((uint32_t)warp << 21), v);
+                float *to = partial + (int64_t)o * q.Ci + i0 + b;
+#pragma unroll
+                for (int j = 0; j < 32; j += 4)
+                    if (o < q.Co && i0 + b + j < q.Ci && b + j < q.bn) *reinterpret_cast<float4 *>(to + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+            }
+    }
+    if (wait.lost) let_copies_land();
+    __syncwarp();
+    tmem_release();
+    __syncthreads();
+    if (warp == 5) tmem_free(tmem, q.columns);
+}
+
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
@@ -402,6 +569,83 @@ int launch_pointwise_mma_input(const PointwiseShape &s, const void *dz, const vo
     q.K = s.Co;
     q.Cn = s.Ci;
     return launch_mma<INPUT>(s, plan, q, dz, weight, stream);
+}
+
+// ---- grad_weight: rows of pointwise_partial_stride() floats, to be added
+namespace {
+struct WeightPlan {
+    int tiles_o, tiles_i, bn, stages, columns, splits;
+    int64_t slices, per;
+    uint32_t smem;
+};
+bool plan_weight(const PointwiseShape &s, WeightPlan *plan)
+{
+    if (!rows_aligned(s)) return false;
+    const int64_t P = s.last ? s.N * s.P : s.P, samples = s.last ? 1 : s.N;
+    if (P > INT32_MAX - 256 || P * std::max(s.Ci, s.Co) >= (int64_t)1 << 38) return false;
+    WeightPlan r{};
+    r.tiles_o = (int)ceil_div(s.Co, 128);
+    r.tiles_i = (int)ceil_div(s.Ci, 256);
+    r.bn = (int)ceil_div(ceil_div(s.Ci, r.tiles_i), 16) * 16;
+    r.tiles_i = (int)ceil_div(s.Ci, r.bn);
+    r.columns = 32;
+    while (r.columns < r.bn) r.columns *= 2;
+    for (r.stages = kMostStages; r.stages > 2; --r.stages) {
+        r.smem = WeightLayout{r.bn, r.stages, s.last}.bytes();
+        if (r.smem <= 200 << 10) break;
+    }
+    r.slices = ceil_div(P, 64);
+    const int64_t all = r.slices * samples, tiles = (int64_t)r.tiles_o * r.tiles_i;
+    // a CTA an SM, of four slices at least
+    r.per = std::max<int64_t>(std::min<int64_t>(4, all), ceil_div(all, std::max<int64_t>(1, 148 / tiles)));
+    r.splits = (int)ceil_div(all, r.per);
+    if (r.splits * tiles > INT32_MAX) return false;
+    *plan = r;
+    return true;
+}
+}  // namespace
+
+int pointwise_mma_weight_splits(const PointwiseShape &s)
+{
+    WeightPlan plan;
+    return plan_weight(s, &plan) ? plan.splits : 0;
+}
+int launch_pointwise_mma_weight(const PointwiseShape &s, const void *dz, const void *x, float *partial, bool sums, cudaStream_t stream)
+{
+    WeightPlan plan;
+    plan_weight(s, &plan);
+    const bool bf16 = s.io_kind == BC_IO_BF16;
+    WeightMma q{};
+    q.partial = partial;
+    q.per = plan.per;
+    q.slices = plan.slices;
+    q.samples = s.last ? 1 : s.N;
+    q.Ci = s.Ci;
+    q.Co = s.Co;
+    q.tiles_i = plan.tiles_i;
+    q.bn = plan.bn;
+    q.rows = std::min(128, (int)ceil_div(s.Co, 8) * 8);
+    q.stages = plan.stages;
+    q.columns = plan.columns;
+    q.sums = sums;
+    q.instruction = mma_instruction(bf16, s.last, s.last, plan.bn);
+    const int64_t P = s.last ? s.N * s.P : s.P;
+    auto map = [&](CUtensorMap *to, const void *from, int C, uint32_t rows) {
+        const uint64_t last_sizes[2] = {(uint64_t)C, (uint64_t)P}, last_strides[1] = {(uint64_t)C};
+        const uint64_t sizes[3] = {(uint64_t)P, (uint64_t)C, (uint64_t)s.N}, strides[2] = {(uint64_t)P, (uint64_t)P * C};
+        const uint32_t last_box[2] = {64, 64}, box[3] = {64, rows, 1};
+        return s.last ? make_map(to, from, bf16, 2, last_sizes, last_strides, last_box) : make_map(to, from, bf16, 3, sizes, strides, box);
+    };
+    if (const int e = map(&q.dz, dz, s.Co, q.rows)) return e;
+    if (const int e = map(&q.x, x, s.Ci, plan.bn)) return e;
+    auto go = [&](auto kernel) {
+        if (const int e = raise_smem_limit((const void *)kernel, 200 << 10)) return e;
+        const LaunchScope scope(KID_POINTWISE_WEIGHT_MMA, stream);
+        launch_overlapped(kernel, (unsigned)(plan.splits * plan.tiles_o * plan.tiles_i), kWeightThreads, plan.smem, stream, q);
+        return check_launch("pointwise_weight_mma_kernel");
+    };
+    if (bf16) return s.last ? go(pointwise_weight_mma_kernel<__nv_bfloat16, true>) : go(pointwise_weight_mma_kernel<__nv_bfloat16, false>);
+    return s.last ? go(pointwise_weight_mma_kernel<__half, true>) : go(pointwise_weight_mma_kernel<__half, false>);
 }
 
 int read_wait_timeouts_mma(int *count) { return read_wait_timeouts_here(count); }
