@@ -115,8 +115,9 @@ __device__ __forceinline__ f2_t of_each(f2_t v, F &&f)
     unpack2(v, a, b);
     return pack2(f(a), f(b));
 }
-// 1 / (1 + exp(-z)).  One reciprocal for two, 1 / a = b / (a b): reciprocals and powers of two are what 16-bit
-// normalisations wait for.  exp(-z) ends at 2^60, so that the product stays finite (and a NaN to itself); beyond, 0 is the result.
+// 1 / (1 + exp(-z)).  16-bit tensors: one reciprocal for two, 1 / a = b / (a b), since reciprocals and powers of two are what
+// their normalisations wait for; a value then depends on its neighbour in its 22nd bit.  exp(-z) ends at 2^60, so that the
+// product stays finite (and a NaN to itself); beyond, 0 is the result.
 template <typename T>
 __device__ __forceinline__ f2_t logistic2(f2_t z)
 {
@@ -131,8 +132,15 @@ __device__ __forceinline__ f2_t logistic2(f2_t z)
     }
     float a, b;
     unpack2(add2(e, both(1.f)), a, b);
-    const float r = reciprocal(a * b);
-    return pack2(t0 > 60.f ? 0.f : b * r, t1 > 60.f ? 0.f : a * r);
+    if constexpr (sizeof(T) == 4) {
+        a = reciprocal(a);
+        b = reciprocal(b);
+    } else {
+        const float r = reciprocal(a * b), swap = a * r;
+        a = b * r;
+        b = swap;
+    }
+    return pack2(t0 > 60.f ? 0.f : a, t1 > 60.f ? 0.f : b);
 }
 // The normal distribution function, and exp(-z^2 / 2).
 template <typename T>

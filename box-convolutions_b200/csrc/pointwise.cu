@@ -7,7 +7,7 @@
 //   grad_input   D[p, i] = sum_o dz[o, p] W[o, i]
 //   grad_weight  D[o, i] = sum_p dz[o, p] x[i, p]          split over the pixels; partial sums added in order
 // A CTA makes a tile of D from slices of 16 k that pass through shared memory as floats; a thread keeps 8 x 8 (8 x 4)
-// sums in registers, so that 16 (12) words read from shared memory feed 64 (32) multiply-adds.
+// sums in registers.
 #include "bc_layers.cuh"
 
 namespace bc {
@@ -26,46 +26,121 @@ struct Product {
     int tiles_p, tiles_n;    // tiles of a sample's pixels, and of the output's channels
 };
 
-// D's tile: kBM pixels of a sample x BN channels.
-template <typename T, int MODE, int ACT, bool LAST, int BN>
-__global__ void __launch_bounds__(kThreads) pointwise_kernel(Product q)
+// Four values in a row, aligned.
+template <typename T>
+__device__ __forceinline__ float4 load4(const T *p)
+{
+    if constexpr (sizeof(T) == 4) {
+        return *reinterpret_cast<const float4 *>(p);
+    } else {
+        const uint2 w = *reinterpret_cast<const uint2 *>(p);
+        float4 v;
+        widen2(w.x, v.x, v.y, T());
+        widen2(w.y, v.z, v.w, T());
+        return v;
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store4(T *p, const float (&v)[4])
+{
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    else *reinterpret_cast<uint2 *>(p) = make_uint2(narrow2(v[0], v[1], T()), narrow2(v[2], v[3], T()));
+}
+
+// What becomes of four sums whose values lie in a row; `bias` four of them.
+template <typename T, int MODE, int ACT, bool VEC>
+__device__ __forceinline__ void finish4(const Product &q, int64_t at, float (&z)[4], const float (&bias)[4])
+{
+    const T *residual = static_cast<const T *>(q.residual) + at, *grad = static_cast<const T *>(q.grad) + at;
+    T *out = static_cast<T *>(q.out) + at;
+    if (MODE != INPUT) {
+        float r[4] = {}, g[4];
+        if (q.residual) *reinterpret_cast<float4 *>(r) = load4(residual);
+        if (MODE == SLOPE) *reinterpret_cast<float4 *>(g) = load4(grad);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            z[i] += bias[i] + r[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+            const f2_t v = MODE == SLOPE ? times_slope2<ACT, T>(pack2(g[i], g[i + 1]), pack2(z[i], z[i + 1])) : activate2<ACT, T>(pack2(z[i], z[i + 1]));
+            unpack2(v, z[i], z[i + 1]);
+        }
+    }
+    store4<T>(out, z);
+}
+
+// D's tile: kBM pixels of a sample x BN channels.  VEC: rows and arrays allow vectors of four values; a thread's pixels are
+// 4 tm + {0..3} and 64 + that.  Otherwise they are tm + 16 i, so that neighbouring lanes store neighbouring values.
+// Multiply-adds go two pixels an instruction; the weights' slice holds every weight twice for that.
+// Measured (f32, 128 -> 32, 16 x 64 x 128 planes): one value an instruction, scalar stores 40 us.
+template <typename T, int MODE, int ACT, bool LAST, int BN, bool VEC>
+__global__ void __launch_bounds__(kThreads, BN == 64 ? 3 : 4) pointwise_kernel(Product q)
 {
     constexpr int TN = BN / 8;      // channels of a thread
-    __shared__ __align__(16) float As[2][kBK][kBM + 4], Bs[2][kBK][BN + 4];
+    __shared__ __align__(16) float As[2][kBK][kBM + 4];
+    __shared__ __align__(16) float2 Bs[2][kBK][BN + 2];
     const int tid = threadIdx.x, tm = tid & 15, tn = tid >> 4;
-    const int64_t tile = blockIdx.x / q.tiles_n;
+    const unsigned tile = blockIdx.x / (unsigned)q.tiles_n;
     const int n0 = (int)(blockIdx.x - tile * q.tiles_n) * BN;
-    const int64_t sample = tile / q.tiles_p, p0 = (tile - sample * q.tiles_p) * kBM;
+    const int64_t sample = tile / (unsigned)q.tiles_p, p0 = (int64_t)(tile - (unsigned)sample * q.tiles_p) * kBM;
     const int pixels = (int)min((int64_t)kBM, q.P - p0);
     const T *a = static_cast<const T *>(q.a) + sample * q.K * q.P + (LAST ? p0 * q.K : p0);
     const T *w = static_cast<const T *>(q.w);
     grid_dependency_wait();
 
-    float ra[kBM * kBK / kThreads], rb[BN * kBK / kThreads];
+    float ra[16], rb[BN / 8];
     auto load = [&](int k0) {
+        if constexpr (VEC) {
 #pragma unroll
-        for (int j = 0; j < kBM * kBK / kThreads; ++j) {
-            const int k = k0 + (LAST ? tid & 15 : j), m = LAST ? (tid >> 4) + 8 * j : tid;
-            ra[j] = k < q.K && m < pixels ? to_float(a[LAST ? (int64_t)m * q.K + k : k * q.P + m]) : 0.f;
+            for (int j = 0; j < 4; ++j) {
+                const int e = tid + kThreads * j, k = k0 + (LAST ? 4 * (e & 3) : e >> 5), m = LAST ? e >> 2 : 4 * (e & 31);
+                *reinterpret_cast<float4 *>(ra + 4 * j) =
+                    k < q.K && m < pixels ? load4(a + (LAST ? (int64_t)m * q.K + k : k * q.P + m)) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const int k = k0 + (LAST ? tid & 15 : j), m = LAST ? (tid >> 4) + 8 * j : tid;
+                ra[j] = k < q.K && m < pixels ? to_float(a[LAST ? (int64_t)m * q.K + k : k * q.P + m]) : 0.f;
+            }
         }
 #pragma unroll
-        for (int j = 0; j < BN * kBK / kThreads; ++j) {
+        for (int j = 0; j < BN / 8; ++j) {
             const int e = tid + kThreads * j;
             const int k = k0 + (MODE == INPUT ? e / BN : e % kBK), n = n0 + (MODE == INPUT ? e % BN : e / kBK);
             rb[j] = k < q.K && n < q.Cn ? to_float(w[(int64_t)n * q.wn + (int64_t)k * q.wk]) : 0.f;
         }
     };
     auto store = [&](int b) {
+        if constexpr (VEC) {
 #pragma unroll
-        for (int j = 0; j < kBM * kBK / kThreads; ++j) As[b][LAST ? tid & 15 : j][LAST ? (tid >> 4) + 8 * j : tid] = ra[j];
+            for (int j = 0; j < 4; ++j) {
+                const int e = tid + kThreads * j;
+                if (LAST) {
 #pragma unroll
-        for (int j = 0; j < BN * kBK / kThreads; ++j) {
+                    for (int i = 0; i < 4; ++i) As[b][4 * (e & 3) + i][e >> 2] = ra[4 * j + i];
+                } else {
+                    *reinterpret_cast<float4 *>(&As[b][e >> 5][4 * (e & 31)]) = *reinterpret_cast<const float4 *>(ra + 4 * j);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) As[b][LAST ? tid & 15 : j][LAST ? (tid >> 4) + 8 * j : tid] = ra[j];
+        }
+#pragma unroll
+        for (int j = 0; j < BN / 8; ++j) {
             const int e = tid + kThreads * j;
-            Bs[b][MODE == INPUT ? e / BN : e % kBK][MODE == INPUT ? e % BN : e / kBK] = rb[j];
+            Bs[b][MODE == INPUT ? e / BN : e % kBK][MODE == INPUT ? e % BN : e / kBK] = make_float2(rb[j], rb[j]);
         }
     };
 
-    float acc[8][TN] = {};
+    // pairs of pixels: VEC, 4 tm + {0, 1}, {2, 3} and 64 + those; tm + 16 {2 i, 2 i + 1} otherwise
+    f2_t acc[4][TN];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = both(0.f);
     if (q.K) {
         load(0);
         store(0);
@@ -76,37 +151,90 @@ __global__ void __launch_bounds__(kThreads) pointwise_kernel(Product q)
         if (more) load(k0 + kBK);
 #pragma unroll
         for (int k = 0; k < kBK; ++k) {
-            float av[8], bv[TN];
-            *reinterpret_cast<float4 *>(av) = *reinterpret_cast<const float4 *>(&As[b][k][4 * tm]);
-            *reinterpret_cast<float4 *>(av + 4) = *reinterpret_cast<const float4 *>(&As[b][k][64 + 4 * tm]);
+            f2_t av[4], bv[TN];
+            if constexpr (VEC) {
+                const ulonglong2 u = *reinterpret_cast<const ulonglong2 *>(&As[b][k][4 * tm]), v = *reinterpret_cast<const ulonglong2 *>(&As[b][k][64 + 4 * tm]);
+                av[0] = u.x;
+                av[1] = u.y;
+                av[2] = v.x;
+                av[3] = v.y;
+            } else {
 #pragma unroll
-            for (int j = 0; j < TN; j += 4) *reinterpret_cast<float4 *>(bv + j) = *reinterpret_cast<const float4 *>(&Bs[b][k][8 * j + 4 * tn]);
+                for (int i = 0; i < 4; ++i) av[i] = pack2(As[b][k][tm + 32 * i], As[b][k][tm + 32 * i + 16]);
+            }
+            // channel 32 (j / 4) + 4 tn + j % 4
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
+            for (int j = 0; j < TN; j += 2) {
+                const ulonglong2 u = *reinterpret_cast<const ulonglong2 *>(&Bs[b][k][32 * (j / 4) + 4 * tn + j % 4]);
+                bv[j] = u.x;
+                bv[j + 1] = u.y;
+            }
 #pragma unroll
-                for (int j = 0; j < TN; ++j) acc[i][j] = fmaf(av[i], bv[j], acc[i][j]);
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) acc[i][j] = fma2(av[i], bv[j], acc[i][j]);
         }
         if (more) store(b ^ 1);
         __syncthreads();
     }
 
-    // pixel 64 * (i / 4) + 4 * tm + i % 4, channel 32 * (j / 4) + 4 * tn + j % 4 of the tile
     const int64_t base = sample * q.Cn * q.P + (LAST ? p0 * q.Cn : p0);
     const T *bias = static_cast<const T *>(q.bias), *residual = static_cast<const T *>(q.residual), *grad = static_cast<const T *>(q.grad);
     T *out = static_cast<T *>(q.out);
 #pragma unroll
-    for (int j = 0; j < TN; ++j) {
-        const int n = n0 + 32 * (j / 4) + 4 * tn + j % 4;
-        if (n >= q.Cn) continue;
-        const float b = MODE != INPUT && bias ? to_float(bias[n]) : 0.f;
+    for (int j4 = 0; j4 < TN; j4 += 4) {
+        const int n = n0 + 8 * j4 + 4 * tn;      // four channels from here
+        float b4[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int m = 64 * (i / 4) + 4 * tm + i % 4;
-            if (m >= pixels) continue;
-            const int64_t at = base + (LAST ? (int64_t)m * q.Cn + n : n * q.P + m);
-            float z = acc[i][j] + b;
-            if (MODE != INPUT && residual) z += to_float(residual[at]);
-            out[at] = from_float<T>(MODE == FORWARD ? activate<ACT, T>(z) : MODE == SLOPE ? times_slope<ACT, T>(to_float(grad[at]), z) : z);
+        for (int j = 0; j < 4; ++j) b4[j] = MODE != INPUT && bias && n + j < q.Cn ? to_float(bias[n + j]) : 0.f;
+        if constexpr (VEC && LAST) {
+            if (n < q.Cn)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int m = 64 * (i / 4) + 4 * tm + i % 4;
+                    if (m >= pixels) continue;
+                    float z[4], other;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if (i % 2) unpack2(acc[i / 2][j4 + j], other, z[j]);
+                        else unpack2(acc[i / 2][j4 + j], z[j], other);
+                    }
+                    finish4<T, MODE, ACT, VEC>(q, base + (int64_t)m * q.Cn + n, z, b4);
+                }
+        } else if constexpr (VEC) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (n + j >= q.Cn) continue;
+                const float bj[4] = {b4[j], b4[j], b4[j], b4[j]};
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int m = 64 * h + 4 * tm;
+                    if (m >= pixels) continue;
+                    float z[4];
+                    unpack2(acc[2 * h][j4 + j], z[0], z[1]);
+                    unpack2(acc[2 * h + 1][j4 + j], z[2], z[3]);
+                    finish4<T, MODE, ACT, VEC>(q, base + (n + j) * q.P + m, z, bj);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (n + j >= q.Cn) continue;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float z[2];
+                    unpack2(acc[i][j4 + j], z[0], z[1]);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int m = tm + 32 * i + 16 * h;
+                        if (m >= pixels) continue;
+                        const int64_t at = base + (LAST ? (int64_t)m * q.Cn + n + j : (n + j) * q.P + m);
+                        float v = z[h] + b4[j];
+                        if (MODE != INPUT && residual) v += to_float(residual[at]);
+                        out[at] = from_float<T>(MODE == FORWARD ? activate<ACT, T>(v) : MODE == SLOPE ? times_slope<ACT, T>(to_float(grad[at]), v) : v);
+                    }
+                }
+            }
         }
     }
 }
@@ -122,76 +250,134 @@ struct WeightProduct {
     bool sums;               // the sums of dz too
 };
 
-constexpr int kBO = 64, kBI = 64;
-
-// D's tile: kBO x kBI weights, summed over a split's pixels.
-template <typename T, bool LAST>
-__global__ void __launch_bounds__(kThreads) pointwise_weight_kernel(WeightProduct q)
+// D's tile: BO x 2048 / BO * 2 weights (32 x 128 or 64 x 64), summed over a split's pixels; 8 x 4 sums a thread, two output
+// channels an instruction.  VEC: rows and arrays allow vectors of four values.
+template <typename T, bool LAST, int BO, bool VEC>
+__global__ void __launch_bounds__(kThreads, 4) pointwise_weight_kernel(WeightProduct q)
 {
-    __shared__ __align__(16) float As[2][kBK][kBO + 4], Bs[2][kBK][kBI + 4];
-    const int tid = threadIdx.x, tm = tid & 7, tn = tid >> 3;      // 8 x 16 threads, 8 x 4 sums each
+    constexpr int BI = 4096 / BO, NA = BO * kBK / kThreads, NB = BI * kBK / kThreads;
+    __shared__ __align__(16) float As[2][kBK][BO + 4];
+    __shared__ __align__(16) float2 Bs[2][kBK][BI + 2];
+    const int tid = threadIdx.x, tm = tid % (BO / 8), tn = tid / (BO / 8);
     const int tiles = q.tiles_o * q.tiles_i, split = blockIdx.x / tiles, t = blockIdx.x - split * tiles;
-    const int o0 = t / q.tiles_i * kBO, i0 = t % q.tiles_i * kBI;
+    const int o0 = t / q.tiles_i * BO, i0 = t % q.tiles_i * BI;
     const T *dz = static_cast<const T *>(q.dz), *x = static_cast<const T *>(q.x);
     grid_dependency_wait();
-    float acc[8][4] = {}, sum = 0.f;
-    const int64_t pieces = (int64_t)q.N * q.chunks, first = (int64_t)split * q.per, last = min(pieces, first + q.per);
-    for (int64_t piece = first; piece < last; ++piece) {
+    f2_t acc[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = both(0.f);
+    float sum = 0.f;
+    const int64_t pieces = (int64_t)q.N * q.chunks, end = min(pieces, (int64_t)(split + 1) * q.per);
+    int64_t piece = (int64_t)split * q.per;
+    int pixels = 0, k0 = 0;
+    const T *a = nullptr, *b = nullptr;
+    auto enter = [&] {      // the piece's first slice
         const int64_t sample = piece / q.chunks, p0 = (piece - sample * q.chunks) * q.chunk;
-        const int pixels = (int)min((int64_t)q.chunk, q.P - p0);
-        const T *a = dz + (sample * q.Co * q.P + (LAST ? p0 * q.Co : p0)), *b = x + (sample * q.Ci * q.P + (LAST ? p0 * q.Ci : p0));
-        float ra[8], rb[8];
-        auto load = [&](int k0) {
+        pixels = (int)min((int64_t)q.chunk, q.P - p0);
+        a = dz + (sample * q.Co * q.P + (LAST ? p0 * q.Co : p0));
+        b = x + (sample * q.Ci * q.P + (LAST ? p0 * q.Ci : p0));
+        k0 = 0;
+    };
+    float ra[NA], rb[NB];
+    // `n` values of one operand: channels c0 + {0 .. B - 1} of C
+    auto fetch = [&](auto size, const T *from, int c0, int C, auto &r) {
+        constexpr int B = decltype(size)::value;
+        if constexpr (VEC) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {      // LAST: channels run along the threads, pixels otherwise
-                const int k = k0 + (LAST ? (tid >> 6) + 2 * j : tid & 15), c = LAST ? tid & 63 : (tid >> 4) + 8 * j;
-                ra[j] = k < pixels && o0 + c < q.Co ? to_float(a[LAST ? (int64_t)k * q.Co + o0 + c : (o0 + c) * q.P + k]) : 0.f;
-                rb[j] = k < pixels && i0 + c < q.Ci ? to_float(b[LAST ? (int64_t)k * q.Ci + i0 + c : (i0 + c) * q.P + k]) : 0.f;
+            for (int j = 0; j < B * kBK / kThreads / 4; ++j) {
+                const int e = tid + kThreads * j, k = k0 + (LAST ? e / (B / 4) : 4 * (e & 3)), c = c0 + (LAST ? 4 * (e % (B / 4)) : e >> 2);
+                *reinterpret_cast<float4 *>(&r[4 * j]) =
+                    k < pixels && c < C ? load4(from + (LAST ? (int64_t)k * C + c : c * q.P + k)) : make_float4(0.f, 0.f, 0.f, 0.f);
             }
-        };
-        auto store = [&](int s) {
+        } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int k = LAST ? (tid >> 6) + 2 * j : tid & 15, c = LAST ? tid & 63 : (tid >> 4) + 8 * j;
-                As[s][k][c] = ra[j];
-                Bs[s][k][c] = rb[j];
+            for (int j = 0; j < B * kBK / kThreads; ++j) {
+                const int e = tid + kThreads * j, k = k0 + (LAST ? e / B : e & 15), c = c0 + (LAST ? e % B : e >> 4);
+                r[j] = k < pixels && c < C ? to_float(from[LAST ? (int64_t)k * C + c : c * q.P + k]) : 0.f;
             }
-        };
-        load(0);
+        }
+    };
+    auto place = [&](auto size, const auto &r, auto &&put) {      // put(k, channel, value)
+        constexpr int B = decltype(size)::value;
+#pragma unroll
+        for (int j = 0; j < B * kBK / kThreads; ++j) {
+            if constexpr (VEC) {
+                const int e = tid + kThreads * (j / 4);
+                put(LAST ? e / (B / 4) : 4 * (e & 3) + j % 4, LAST ? 4 * (e % (B / 4)) + j % 4 : e >> 2, r[j]);
+            } else {
+                const int e = tid + kThreads * j;
+                put(LAST ? e / B : e & 15, LAST ? e % B : e >> 4, r[j]);
+            }
+        }
+    };
+    auto load = [&] {
+        fetch(std::integral_constant<int, BO>(), a, o0, q.Co, ra);
+        fetch(std::integral_constant<int, BI>(), b, i0, q.Ci, rb);
+    };
+    auto store = [&](int s) {
+        place(std::integral_constant<int, BO>(), ra, [&](int k, int c, float v) { As[s][k][c] = v; });
+        place(std::integral_constant<int, BI>(), rb, [&](int k, int c, float v) { Bs[s][k][c] = make_float2(v, v); });
+    };
+    auto advance = [&] {      // to the next slice; false behind the last
+        k0 += kBK;
+        if (k0 < pixels) return true;
+        if (++piece >= end) return false;
+        enter();
+        return true;
+    };
+    if (piece < end) {
+        enter();
+        load();
         store(0);
         __syncthreads();
-        for (int k0 = 0, s = 0; k0 < pixels; k0 += kBK, s ^= 1) {
-            const bool more = k0 + kBK < pixels;
-            if (more) load(k0 + kBK);
+        for (int s = 0;; s ^= 1) {
+            const bool more = advance();
+            if (more) load();
 #pragma unroll
             for (int k = 0; k < kBK; ++k) {
-                float av[8], bv[4];
-                *reinterpret_cast<float4 *>(av) = *reinterpret_cast<const float4 *>(&As[s][k][4 * tm]);
-                *reinterpret_cast<float4 *>(av + 4) = *reinterpret_cast<const float4 *>(&As[s][k][32 + 4 * tm]);
-                *reinterpret_cast<float4 *>(bv) = *reinterpret_cast<const float4 *>(&Bs[s][k][4 * tn]);
+                f2_t av[4], bv[4];
+                ulonglong2 u = *reinterpret_cast<const ulonglong2 *>(&As[s][k][4 * tm]);
+                av[0] = u.x;
+                av[1] = u.y;
+                u = *reinterpret_cast<const ulonglong2 *>(&As[s][k][BO / 2 + 4 * tm]);
+                av[2] = u.x;
+                av[3] = u.y;
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
+                for (int j = 0; j < 4; j += 2) {
+                    u = *reinterpret_cast<const ulonglong2 *>(&Bs[s][k][4 * tn + j]);
+                    bv[j] = u.x;
+                    bv[j + 1] = u.y;
+                }
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(av[i], bv[j], acc[i][j]);
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[i][j] = fma2(av[i], bv[j], acc[i][j]);
             }
-            if (q.sums && i0 == 0 && tid < kBO) {
+            if (q.sums && i0 == 0 && tid < BO) {
 #pragma unroll
                 for (int k = 0; k < kBK; ++k) sum += As[s][k][tid];
             }
-            if (more) store(s ^ 1);
+            if (!more) break;
+            store(s ^ 1);
             __syncthreads();
         }
     }
     float *partial = q.partial + split * pointwise_partial_stride(q.Co, q.Ci);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int o = o0 + 32 * (i / 4) + 4 * tm + i % 4;
-        if (o >= q.Co) continue;
+    for (int i = 0; i < 4; ++i) {
+        const int o = o0 + BO / 2 * (i / 2) + 4 * tm + 2 * (i % 2);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (i0 + 4 * tn + j < q.Ci) partial[(int64_t)o * q.Ci + i0 + 4 * tn + j] = acc[i][j];
+        for (int j = 0; j < 4; ++j) {
+            float v[2];
+            unpack2(acc[i][j], v[0], v[1]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                if (o + h < q.Co && i0 + 4 * tn + j < q.Ci) partial[(int64_t)(o + h) * q.Ci + i0 + 4 * tn + j] = v[h];
+        }
     }
-    if (q.sums && i0 == 0 && tid < kBO && o0 + tid < q.Co) partial[(int64_t)q.Co * q.Ci + o0 + tid] = sum;
+    if (q.sums && i0 == 0 && tid < BO && o0 + tid < q.Co) partial[(int64_t)q.Co * q.Ci + o0 + tid] = sum;
 }
 
 // Rows of partial sums, added in a fixed order, rounded once: `count` columns, `stride` floats from row to row.
@@ -241,27 +427,35 @@ int launch_product(const PointwiseShape &s, Product q, cudaStream_t stream)
             using T = decltype(t);
             constexpr int ACT = MODE == INPUT ? BC_ACT_NONE : act();
             const LaunchScope scope(KID_POINTWISE, stream);
-            if (s.last) bn == 32 ? launch_overlapped(pointwise_kernel<T, MODE, ACT, true, 32>, grid, kThreads, 0, stream, q)
-                                 : launch_overlapped(pointwise_kernel<T, MODE, ACT, true, 64>, grid, kThreads, 0, stream, q);
-            else bn == 32 ? launch_overlapped(pointwise_kernel<T, MODE, ACT, false, 32>, grid, kThreads, 0, stream, q)
-                          : launch_overlapped(pointwise_kernel<T, MODE, ACT, false, 64>, grid, kThreads, 0, stream, q);
-            return check_launch("pointwise_kernel");
+            auto go = [&](auto last, auto vec) {
+                constexpr bool LAST = decltype(last)::value, VEC = decltype(vec)::value;
+                bn == 32 ? launch_overlapped(pointwise_kernel<T, MODE, ACT, LAST, 32, VEC>, grid, kThreads, 0, stream, q)
+                         : launch_overlapped(pointwise_kernel<T, MODE, ACT, LAST, 64, VEC>, grid, kThreads, 0, stream, q);
+                return check_launch("pointwise_kernel");
+            };
+            const bool vec = (s.last ? q.K % 4 == 0 && q.Cn % 4 == 0 : q.P % 4 == 0) && pointwise_mma_aligned(q.a, q.residual, q.grad, q.out);
+            if (s.last) return vec ? go(std::true_type(), std::true_type()) : go(std::true_type(), std::false_type());
+            return vec ? go(std::false_type(), std::true_type()) : go(std::false_type(), std::false_type());
         });
     });
 }
 
-// How the pixels of grad_weight are split: pieces of whole slices of k, about two CTAs an SM, at least 256 pixels each.
+// How grad_weight is cut: tiles, and the pixels in pieces of at most 256, about four CTAs an SM.
 struct Splits {
     int chunk, chunks, per, splits;
+    int bo, tiles_o, tiles_i;
 };
 Splits splits_of(const PointwiseShape &s)
 {
     const int64_t P = s.last ? s.N * s.P : s.P, samples = s.last ? 1 : s.N;
     Splits v;
+    v.bo = s.Co <= 32 ? 32 : 64;
+    v.tiles_o = (int)ceil_div(s.Co, v.bo);
+    v.tiles_i = (int)ceil_div(s.Ci ? s.Ci : 1, 4096 / v.bo);
     v.chunk = (int)(P < 256 ? P : 256);
     v.chunks = (int)ceil_div(P, v.chunk);
-    const int64_t pieces = samples * v.chunks, tiles = ceil_div(s.Co, kBO) * ceil_div(s.Ci ? s.Ci : 1, kBI);
-    const int64_t wanted = tiles > 296 ? 1 : 296 / tiles;
+    const int64_t pieces = samples * v.chunks, tiles = (int64_t)v.tiles_o * v.tiles_i;
+    const int64_t wanted = tiles > 592 ? 1 : 592 / tiles;
     v.per = (int)ceil_div(pieces, wanted);
     v.splits = (int)ceil_div(pieces, v.per);
     return v;
@@ -337,16 +531,22 @@ int launch_pointwise_backward(const PointwiseShape &s, const void *x, const void
         } else {
             const Splits v = splits_of(s);
             splits = v.splits;
-            WeightProduct q{dz, x, partial, s.last ? 1 : s.N, s.Ci, s.Co, s.last ? s.N * s.P : s.P, (int)ceil_div(s.Co, kBO),
-                            (int)ceil_div(s.Ci ? s.Ci : 1, kBI), v.chunk, v.chunks, v.per, want_bias && !sums};
+            WeightProduct q{dz, x, partial, s.last ? 1 : s.N, s.Ci, s.Co, s.last ? s.N * s.P : s.P, v.tiles_o, v.tiles_i, v.chunk, v.chunks, v.per,
+                            want_bias && !sums};
             const int64_t ctas = (int64_t)v.splits * q.tiles_o * q.tiles_i;
             if (ctas > INT32_MAX) return BC_ERR_BAD_SHAPE;
+            const bool vec = (s.last ? s.Ci % 4 == 0 && s.Co % 4 == 0 : s.P % 4 == 0) && pointwise_mma_aligned(dz, x);
             e = with_type(s.io_kind, [&](auto t) {
                 using T = decltype(t);
-                const LaunchScope scope(KID_POINTWISE_WEIGHT, stream);
-                if (s.last) launch_overlapped(pointwise_weight_kernel<T, true>, (unsigned)ctas, kThreads, 0, stream, q);
-                else launch_overlapped(pointwise_weight_kernel<T, false>, (unsigned)ctas, kThreads, 0, stream, q);
-                return check_launch("pointwise_weight_kernel");
+                auto go = [&](auto last, auto aligned) {
+                    constexpr bool LAST = decltype(last)::value, VEC = decltype(aligned)::value;
+                    const LaunchScope scope(KID_POINTWISE_WEIGHT, stream);
+                    v.bo == 32 ? launch_overlapped(pointwise_weight_kernel<T, LAST, 32, VEC>, (unsigned)ctas, kThreads, 0, stream, q)
+                               : launch_overlapped(pointwise_weight_kernel<T, LAST, 64, VEC>, (unsigned)ctas, kThreads, 0, stream, q);
+                    return check_launch("pointwise_weight_kernel");
+                };
+                if (s.last) return vec ? go(std::true_type(), std::true_type()) : go(std::true_type(), std::false_type());
+                return vec ? go(std::false_type(), std::true_type()) : go(std::false_type(), std::false_type());
             });
         }
         if (e) return e;
