@@ -275,6 +275,16 @@ int pointwise_mma_weight_splits(const PointwiseShape &s);
 int launch_pointwise_mma_weight(const PointwiseShape &s, const void *dz, const void *x, float *partial, bool sums, cudaStream_t stream);
 int read_wait_timeouts_mma(int *count);
 
+// The same with operands made by threads (pointwise_split.cu): floats as sums of bf16, rows of any alignment.
+bool pointwise_split_suits(const PointwiseShape &s, bool input);
+int pointwise_split_sums_rows(const PointwiseShape &s);
+int launch_pointwise_split_forward(const PointwiseShape &s, const void *x, const void *weight, const void *bias, const void *residual,
+                                   void *out, cudaStream_t stream);
+int launch_pointwise_split_slope(const PointwiseShape &s, const void *x, const void *weight, const void *bias, const void *residual,
+                                 const void *grad, void *dz, float *sums, cudaStream_t stream);
+int launch_pointwise_split_input(const PointwiseShape &s, const void *dz, const void *weight, void *grad_input, cudaStream_t stream);
+int read_wait_timeouts_split(int *count);
+
 size_t pointwise_workspace(const PointwiseShape &s, int need_mask);
 int launch_pointwise_forward(const PointwiseShape &s, const void *x, const void *weight, const void *bias, const void *residual, void *out,
                              cudaStream_t stream);

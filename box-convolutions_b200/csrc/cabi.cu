@@ -738,10 +738,11 @@ uint64_t bc_launch_count(void) { return g_launches.load(); }
 int bc_wait_timeouts(int *count)
 {
     if (!count) return BC_ERR_NULL_POINTER;
-    int mma = 0;
+    int mma = 0, split = 0;
     if (const int e = read_wait_timeouts_mma(&mma)) return e;
+    if (const int e = read_wait_timeouts_split(&split)) return e;
     const int e = read_wait_timeouts(count);
-    if (!e) *count += mma;
+    if (!e) *count += mma + split;
     return e;
 }
 
@@ -813,6 +814,7 @@ const char *bc_kernel_name(int kernel_id)
         case KID_POINTWISE_FINISH: return "pointwise_finish_kernel";
         case KID_POINTWISE_MMA: return "pointwise_mma_kernel";
         case KID_POINTWISE_WEIGHT_MMA: return "pointwise_weight_mma_kernel";
+        case KID_POINTWISE_SPLIT: return "pointwise_split_kernel";
         case KID_NORM_FORWARD: return "norm_forward_kernel";
         case KID_NORM_BACKWARD: return "norm_backward_kernel";
         case KID_NORM_FINISH: return "norm_finish_kernel";

@@ -466,7 +466,22 @@ size_t partial_bytes(const PointwiseShape &s)
     // (either kernel's: the query does not know the arrays)
     return align_up((size_t)std::max(splits_of(s).splits, pointwise_mma_weight_splits(s)) * pointwise_partial_stride(s.Co, s.Ci) * sizeof(float));
 }
-size_t sums_bytes(const PointwiseShape &s) { return align_up((size_t)pointwise_mma_sums_rows(s) * s.Co * sizeof(float)); }
+// Which kernel a product with pixels in the rows takes.
+enum { BY_TMA, BY_SPLIT, BY_FMA };
+int way_of(const PointwiseShape &s, bool input, bool aligned)
+{
+    if (aligned && pointwise_mma_suits(s, input)) return BY_TMA;
+    return pointwise_split_suits(s, input) ? BY_SPLIT : BY_FMA;
+}
+int sums_rows(const PointwiseShape &s, int way)
+{
+    return way == BY_TMA ? pointwise_mma_sums_rows(s) : way == BY_SPLIT ? pointwise_split_sums_rows(s) : 0;
+}
+// (for either: the query does not know the arrays)
+size_t sums_bytes(const PointwiseShape &s)
+{
+    return align_up((size_t)std::max(sums_rows(s, way_of(s, false, true)), sums_rows(s, way_of(s, false, false))) * s.Co * sizeof(float));
+}
 // dz in memory, where it is neither grad_output itself nor asked for.
 bool own_dz(const PointwiseShape &s, int need_mask) { return s.act != BC_ACT_NONE && !(need_mask & BC_NEED_PW_RESIDUAL); }
 
@@ -475,8 +490,9 @@ bool own_dz(const PointwiseShape &s, int need_mask) { return s.act != BC_ACT_NON
 int launch_pointwise_forward(const PointwiseShape &s, const void *x, const void *weight, const void *bias, const void *residual, void *out,
                              cudaStream_t stream)
 {
-    if (pointwise_mma_suits(s, false) && pointwise_mma_aligned(x, weight, residual, out))
-        return launch_pointwise_mma_forward(s, x, weight, bias, residual, out, stream);
+    const int way = way_of(s, false, pointwise_mma_aligned(x, weight, residual, out));
+    if (way == BY_TMA) return launch_pointwise_mma_forward(s, x, weight, bias, residual, out, stream);
+    if (way == BY_SPLIT) return launch_pointwise_split_forward(s, x, weight, bias, residual, out, stream);
     return launch_product<FORWARD>(s, {x, weight, bias, residual, nullptr, out, s.Ci, s.Co, s.Ci, 1}, stream);
 }
 
@@ -484,7 +500,7 @@ size_t pointwise_workspace(const PointwiseShape &s, int need_mask)
 {
     size_t bytes = own_dz(s, need_mask) ? align_up((size_t)io_size(s.io_kind) * s.N * s.Co * s.P) : 0;
     if (need_mask & (BC_NEED_PW_WEIGHT | BC_NEED_PW_BIAS)) bytes += partial_bytes(s);
-    if ((need_mask & BC_NEED_PW_BIAS) && s.act != BC_ACT_NONE && pointwise_mma_suits(s, false)) bytes += sums_bytes(s);
+    if ((need_mask & BC_NEED_PW_BIAS) && s.act != BC_ACT_NONE) bytes += sums_bytes(s);
     return bytes;
 }
 
@@ -500,29 +516,32 @@ int launch_pointwise_backward(const PointwiseShape &s, const void *x, const void
     };
     const bool want_weight = need_mask & BC_NEED_PW_WEIGHT, want_bias = need_mask & BC_NEED_PW_BIAS;
     const void *dz = grad;
-    float *sums = nullptr;      // of dz as it was before its rounding
+    float *sums = nullptr;      // rows of sums of dz as it was before its rounding
+    int rows = 0;
     if (s.act != BC_ACT_NONE) {
         void *to = own_dz(s, need_mask) ? take(align_up((size_t)io_size(s.io_kind) * s.N * s.Co * s.P)) : grad_residual;
-        int e;
-        if (pointwise_mma_suits(s, false) && pointwise_mma_aligned(x, weight, residual, grad, to)) {
-            if (want_bias) sums = static_cast<float *>(take(sums_bytes(s)));
-            e = launch_pointwise_mma_slope(s, x, weight, bias, residual, grad, to, sums, stream);
-        } else {
-            e = launch_product<SLOPE>(s, {x, weight, bias, residual, grad, to, s.Ci, s.Co, s.Ci, 1}, stream);
+        const int way = way_of(s, false, pointwise_mma_aligned(x, weight, residual, grad, to));
+        if (want_bias && way != BY_FMA) {
+            sums = static_cast<float *>(take(sums_bytes(s)));
+            rows = sums_rows(s, way);
         }
+        const int e = way == BY_TMA     ? launch_pointwise_mma_slope(s, x, weight, bias, residual, grad, to, sums, stream)
+                      : way == BY_SPLIT ? launch_pointwise_split_slope(s, x, weight, bias, residual, grad, to, sums, stream)
+                                        : launch_product<SLOPE>(s, {x, weight, bias, residual, grad, to, s.Ci, s.Co, s.Ci, 1}, stream);
         if (e) return e;
         dz = to;
     }
     if (need_mask & BC_NEED_PW_INPUT) {
-        const int e = pointwise_mma_suits(s, true) && pointwise_mma_aligned(dz, weight, grad_input)
-                          ? launch_pointwise_mma_input(s, dz, weight, grad_input, stream)
-                          : launch_product<INPUT>(s, {dz, weight, nullptr, nullptr, nullptr, grad_input, s.Co, s.Ci, 1, s.Ci}, stream);
+        const int way = way_of(s, true, pointwise_mma_aligned(dz, weight, grad_input));
+        const int e = way == BY_TMA     ? launch_pointwise_mma_input(s, dz, weight, grad_input, stream)
+                      : way == BY_SPLIT ? launch_pointwise_split_input(s, dz, weight, grad_input, stream)
+                                        : launch_product<INPUT>(s, {dz, weight, nullptr, nullptr, nullptr, grad_input, s.Co, s.Ci, 1, s.Ci}, stream);
         if (e) return e;
     }
     if (!want_weight && !want_bias) return BC_OK;
     const int64_t weights = (int64_t)s.Co * s.Ci;
     Partials of_weights{}, of_sums{};
-    if (sums) of_sums = {sums, s.Co, s.Co, pointwise_mma_sums_rows(s), grad_bias};
+    if (sums) of_sums = {sums, s.Co, s.Co, rows, grad_bias};
     if (want_weight || !sums) {
         float *partial = static_cast<float *>(take(partial_bytes(s)));
         int splits = pointwise_mma_weight_splits(s), e;

@@ -1,0 +1,476 @@
+// Pointwise convolutions on the tensor cores with operands that threads bring into shared memory: float tensors, and 16-bit
+// ones whose rows TMA does not take (odd planes, channels that are no multiple of eight).  The products of pointwise.cu with
+// pixels in the rows, built like pointwise_mma_kernel: persistent CTAs, weights in shared memory, two sets of accumulators.
+//
+// A float is the sum of three bf16 values, its upper, middle and lower eight bits, so a product of floats is that of nine
+// pairs; the six that reach above 2^-24 of it are made: the upper ones into one accumulator, the others into a second, added at
+// the end.  (An accumulator's additions round towards zero: the second stays 2^-8 of the first, and the first sees a
+// sixth of the additions.)  Measured against multiply-adds, which wait for shared memory here ((16,128->32,64,128) planes: 38 us).
+// Infinities and NaN have no such sum: a result that is not finite is computed again by multiply-adds.
+#include "bc_mma.cuh"
+
+namespace bc {
+
+namespace {
+
+enum { FORWARD, SLOPE, INPUT };
+constexpr int kEpilogue = 4, kGroups = 2, kGroupWarps = 4;
+constexpr int kThreads = 32 * (kEpilogue + kGroups * kGroupWarps + 1);
+constexpr int kPitch = 33;
+constexpr uint32_t kPart = 16384;      // 128 pixels x 64 k
+constexpr uint32_t kMostShared = 227 << 10;
+
+template <typename T>
+constexpr int kParts = sizeof(T) == 4 ? 3 : 1;
+
+struct SplitProduct {
+    const void *a, *w, *bias, *residual, *grad;
+    void *out;
+    float *sums;             // SLOPE: [CTA / tiles_n][Cn] sums of dz over the CTA's pixels, or null
+    int64_t P;               // pixels of a sample (of all of them together, channels last)
+    int K, Cn, samples;
+    int wn, wk;              // strides of W along the output's and the operand's channels
+    int tiles_p, tiles_n;
+    int bn, stages, columns;
+    uint32_t instruction;
+};
+
+// Shared memory from a 1024-byte boundary on.
+struct SplitLayout {
+    int bn, stages, chunks, parts;
+    bool last;
+    __host__ __device__ uint32_t slice() const { return (uint32_t)bn * 128; }      // 64 k of one part of the weights
+    __host__ __device__ uint32_t ring() const { return parts * chunks * slice(); }
+    __host__ __device__ uint32_t staging() const { return ring() + stages * parts * kPart; }
+    __host__ __device__ uint32_t bias() const { return staging() + (last ? kEpilogue * 32 * kPitch * 4 : 0); }
+    __host__ __device__ uint32_t sums() const { return bias() + bn * 4; }
+    __host__ __device__ uint32_t barriers() const { return (sums() + 4 * bn * 4 + 7) / 8 * 8; }
+    __host__ __device__ uint32_t bytes() const { return barriers() + (2 * stages + 4) * 8 + 8 + 1024; }
+};
+
+__device__ __forceinline__ float upper(float v) { return __uint_as_float(__float_as_uint(v) & 0xffff0000u); }
+// What is left of v without its upper part; nothing of an infinity.
+__device__ __forceinline__ float rest(float v, float u) { return v == u ? 0.f : v - u; }
+__device__ __forceinline__ uint32_t halves(float lo, float hi) { return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632); }
+
+// Eight floats as three vectors of bf16.
+__device__ __forceinline__ void split8(const float (&v)[8], uint4 (&part)[3])
+{
+    uint32_t w[3][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float x[2] = {v[2 * i], v[2 * i + 1]};
+#pragma unroll
+        for (int p = 0; p < 3; ++p) {
+            w[p][i] = halves(x[0], x[1]);
+            x[0] = rest(x[0], upper(x[0]));
+            x[1] = rest(x[1], upper(x[1]));
+        }
+    }
+#pragma unroll
+    for (int p = 0; p < 3; ++p) part[p] = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
+}
+
+// Sums of 32 values over the warp's lanes, value j's in lane j.
+__device__ __forceinline__ float transposed_sum(float (&v)[32], int lane)
+{
+#pragma unroll
+    for (int w = 16; w; w >>= 1)
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+            if (j < w) {
+                const bool high = lane & w;
+                const float keep = high ? v[j + w] : v[j], send = high ? v[j] : v[j + w];
+                v[j] = keep + __shfl_xor_sync(0xffffffffu, send, w);
+            }
+    return v[0];
+}
+
+template <typename T, int MODE, int ACT, bool LAST, bool VEC>
+__global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const SplitProduct q)
+{
+    constexpr int PARTS = kParts<T>;
+    extern __shared__ char raw_smem[];
+    const uint32_t raw = smem_u32(raw_smem), base = (raw + 1023) & ~1023u;
+    char *smem = raw_smem + (base - raw);
+    const int chunks = (q.K + 63) / 64;
+    const SplitLayout lay{q.bn, q.stages, chunks, PARTS, LAST};
+    float *bias_smem = reinterpret_cast<float *>(smem + lay.bias()), *sums_smem = reinterpret_cast<float *>(smem + lay.sums());
+    const uint32_t full = base + lay.barriers(), empty = full + 8 * q.stages, ready = empty + 8 * q.stages, drained = ready + 16;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + lay.barriers() + (2 * q.stages + 4) * 8);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const unsigned walkers = gridDim.x / (unsigned)q.tiles_n, walker = blockIdx.x / (unsigned)q.tiles_n;
+    const int n0 = (int)(blockIdx.x - walker * q.tiles_n) * q.bn;
+    const int64_t tiles = (int64_t)q.samples * q.tiles_p;
+    const uint32_t set_columns = (PARTS > 1 ? 2 : 1) * q.columns;
+    const T *w_all = static_cast<const T *>(q.w), *a_all = static_cast<const T *>(q.a);
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < q.stages; ++i) {
+            mbar_init(full + 8 * i, kGroupWarps);
+            mbar_init(empty + 8 * i, 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(ready + 8 * i, 1);
+            mbar_init(drained + 8 * i, kEpilogue);
+        }
+        fence_mbar_init();
+    }
+    __syncthreads();
+    grid_dependency_wait();
+    if (warp == kEpilogue + kGroups * kGroupWarps) tmem_alloc(tmem_slot, 2 * set_columns);
+    for (int i = threadIdx.x; i < q.bn; i += kThreads)
+        bias_smem[i] = MODE != INPUT && q.bias && n0 + i < q.Cn ? to_float(static_cast<const T *>(q.bias)[n0 + i]) : 0.f;
+    for (int i = threadIdx.x; i < 4 * q.bn; i += kThreads) sums_smem[i] = 0.f;
+    // the weights, K-major, eight k a thread
+    {
+        for (int e = threadIdx.x; e < q.bn * chunks * 8; e += kThreads) {
+            // (along the weights' rows: k forward, channels for grad_input)
+            const int n = MODE == INPUT ? e % q.bn : e / (chunks * 8), k8 = MODE == INPUT ? e / q.bn : e % (chunks * 8);
+            float v[8];
+            uint4 part[3];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int k = 8 * k8 + j;
+                v[j] = k < q.K && n0 + n < q.Cn ? to_float(w_all[(int64_t)(n0 + n) * q.wn + (int64_t)k * q.wk]) : 0.f;
+            }
+            if constexpr (PARTS == 3) split8(v, part);
+            else part[0] = pack<T>(v);
+            char *to = smem + (k8 >> 3) * lay.slice() + n * 128 + (((k8 & 7) ^ (n & 7)) << 4);
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p) *reinterpret_cast<uint4 *>(to + p * chunks * lay.slice()) = part[p];
+        }
+    }
+    fence_proxy_async();
+    tmem_release();
+    __syncthreads();
+    tmem_acquire();
+    const uint32_t tmem = *tmem_slot;
+    Waiter wait;
+
+    if (warp >= kEpilogue && warp < kEpilogue + kGroups * kGroupWarps) {
+        // group g brings every second slice: while one waits for memory the other writes
+        const int group = (warp - kEpilogue) / kGroupWarps, t = threadIdx.x - 32 * (kEpilogue + group * kGroupWarps);
+        int64_t slice = group;      // counts this CTA's slices
+        const int64_t my_tiles = walker < tiles ? (tiles - walker + walkers - 1) / walkers : 0;
+        for (; slice < my_tiles * chunks; slice += kGroups) {
+            const int64_t nth = slice / chunks, tile = walker + nth * walkers;
+            const int c = (int)(slice - nth * chunks), stage = (int)(slice % q.stages);
+            const uint32_t phase = (uint32_t)(slice / q.stages) & 1;
+            const int sample = (int)(tile / q.tiles_p);
+            const int64_t p0 = (tile - (int64_t)sample * q.tiles_p) * 128;
+            const int pixels = (int)min((int64_t)128, q.P - p0), k_left = q.K - 64 * c;
+            const T *a = a_all + (LAST ? p0 * q.K + 64 * c : ((int64_t)sample * q.K + 64 * c) * q.P + p0);
+            // a vector: planes, eight pixels of a k; last, eight k of a pixel.  `inner` of it are there.
+            uint4 raw_v[8][PARTS == 3 ? 2 : 1];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int e = t + 128 * j, in = 8 * (LAST ? e & 7 : e & 15), outer = LAST ? e >> 3 : e >> 4;
+                const int inner = outer < (LAST ? pixels : k_left) ? (LAST ? k_left : pixels) - in : 0;
+                const T *from = a + outer * (LAST ? (int64_t)q.K : q.P) + in;
+                if constexpr (VEC) {
+                    constexpr int EACH = 16 / sizeof(T);
+#pragma unroll
+                    for (int i = 0; i < 8 / EACH; ++i)
+                        raw_v[j][i] = inner > i * EACH ? *reinterpret_cast<const uint4 *>(from + i * EACH) : make_uint4(0, 0, 0, 0);
+                } else if constexpr (PARTS == 3) {
+                    float v[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] = i < inner ? to_float(from[i]) : 0.f;
+                    raw_v[j][0] = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+                    raw_v[j][1] = make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7]));
+                } else {
+                    const unsigned short *bits = reinterpret_cast<const unsigned short *>(from);
+                    uint32_t v[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] = i < inner ? bits[i] : 0;
+                    raw_v[j][0] = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
+                }
+            }
+            if (!wait(empty + 8 * stage, phase ^ 1)) break;
+            char *to = smem + lay.ring() + stage * PARTS * kPart;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int e = t + 128 * j;
+                const uint32_t at = LAST ? (e >> 3) * 128 + (((e & 7) ^ (e >> 3 & 7)) << 4)
+                                         : (e >> 3 & 1) * kBlockBytes + (e >> 4) * 128 + (((e & 7) ^ (e >> 4 & 7)) << 4);
+                if constexpr (PARTS == 3) {
+                    const uint4 &u = raw_v[j][0], &v = raw_v[j][1];
+                    const float f[8] = {__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w),
+                                        __uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w)};
+                    uint4 part[3];
+                    split8(f, part);
+#pragma unroll
+                    for (int p = 0; p < 3; ++p) *reinterpret_cast<uint4 *>(to + p * kPart + at) = part[p];
+                } else {
+                    *reinterpret_cast<uint4 *>(to + at) = raw_v[j][0];
+                }
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(full + 8 * stage);
+        }
+    } else if (warp == kEpilogue + kGroups * kGroupWarps) {
+        if (lane == 0) {
+            uint32_t stage = 0, phase = 0, set = 0, set_phase = 0;
+            for (int64_t tile = walker; tile < tiles; tile += walkers) {
+                if (!wait(drained + 8 * set, set_phase ^ 1)) break;
+                tmem_acquire();
+                for (int c = 0; c < chunks; ++c) {
+                    if (!wait(full + 8 * stage, phase)) break;
+                    tmem_acquire();
+                    const uint32_t a = base + lay.ring() + stage * PARTS * kPart, w = base + c * lay.slice();
+                    const int steps = (min(64, q.K - 64 * c) + 15) / 16;
+                    for (int k = 0; k < 16 * steps; k += 16) {
+#pragma unroll
+                        for (int i = 0; i < PARTS; ++i)
+#pragma unroll
+                            for (int j = 0; j < PARTS - i; ++j) {
+                                const uint32_t ai = a + i * kPart, wj = w + j * chunks * lay.slice();
+                                mma(tmem + set * set_columns + (i + j ? q.columns : 0), LAST ? k_major(ai, k) : mn_major(ai, k, kBlockBytes), k_major(wj, k),
+                                    q.instruction, c || k || i + j > 1 || i > 0);
+                            }
+                    }
+                    mma_commit(empty + 8 * stage);
+                    if (++stage == (uint32_t)q.stages) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                }
+                if (wait.lost) break;
+                mma_commit(ready + 8 * set);
+                if (set ^= 1; set == 0) set_phase ^= 1;
+            }
+        }
+    } else {
+        float *staging = reinterpret_cast<float *>(smem + lay.staging()) + warp * 32 * kPitch;
+        const int quarter = warp, blocks = (q.bn + 31) / 32;
+        const T *residual = static_cast<const T *>(q.residual), *grad = static_cast<const T *>(q.grad);
+        T *out = static_cast<T *>(q.out);
+        uint32_t set = 0, set_phase = 0;
+        for (int64_t tile = walker; tile < tiles; tile += walkers) {
+            const int sample = (int)(tile / q.tiles_p);
+            const int64_t p0 = (tile - (int64_t)sample * q.tiles_p) * 128 + quarter * 32;
+            const int rows = (int)max((int64_t)0, min((int64_t)32, q.P - p0));
+            wait(ready + 8 * set, set_phase);
+            __syncwarp();
+            tmem_acquire();
+            for (int b = 0; b < blocks; ++b) {
+                float v[32];
+                const uint32_t from = tmem + set * set_columns + 32 * b + ((uint32_t)quarter << 21);
+                tmem_load32(from, v);
+                if constexpr (PARTS == 3) {
+                    float u[32];
+                    tmem_load32(from + q.columns, u);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] += u[j];
+                    float finite = 0.f;
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) finite = fmaf(v[j], 0.f, finite);
+                    if (finite != 0.f && lane < rows) {      // (a NaN: some value is not finite)
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) u[j] = 0.f;
+                        for (int k = 0; k < q.K; ++k) {
+                            const float x = to_float(a_all[LAST ? (p0 + lane) * q.K + k : ((int64_t)sample * q.K + k) * q.P + p0 + lane]);
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) {
+                                const int c = n0 + 32 * b + j;
+                                if (c < q.Cn) u[j] = fmaf(x, to_float(w_all[(int64_t)c * q.wn + (int64_t)k * q.wk]), u[j]);
+                            }
+                        }
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (!(fabsf(v[j]) < INFINITY)) v[j] = u[j];
+                    }
+                }
+                const int c0 = n0 + 32 * b, channels = min(32, min(q.Cn - c0, q.bn - 32 * b));
+                if constexpr (LAST) {
+                    // a lane a channel, row after row
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) staging[lane * kPitch + j] = v[j];
+                    __syncwarp();
+                    const int64_t at = p0 * q.Cn + c0 + lane;
+                    const float bias = bias_smem[32 * b + (lane < channels ? lane : 0)];
+                    float total = 0.f;
+                    if (lane < channels) {
+#pragma unroll
+                        for (int r0 = 0; r0 < 32; r0 += 8) {
+                            float z[8], res[8], g[8];
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const bool there = r0 + i < rows;
+                                const int64_t e = at + (int64_t)(r0 + i) * q.Cn;
+                                if (MODE != INPUT) res[i] = residual && there ? to_float(residual[e]) : 0.f;
+                                if (MODE == SLOPE) g[i] = there ? to_float(grad[e]) : 0.f;
+                                z[i] = staging[(r0 + i) * kPitch + lane];
+                            }
+#pragma unroll
+                            for (int i = 0; i < 8; i += 2) {
+                                if (MODE != INPUT) {
+                                    const f2_t zz = pack2(z[i] + bias + res[i], z[i + 1] + bias + res[i + 1]);
+                                    unpack2(MODE == SLOPE ? times_slope2<ACT, T>(pack2(g[i], g[i + 1]), zz) : activate2<ACT, T>(zz), z[i], z[i + 1]);
+                                }
+#pragma unroll
+                                for (int h = 0; h < 2; ++h)
+                                    if (r0 + i + h < rows) {
+                                        if (MODE == SLOPE) total += z[i + h];
+                                        out[at + (int64_t)(r0 + i + h) * q.Cn] = from_float<T>(z[i + h]);
+                                    }
+                            }
+                        }
+                        if (MODE == SLOPE && q.sums) sums_smem[quarter * q.bn + 32 * b + lane] += total;
+                    }
+                    __syncwarp();
+                } else {
+                    // a lane a pixel, channel after channel
+                    const int64_t at = ((int64_t)sample * q.Cn + c0) * q.P + p0 + lane;
+                    const bool mine = lane < rows;
+#pragma unroll
+                    for (int j0 = 0; j0 < 32; j0 += 8) {
+                        float res[8], g[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const bool there = mine && j0 + i < channels;
+                            const int64_t e = at + (j0 + i) * q.P;
+                            if (MODE != INPUT) res[i] = residual && there ? to_float(residual[e]) : 0.f;
+                            if (MODE == SLOPE) g[i] = there ? to_float(grad[e]) : 0.f;
+                        }
+#pragma unroll
+                        for (int i = 0; i < 8; i += 2) {
+                            float &z0 = v[j0 + i], &z1 = v[j0 + i + 1];
+                            if (MODE != INPUT) {
+                                // (columns past the tile are there in memory, but hold nothing)
+                                const bool there = j0 + i < channels;
+                                const f2_t zz = pack2(there ? z0 + bias_smem[32 * b + j0 + i] + res[i] : 0.f,
+                                                      j0 + i + 1 < channels ? z1 + bias_smem[32 * b + j0 + i + 1] + res[i + 1] : 0.f);
+                                unpack2(MODE == SLOPE ? times_slope2<ACT, T>(pack2(g[i], g[i + 1]), zz) : activate2<ACT, T>(zz), z0, z1);
+                            }
+#pragma unroll
+                            for (int h = 0; h < 2; ++h)
+                                if (mine && j0 + i + h < channels) out[at + (j0 + i + h) * q.P] = from_float<T>(v[j0 + i + h]);
+                        }
+                    }
+                    if (MODE == SLOPE && q.sums) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (!mine) v[j] = 0.f;
+                        const float total = transposed_sum(v, lane);
+                        if (lane < channels) sums_smem[quarter * q.bn + 32 * b + lane] += total;
+                    }
+                }
+            }
+            tmem_release();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(drained + 8 * set);
+            if (wait.lost) break;
+            if (set ^= 1; set == 0) set_phase ^= 1;
+        }
+    }
+    __syncwarp();
+    tmem_release();
+    __syncthreads();
+    if (warp == kEpilogue + kGroups * kGroupWarps) tmem_free(tmem, 2 * set_columns);
+    if (MODE == SLOPE && q.sums)
+        for (int i = threadIdx.x; i < q.bn; i += kThreads)
+            if (n0 + i < q.Cn)
+                q.sums[(int64_t)walker * q.Cn + n0 + i] = (sums_smem[i] + sums_smem[q.bn + i]) + (sums_smem[2 * q.bn + i] + sums_smem[3 * q.bn + i]);
+}
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+struct SplitPlan {
+    int bn, tiles_n, stages, columns;
+    int64_t tiles_p;
+    unsigned walkers;
+    uint32_t smem;
+};
+bool plan_split(const PointwiseShape &s, int K, int Cn, SplitPlan *plan)
+{
+    const int parts = s.io_kind == BC_IO_F32 ? 3 : 1, chunks = (int)ceil_div(K, 64), samples = s.last ? 1 : s.N;
+    const int64_t P = s.last ? s.N * s.P : s.P;
+    if (K < 1 || Cn < 1) return false;
+    SplitPlan r{};
+    r.stages = parts == 3 ? 2 : 4;
+    // channels of a tile: what shared memory holds of the weights, and tensor memory of the sums
+    const uint32_t others = SplitLayout{16, r.stages, 0, parts, s.last}.bytes() + 8192;
+    const int64_t most = std::min<int64_t>(parts == 3 ? 128 : 256, (int64_t)(kMostShared - others) / (parts * chunks * 128) / 16 * 16);
+    if (most < 16) return false;
+    r.tiles_n = (int)ceil_div(Cn, most);
+    r.bn = (int)ceil_div(ceil_div(Cn, r.tiles_n), 16) * 16;
+    r.tiles_n = (int)ceil_div(Cn, r.bn);
+    r.columns = 32;
+    while (r.columns < r.bn) r.columns *= 2;
+    r.smem = SplitLayout{r.bn, r.stages, chunks, parts, s.last}.bytes();
+    r.tiles_p = ceil_div(P, 128);
+    const int64_t tiles = r.tiles_p * samples;
+    if (r.smem > kMostShared || tiles > INT32_MAX) return false;
+    r.walkers = (unsigned)std::min<int64_t>(tiles, std::max<int64_t>(1, 148 / r.tiles_n));
+    *plan = r;
+    return true;
+}
+
+template <int MODE>
+int launch_split(const PointwiseShape &s, const SplitPlan &plan, SplitProduct q, cudaStream_t stream)
+{
+    q.samples = s.last ? 1 : s.N;
+    q.P = s.last ? s.N * s.P : s.P;
+    q.tiles_p = (int)plan.tiles_p;
+    q.tiles_n = plan.tiles_n;
+    q.bn = plan.bn;
+    q.stages = plan.stages;
+    q.columns = plan.columns;
+    q.instruction = mma_instruction(s.io_kind != BC_IO_F16, !s.last, false, plan.bn);
+    const int each = 16 / io_size(s.io_kind);
+    const bool vec = (s.last ? q.K : q.P) % each == 0 && pointwise_mma_aligned(q.a, nullptr);
+    return with_type(s.io_kind, [&](auto t) {
+        return with_activation(MODE == INPUT ? BC_ACT_NONE : s.act, [&](auto act) {
+            using T = decltype(t);
+            constexpr int ACT = MODE == INPUT ? BC_ACT_NONE : act();
+            auto go = [&](auto kernel) {
+                if (const int e = raise_smem_limit((const void *)kernel, kMostShared)) return e;
+                const LaunchScope scope(KID_POINTWISE_SPLIT, stream);
+                launch_overlapped(kernel, plan.walkers * plan.tiles_n, kThreads, plan.smem, stream, q);
+                return check_launch("pointwise_split_kernel");
+            };
+            if (s.last) return vec ? go(pointwise_split_kernel<T, MODE, ACT, true, true>) : go(pointwise_split_kernel<T, MODE, ACT, true, false>);
+            return vec ? go(pointwise_split_kernel<T, MODE, ACT, false, true>) : go(pointwise_split_kernel<T, MODE, ACT, false, false>);
+        });
+    });
+}
+
+}  // namespace
+
+bool pointwise_split_suits(const PointwiseShape &s, bool input)
+{
+    SplitPlan plan;
+    return plan_split(s, input ? s.Co : s.Ci, input ? s.Ci : s.Co, &plan);
+}
+int pointwise_split_sums_rows(const PointwiseShape &s)
+{
+    SplitPlan plan;
+    return plan_split(s, s.Ci, s.Co, &plan) ? (int)plan.walkers : 0;
+}
+int launch_pointwise_split_forward(const PointwiseShape &s, const void *x, const void *weight, const void *bias, const void *residual,
+                                   void *out, cudaStream_t stream)
+{
+    SplitPlan plan;
+    plan_split(s, s.Ci, s.Co, &plan);
+    return launch_split<FORWARD>(s, plan, {x, weight, bias, residual, nullptr, out, nullptr, 0, s.Ci, s.Co, 0, s.Ci, 1}, stream);
+}
+int launch_pointwise_split_slope(const PointwiseShape &s, const void *x, const void *weight, const void *bias, const void *residual,
+                                 const void *grad, void *dz, float *sums, cudaStream_t stream)
+{
+    SplitPlan plan;
+    plan_split(s, s.Ci, s.Co, &plan);
+    return launch_split<SLOPE>(s, plan, {x, weight, bias, residual, grad, dz, sums, 0, s.Ci, s.Co, 0, s.Ci, 1}, stream);
+}
+int launch_pointwise_split_input(const PointwiseShape &s, const void *dz, const void *weight, void *grad_input, cudaStream_t stream)
+{
+    SplitPlan plan;
+    plan_split(s, s.Co, s.Ci, &plan);
+    return launch_split<INPUT>(s, plan, {dz, weight, nullptr, nullptr, nullptr, grad_input, nullptr, 0, s.Co, s.Ci, 0, 1, s.Ci}, stream);
+}
+
+int read_wait_timeouts_split(int *count) { return read_wait_timeouts_here(count); }
+
+}  // namespace bc
