@@ -59,16 +59,32 @@ __device__ __forceinline__ void tile_load(uint32_t dst, const CUtensorMap *map, 
 }
 __device__ __forceinline__ void map_prefetch(const CUtensorMap *map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 
-// 32 accumulators of the warp's lanes.
-__device__ __forceinline__ void tmem_load32(uint32_t at, float (&v)[32])
+// 16 accumulators of each of the warp's lanes.
+__device__ __forceinline__ void accumulators16(uint32_t at, float (&v)[16])
 {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,"
-                 "%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n tcgen05.wait::ld.sync.aligned;"
-                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]),
-                   "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]),
-                   "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]),
-                   "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
-                 : "r"(at) : "memory");
+    float4 q[4];
+    tmem_load16(at, q);
+    tmem_wait_load(q);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[4 * i] = q[i].x;
+        v[4 * i + 1] = q[i].y;
+        v[4 * i + 2] = q[i].z;
+        v[4 * i + 3] = q[i].w;
+    }
+}
+
+// Halves the values of the two lanes that `mask` tells apart: the one without the bit goes on with the lower half of both's sums.
+template <int N>
+__device__ __forceinline__ void fold(float (&v)[N], int lane, int mask, int half)
+{
+#pragma unroll
+    for (int j = 0; j < N / 2; ++j)
+        if (j < half) {
+            const bool high = lane & mask;
+            const float keep = high ? v[j + half] : v[j], send = high ? v[j] : v[j + half];
+            v[j] = keep + __shfl_xor_sync(0xffffffffu, send, mask);
+        }
 }
 
 // A wait whose expiry ends all further ones of the thread: a lost arrival is counted (bc_wait_timeouts), and nothing hangs.

@@ -4,8 +4,9 @@
 // channels.  The weights stay in shared memory; persistent CTAs walk over the pixels.  One thread brings slices of 64 k by
 // TMA into a ring, one issues tcgen05.mma into one of two sets of accumulators in tensor memory, eight warps take the other set
 // out.  Planes are an MN-major operand and channels last a K-major one: no transposition in either.
-// A warp of the epilogue passes 32 x 32 accumulators through shared memory (rows of 33 words: no bank conflicts), so that it
-// reads residuals and gradients and writes results 16 bytes a lane, along whichever index runs in memory.
+// A warp of the epilogue passes 32 x 32 sums through shared memory (rows of 33 words: no bank conflicts), so that it reads
+// residuals and gradients and writes results 16 bytes a lane, 64 bytes in a row, along whichever index runs in memory.  Where a
+// CTA has its SM to itself, the next block's are on their way while a block is dealt with.
 //
 // pointwise_weight_mma_kernel: grad_weight, D[o, i] = sum_p dz[o, p] x[i, p], 128 x up to 256 weights, split over the pixels.
 #include "bc_mma.cuh"
@@ -46,8 +47,8 @@ struct MmaLayout {
     __host__ __device__ uint32_t bytes() const { return barriers() + (2 * stages + 5) * 8 + 8 + 1024; }
 };
 
-template <typename T, int MODE, int ACT, bool LAST>
-__global__ void __launch_bounds__(kThreads, 2) pointwise_mma_kernel(const __grid_constant__ MmaProduct q)
+template <typename T, int MODE, int ACT, bool LAST, int CTAS>
+__global__ void __launch_bounds__(kThreads, CTAS) pointwise_mma_kernel(const __grid_constant__ MmaProduct q)
 {
     extern __shared__ char raw_smem[];
     const uint32_t raw = smem_u32(raw_smem), base = (raw + 1023) & ~1023u;
@@ -148,112 +149,116 @@ __global__ void __launch_bounds__(kThreads, 2) pointwise_mma_kernel(const __grid
     } else {
         float *staging = reinterpret_cast<float *>(smem + lay.staging()) + warp * 32 * kPitch;
         const int quarter = warp & 3, half = warp >> 2, blocks = (q.bn + 31) / 32;
-        const int row8 = lane >> 2, col8 = (lane & 3) * 8;
+        // A lane's four vectors of a block: planes, channel 8 i + outer and pixels from inner; last, that pixel and channels from
+        // inner.  Warps in pairs take every second block.
+        const int outer = lane >> 2, inner = 8 * (lane & 3);
         const T *residual = static_cast<const T *>(q.residual), *grad = static_cast<const T *>(q.grad);
         T *out = static_cast<T *>(q.out);
+        struct Block {
+            int64_t at;
+            int there;                // bits
+            uint4 res[MODE == INPUT ? 1 : 4], grad[MODE == SLOPE ? 4 : 1];
+        };
         uint32_t set = 0, set_phase = 0;
         for (int64_t tile = walker; tile < tiles; tile += walkers) {
             const int sample = (int)(tile / q.tiles_p);
             const int64_t p0 = (tile - (int64_t)sample * q.tiles_p) * 128 + quarter * 32;
-            bool waited = false;
-            for (int b = half; b < blocks; b += 2) {
-                // the lane's four vectors: planes, channel 8 i + row8 and pixels from col8; last, pixel 8 i + row8 and channels
-                int64_t at[4];
-                bool there[4];
-                uint4 res[4], gr[4];
+            auto fetch = [&](int b, Block &v) {
+                const int64_t p = p0 + (LAST ? outer : inner);
+                const int column = 32 * b + (LAST ? inner : outer), c = n0 + column;
+                v.at = LAST ? p * q.Cn + c : ((int64_t)sample * q.Cn + c) * q.P + p;
+                v.there = 0;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int64_t p = p0 + (LAST ? 8 * i + row8 : col8);
-                    const int c = n0 + 32 * b + (LAST ? col8 : 8 * i + row8);
-                    there[i] = p < q.P && c < q.Cn && 32 * b + (LAST ? col8 : 8 * i + row8) < q.bn;
-                    at[i] = LAST ? p * q.Cn + c : ((int64_t)sample * q.Cn + c) * q.P + p;
-                    if (MODE != INPUT && residual && there[i]) res[i] = *reinterpret_cast<const uint4 *>(residual + at[i]);
-                    if (MODE == SLOPE && there[i]) gr[i] = *reinterpret_cast<const uint4 *>(grad + at[i]);
+                    const bool there = LAST ? p + 8 * i < q.P && c < q.Cn && column < q.bn : p < q.P && c + 8 * i < q.Cn && column + 8 * i < q.bn;
+                    const int64_t at = v.at + 8 * i * (LAST ? (int64_t)q.Cn : q.P);
+                    v.there |= (int)there << i;
+                    if (MODE != INPUT && residual && there) v.res[i] = *reinterpret_cast<const uint4 *>(residual + at);
+                    if (MODE == SLOPE && there) v.grad[i] = *reinterpret_cast<const uint4 *>(grad + at);
                 }
-                if (!waited) {
-                    waited = true;
-                    wait(ready + 8 * set, set_phase);
-                    __syncwarp();
-                    tmem_acquire();
-                }
-                float v[32];
-                tmem_load32(tmem + set * q.columns + 32 * b + ((uint32_t)quarter << 21), v);
-                if (b + 2 >= blocks) {
-                    tmem_release();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(drained + 8 * set);
-                }
+            };
+            auto finish = [&](int b, const Block &now) {
 #pragma unroll
-                for (int j = 0; j < 32; ++j) staging[lane * kPitch + j] = v[j];
+                for (int part = 0; part < 2; ++part) {
+                    float v[16];
+                    accumulators16(tmem + set * q.columns + 32 * b + 16 * part + ((uint32_t)quarter << 21), v);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) staging[lane * kPitch + 16 * part + j] = v[j];
+                }
                 __syncwarp();
                 float total[8] = {};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
+                    const int row = 8 * i + outer;
+                    const bool there = now.there >> i & 1;
                     f2_t z[4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const float *from = LAST ? staging + (8 * i + row8) * kPitch + col8 + 2 * j : staging + (col8 + 2 * j) * kPitch + 8 * i + row8;
+                        const float *from = LAST ? staging + row * kPitch + inner + 2 * j : staging + (inner + 2 * j) * kPitch + row;
                         z[j] = pack2(from[0], from[LAST ? 1 : kPitch]);
                     }
-                    if (MODE != INPUT) {
+                    if (MODE != INPUT && there) {
+                        const float *bias = bias_smem + 32 * b + (LAST ? inner : row);
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const int c = 32 * b + (LAST ? col8 + 2 * j : 8 * i + row8);
-                            if (there[i]) z[j] = add2(z[j], pack2(bias_smem[c], bias_smem[LAST ? c + 1 : c]));
-                        }
-                        if (residual && there[i]) {
+                        for (int j = 0; j < 4; ++j) z[j] = add2(z[j], pack2(bias[LAST ? 2 * j : 0], bias[LAST ? 2 * j + 1 : 0]));
+                        if (residual) {
                             f2_t r[4];
-                            unpack_pairs<T>(res[i], r);
+                            unpack_pairs<T>(now.res[i], r);
 #pragma unroll
                             for (int j = 0; j < 4; ++j) z[j] = add2(z[j], r[j]);
                         }
-                        if (MODE == SLOPE) {
-                            f2_t g[4];
-                            if (there[i]) {
-                                unpack_pairs<T>(gr[i], g);
+                    }
+                    if (MODE == SLOPE) {
+                        f2_t g[4];
+                        unpack_pairs<T>(there ? now.grad[i] : make_uint4(0, 0, 0, 0), g);
 #pragma unroll
-                                for (int j = 0; j < 4; ++j) z[j] = times_slope2<ACT, T>(g[j], z[j]);
+                        for (int j = 0; j < 4; ++j) z[j] = there ? times_slope2<ACT, T>(g[j], z[j]) : both(0.f);
+                        if (q.sums) {
+                            float s[8];
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) unpack2(z[j], s[2 * j], s[2 * j + 1]);
+                            if (LAST) {
+#pragma unroll
+                                for (int j = 0; j < 8; ++j) total[j] += s[j];
                             } else {
-#pragma unroll
-                                for (int j = 0; j < 4; ++j) z[j] = both(0.f);
+                                float t = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+                                t += __shfl_xor_sync(0xffffffffu, t, 1);
+                                t += __shfl_xor_sync(0xffffffffu, t, 2);
+                                if ((lane & 3) == 0 && 32 * b + row < q.bn) sums_smem[quarter * q.bn + 32 * b + row] += t;
                             }
-                            if (q.sums) {
-                                float s[8];
-#pragma unroll
-                                for (int j = 0; j < 4; ++j) unpack2(z[j], s[2 * j], s[2 * j + 1]);
-                                if (LAST) {
-#pragma unroll
-                                    for (int j = 0; j < 8; ++j) total[j] += s[j];
-                                } else {
-                                    float t = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
-                                    t += __shfl_xor_sync(0xffffffffu, t, 1);
-                                    t += __shfl_xor_sync(0xffffffffu, t, 2);
-                                    if ((lane & 3) == 0 && there[i]) sums_smem[quarter * q.bn + 32 * b + 8 * i + row8] += t;
-                                }
-                            }
-                        } else {
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) z[j] = activate2<ACT, T>(z[j]);
                         }
-                    }
-                    if (there[i]) *reinterpret_cast<uint4 *>(out + at[i]) = pack_pairs<T>(z);
-                }
-                if (MODE == SLOPE && LAST && q.sums) {
+                    } else if (MODE == FORWARD) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        total[j] += __shfl_xor_sync(0xffffffffu, total[j], 4);
-                        total[j] += __shfl_xor_sync(0xffffffffu, total[j], 8);
-                        total[j] += __shfl_xor_sync(0xffffffffu, total[j], 16);
-                        if (row8 == j && 32 * b + col8 + j < q.bn) sums_smem[quarter * q.bn + 32 * b + col8 + j] += total[j];
+                        for (int j = 0; j < 4; ++j) z[j] = activate2<ACT, T>(z[j]);
                     }
+                    if (there) *reinterpret_cast<uint4 *>(out + now.at + 8 * i * (LAST ? (int64_t)q.Cn : q.P)) = pack_pairs<T>(z);
+                }
+                if (MODE == SLOPE && LAST && q.sums) {      // eight channels over the eight lanes of their vectors
+                    fold(total, lane, 4, 4);
+                    fold(total, lane, 8, 2);
+                    fold(total, lane, 16, 1);
+                    const int c = 32 * b + inner + (lane & 4 ? 4 : 0) + (lane & 8 ? 2 : 0) + (lane & 16 ? 1 : 0);
+                    if (c < q.bn) sums_smem[quarter * q.bn + c] += total[0];
                 }
                 __syncwarp();
+            };
+            Block one, two;
+            fetch(half, one);
+            wait(ready + 8 * set, set_phase);
+            __syncwarp();
+            tmem_acquire();
+            for (int b = half; b < blocks; b += 4) {
+                if (CTAS == 1) fetch(b + 2, two);
+                finish(b, one);
+                if (b + 2 >= blocks) break;
+                if (CTAS == 1) fetch(b + 4, one);
+                else fetch(b + 2, two);
+                finish(b + 2, two);
+                if (CTAS != 1 && b + 4 < blocks) fetch(b + 4, one);
             }
-            if (!waited) {      // (no columns for this half: it drains by arriving)
-                wait(ready + 8 * set, set_phase);
-                __syncwarp();
-                if (lane == 0) mbar_arrive(drained + 8 * set);
-            }
+            tmem_release();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(drained + 8 * set);
             if (wait.lost) break;
             if (set ^= 1; set == 0) set_phase ^= 1;
         }
@@ -265,8 +270,10 @@ __global__ void __launch_bounds__(kThreads, 2) pointwise_mma_kernel(const __grid
     if (warp == kEpilogue + 1) tmem_free(tmem, 2 * q.columns);
     if (MODE == SLOPE && q.sums)
         for (int i = threadIdx.x; i < q.bn; i += kThreads)
-            if (n0 + i < q.Cn)
-                q.sums[(int64_t)walker * q.Cn + n0 + i] = (sums_smem[i] + sums_smem[q.bn + i]) + (sums_smem[2 * q.bn + i] + sums_smem[3 * q.bn + i]);
+            if (n0 + i < q.Cn) {
+                const float *t = sums_smem + i;
+                q.sums[(int64_t)walker * q.Cn + n0 + i] = (t[0] + t[q.bn]) + (t[2 * q.bn] + t[3 * q.bn]);
+            }
 }
 
 // ---- grad_weight
@@ -420,13 +427,13 @@ __global__ void __launch_bounds__(kWeightThreads) pointwise_weight_mma_kernel(co
         tmem_acquire();
         const int o = o0 + warp * 32 + lane;
         if (!__any_sync(0xffffffffu, wait.lost))
-            for (int b = 0; b < q.bn; b += 32) {
-                float v[32];
-                tmem_load32(tmem + b + ((uint32_t)warp << 21), v);
+            for (int b = 0; b < q.bn; b += 16) {
+                float v[16];
+                accumulators16(tmem + b + ((uint32_t)warp << 21), v);
                 float *to = partial + (int64_t)o * q.Ci + i0 + b;
 #pragma unroll
-                for (int j = 0; j < 32; j += 4)
-                    if (o < q.Co && i0 + b + j < q.Ci && b + j < q.bn) *reinterpret_cast<float4 *>(to + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+                for (int j = 0; j < 16; j += 4)
+                    if (o < q.Co && i0 + b + j < q.Ci) *reinterpret_cast<float4 *>(to + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
             }
     }
     if (wait.lost) let_copies_land();
@@ -441,7 +448,7 @@ bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
 // Tiles, ring and grid of a product; false where the weights do not fit.
 struct Plan {
-    int bn, tiles_n, stages, columns;
+    int bn, tiles_n, stages, columns, per_sm;
     int64_t tiles_p;
     unsigned walkers;
     uint32_t smem;
@@ -467,8 +474,8 @@ bool plan_product(const PointwiseShape &s, int K, int Cn, bool input, Plan *plan
     }
     // (coordinates of 32 bits, strides below 2^40 bytes)
     if (r.stages < 2 || tiles > INT32_MAX || P > INT32_MAX - 256 || P * std::max(s.Ci, s.Co) >= (int64_t)1 << 38) return false;
-    const int per_sm = r.columns <= 128 && 2 * (r.smem + 1024) <= 228 << 10 ? 2 : 1;
-    r.walkers = (unsigned)std::min<int64_t>(tiles, std::max<int64_t>(1, 148 * per_sm / r.tiles_n));
+    r.per_sm = r.columns <= 128 && 2 * (r.smem + 1024) <= 228 << 10 ? 2 : 1;
+    r.walkers = (unsigned)std::min<int64_t>(tiles, std::max<int64_t>(1, 148 * r.per_sm / r.tiles_n));
     *plan = r;
     return true;
 }
@@ -503,8 +510,13 @@ int launch_mma(const PointwiseShape &s, const Plan &plan, MmaProduct q, const vo
             launch_overlapped(kernel, plan.walkers * plan.tiles_n, kThreads, plan.smem, stream, q);
             return check_launch("pointwise_mma_kernel");
         };
-        if (bf16) return s.last ? go(pointwise_mma_kernel<__nv_bfloat16, MODE, ACT, true>) : go(pointwise_mma_kernel<__nv_bfloat16, MODE, ACT, false>);
-        return s.last ? go(pointwise_mma_kernel<__half, MODE, ACT, true>) : go(pointwise_mma_kernel<__half, MODE, ACT, false>);
+        auto of_type = [&](auto t, auto ctas) {
+            using T = decltype(t);
+            constexpr int CTAS = decltype(ctas)::value;
+            return s.last ? go(pointwise_mma_kernel<T, MODE, ACT, true, CTAS>) : go(pointwise_mma_kernel<T, MODE, ACT, false, CTAS>);
+        };
+        auto run = [&](auto ctas) { return bf16 ? of_type(__nv_bfloat16(), ctas) : of_type(__half(), ctas); };
+        return plan.per_sm == 1 ? run(std::integral_constant<int, 1>()) : run(std::integral_constant<int, 2>());
     });
 }
 

@@ -14,9 +14,9 @@ namespace bc {
 namespace {
 
 enum { FORWARD, SLOPE, INPUT };
-constexpr int kEpilogue = 4, kGroups = 2, kGroupWarps = 4;
+constexpr int kEpilogue = 8, kGroups = 2, kGroupWarps = 4;
 constexpr int kThreads = 32 * (kEpilogue + kGroups * kGroupWarps + 1);
-constexpr int kPitch = 33;
+constexpr int kPitch = 17;
 constexpr uint32_t kPart = 16384;      // 128 pixels x 64 k
 constexpr uint32_t kMostShared = 227 << 10;
 
@@ -69,21 +69,6 @@ __device__ __forceinline__ void split8(const float (&v)[8], uint4 (&part)[3])
     }
 #pragma unroll
     for (int p = 0; p < 3; ++p) part[p] = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
-}
-
-// Sums of 32 values over the warp's lanes, value j's in lane j.
-__device__ __forceinline__ float transposed_sum(float (&v)[32], int lane)
-{
-#pragma unroll
-    for (int w = 16; w; w >>= 1)
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-            if (j < w) {
-                const bool high = lane & w;
-                const float keep = high ? v[j + w] : v[j], send = high ? v[j] : v[j + w];
-                v[j] = keep + __shfl_xor_sync(0xffffffffu, send, w);
-            }
-    return v[0];
 }
 
 template <typename T, int MODE, int ACT, bool LAST, bool VEC>
@@ -159,7 +144,7 @@ __global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const Spli
             const uint32_t phase = (uint32_t)(slice / q.stages) & 1;
             const int sample = (int)(tile / q.tiles_p);
             const int64_t p0 = (tile - (int64_t)sample * q.tiles_p) * 128;
-            const int pixels = (int)min((int64_t)128, q.P - p0), k_left = q.K - 64 * c;
+            const int pixels = (int)min((int64_t)128, q.P - p0), k_left = q.K - 64 * c, k_used = (k_left + 15) / 16 * 16;
             const T *a = a_all + (LAST ? p0 * q.K + 64 * c : ((int64_t)sample * q.K + 64 * c) * q.P + p0);
             // a vector: planes, eight pixels of a k; last, eight k of a pixel.  `inner` of it are there.
             uint4 raw_v[8][PARTS == 3 ? 2 : 1];
@@ -194,6 +179,7 @@ __global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const Spli
                 const int e = t + 128 * j;
                 const uint32_t at = LAST ? (e >> 3) * 128 + (((e & 7) ^ (e >> 3 & 7)) << 4)
                                          : (e >> 3 & 1) * kBlockBytes + (e >> 4) * 128 + (((e & 7) ^ (e >> 4 & 7)) << 4);
+                if ((LAST ? 8 * (e & 7) : e >> 4) >= k_used) continue;
                 if constexpr (PARTS == 3) {
                     const uint4 &u = raw_v[j][0], &v = raw_v[j][1];
                     const float f[8] = {__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w),
@@ -244,7 +230,7 @@ __global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const Spli
         }
     } else {
         float *staging = reinterpret_cast<float *>(smem + lay.staging()) + warp * 32 * kPitch;
-        const int quarter = warp, blocks = (q.bn + 31) / 32;
+        const int quarter = warp & 3, half = warp >> 2, blocks = q.bn / 16;
         const T *residual = static_cast<const T *>(q.residual), *grad = static_cast<const T *>(q.grad);
         T *out = static_cast<T *>(q.out);
         uint32_t set = 0, set_phase = 0;
@@ -252,111 +238,96 @@ __global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const Spli
             const int sample = (int)(tile / q.tiles_p);
             const int64_t p0 = (tile - (int64_t)sample * q.tiles_p) * 128 + quarter * 32;
             const int rows = (int)max((int64_t)0, min((int64_t)32, q.P - p0));
-            wait(ready + 8 * set, set_phase);
-            __syncwarp();
-            tmem_acquire();
-            for (int b = 0; b < blocks; ++b) {
-                float v[32];
-                const uint32_t from = tmem + set * set_columns + 32 * b + ((uint32_t)quarter << 21);
-                tmem_load32(from, v);
+            // Blocks of 16 channels, 16 values a lane, coalesced: planes, the lane's pixel and channel i; last, pixel
+            // 2 i + (lane >> 4) and channel lane & 15.  What the block reads is on its way before its sums are there.
+            bool waited = false;
+            for (int b = half; b < blocks || !waited; b += 2) {
+                const int c0 = n0 + 16 * b, channels = min(16, q.Cn - c0);
+                const int64_t at = LAST ? (p0 + (lane >> 4)) * q.Cn + c0 + (lane & 15) : ((int64_t)sample * q.Cn + c0) * q.P + p0 + lane;
+                const int64_t step = LAST ? 2 * (int64_t)q.Cn : q.P;
+                auto there = [&](int i) { return LAST ? 2 * i + (lane >> 4) < rows && (lane & 15) < channels : lane < rows && i < channels; };
+                T res[16], g[16];
+                if (b < blocks) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        if (MODE != INPUT && residual && there(i)) res[i] = residual[at + i * step];
+                        if (MODE == SLOPE && there(i)) g[i] = grad[at + i * step];
+                    }
+                }
+                if (!waited) {
+                    waited = true;
+                    wait(ready + 8 * set, set_phase);
+                    __syncwarp();
+                    tmem_acquire();
+                    if (b >= blocks) break;
+                }
+                float v[16];
+                const uint32_t from = tmem + set * set_columns + 16 * b + ((uint32_t)quarter << 21);
+                accumulators16(from, v);
                 if constexpr (PARTS == 3) {
-                    float u[32];
-                    tmem_load32(from + q.columns, u);
+                    float u[16], finite = 0.f;
+                    accumulators16(from + q.columns, u);
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] += u[j];
-                    float finite = 0.f;
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) finite = fmaf(v[j], 0.f, finite);
+                    for (int j = 0; j < 16; ++j) {
+                        v[j] += u[j];
+                        finite = fmaf(v[j], 0.f, finite);
+                    }
                     if (finite != 0.f && lane < rows) {      // (a NaN: some value is not finite)
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) u[j] = 0.f;
+                        for (int j = 0; j < 16; ++j) u[j] = 0.f;
                         for (int k = 0; k < q.K; ++k) {
                             const float x = to_float(a_all[LAST ? (p0 + lane) * q.K + k : ((int64_t)sample * q.K + k) * q.P + p0 + lane]);
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) {
-                                const int c = n0 + 32 * b + j;
-                                if (c < q.Cn) u[j] = fmaf(x, to_float(w_all[(int64_t)c * q.wn + (int64_t)k * q.wk]), u[j]);
-                            }
+                            for (int j = 0; j < 16; ++j)
+                                if (j < channels) u[j] = fmaf(x, to_float(w_all[(int64_t)(c0 + j) * q.wn + (int64_t)k * q.wk]), u[j]);
                         }
 #pragma unroll
-                        for (int j = 0; j < 32; ++j)
+                        for (int j = 0; j < 16; ++j)
                             if (!(fabsf(v[j]) < INFINITY)) v[j] = u[j];
                     }
+                    __syncwarp();
                 }
-                const int c0 = n0 + 32 * b, channels = min(32, min(q.Cn - c0, q.bn - 32 * b));
-                if constexpr (LAST) {
-                    // a lane a channel, row after row
+                if (LAST) {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) staging[lane * kPitch + j] = v[j];
+                    for (int j = 0; j < 16; ++j) staging[lane * kPitch + j] = v[j];
                     __syncwarp();
-                    const int64_t at = p0 * q.Cn + c0 + lane;
-                    const float bias = bias_smem[32 * b + (lane < channels ? lane : 0)];
-                    float total = 0.f;
-                    if (lane < channels) {
 #pragma unroll
-                        for (int r0 = 0; r0 < 32; r0 += 8) {
-                            float z[8], res[8], g[8];
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) {
-                                const bool there = r0 + i < rows;
-                                const int64_t e = at + (int64_t)(r0 + i) * q.Cn;
-                                if (MODE != INPUT) res[i] = residual && there ? to_float(residual[e]) : 0.f;
-                                if (MODE == SLOPE) g[i] = there ? to_float(grad[e]) : 0.f;
-                                z[i] = staging[(r0 + i) * kPitch + lane];
-                            }
-#pragma unroll
-                            for (int i = 0; i < 8; i += 2) {
-                                if (MODE != INPUT) {
-                                    const f2_t zz = pack2(z[i] + bias + res[i], z[i + 1] + bias + res[i + 1]);
-                                    unpack2(MODE == SLOPE ? times_slope2<ACT, T>(pack2(g[i], g[i + 1]), zz) : activate2<ACT, T>(zz), z[i], z[i + 1]);
-                                }
-#pragma unroll
-                                for (int h = 0; h < 2; ++h)
-                                    if (r0 + i + h < rows) {
-                                        if (MODE == SLOPE) total += z[i + h];
-                                        out[at + (int64_t)(r0 + i + h) * q.Cn] = from_float<T>(z[i + h]);
-                                    }
-                            }
-                        }
-                        if (MODE == SLOPE && q.sums) sums_smem[quarter * q.bn + 32 * b + lane] += total;
-                    }
+                    for (int i = 0; i < 16; ++i) v[i] = staging[(2 * i + (lane >> 4)) * kPitch + (lane & 15)];
                     __syncwarp();
-                } else {
-                    // a lane a pixel, channel after channel
-                    const int64_t at = ((int64_t)sample * q.Cn + c0) * q.P + p0 + lane;
-                    const bool mine = lane < rows;
+                }
+                float total = 0.f;
 #pragma unroll
-                    for (int j0 = 0; j0 < 32; j0 += 8) {
-                        float res[8], g[8];
+                for (int i = 0; i < 16; i += 2) {
+                    if (MODE != INPUT) {
+                        const float *bias = bias_smem + 16 * b;
+                        float z[2], gg[2];
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const bool there = mine && j0 + i < channels;
-                            const int64_t e = at + (j0 + i) * q.P;
-                            if (MODE != INPUT) res[i] = residual && there ? to_float(residual[e]) : 0.f;
-                            if (MODE == SLOPE) g[i] = there ? to_float(grad[e]) : 0.f;
+                        for (int h = 0; h < 2; ++h) {
+                            z[h] = v[i + h] + bias[LAST ? lane & 15 : i + h];
+                            if (residual && there(i + h)) z[h] += to_float(res[i + h]);
+                            gg[h] = MODE == SLOPE && there(i + h) ? to_float(g[i + h]) : 0.f;
                         }
-#pragma unroll
-                        for (int i = 0; i < 8; i += 2) {
-                            float &z0 = v[j0 + i], &z1 = v[j0 + i + 1];
-                            if (MODE != INPUT) {
-                                // (columns past the tile are there in memory, but hold nothing)
-                                const bool there = j0 + i < channels;
-                                const f2_t zz = pack2(there ? z0 + bias_smem[32 * b + j0 + i] + res[i] : 0.f,
-                                                      j0 + i + 1 < channels ? z1 + bias_smem[32 * b + j0 + i + 1] + res[i + 1] : 0.f);
-                                unpack2(MODE == SLOPE ? times_slope2<ACT, T>(pack2(g[i], g[i + 1]), zz) : activate2<ACT, T>(zz), z0, z1);
-                            }
-#pragma unroll
-                            for (int h = 0; h < 2; ++h)
-                                if (mine && j0 + i + h < channels) out[at + (j0 + i + h) * q.P] = from_float<T>(v[j0 + i + h]);
-                        }
+                        const f2_t zz = pack2(z[0], z[1]);
+                        unpack2(MODE == SLOPE ? times_slope2<ACT, T>(pack2(gg[0], gg[1]), zz) : activate2<ACT, T>(zz), v[i], v[i + 1]);
                     }
-                    if (MODE == SLOPE && q.sums) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (!mine) v[j] = 0.f;
-                        const float total = transposed_sum(v, lane);
-                        if (lane < channels) sums_smem[quarter * q.bn + 32 * b + lane] += total;
+                    for (int h = 0; h < 2; ++h) {
+                        if (there(i + h)) out[at + (i + h) * step] = from_float<T>(v[i + h]);
+                        else v[i + h] = 0.f;
+                        if (LAST) total += v[i + h];
                     }
+                }
+                if (MODE == SLOPE && q.sums) {
+                    if (LAST) {
+                        total += __shfl_xor_sync(0xffffffffu, total, 16);
+                    } else {      // sixteen channels over the lanes
+                        fold(v, lane, 8, 8);
+                        fold(v, lane, 4, 4);
+                        fold(v, lane, 2, 2);
+                        fold(v, lane, 1, 1);
+                        total = v[0] + __shfl_xor_sync(0xffffffffu, v[0], 16);
+                    }
+                    if (lane < 16) sums_smem[quarter * q.bn + 16 * b + lane] += total;
                 }
             }
             tmem_release();
