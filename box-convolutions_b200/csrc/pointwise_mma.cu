@@ -16,7 +16,7 @@ namespace bc {
 namespace {
 
 enum { FORWARD, SLOPE, INPUT };
-constexpr int kEpilogue = 8, kThreads = 32 * (kEpilogue + 2);
+constexpr int kEpilogue = 8;      // warps of the epilogue, or pairs of them
 constexpr int kPitch = 33;
 constexpr uint32_t kStage = 16384;      // 128 pixels x 64 k
 constexpr size_t kMostShared = 227 << 10;
@@ -35,7 +35,7 @@ struct MmaProduct {
 
 // Shared memory from a 1024-byte boundary on.
 struct MmaLayout {
-    int bn, stages, chunks;
+    int bn, stages, chunks, pair;
     bool input;
     // of one slice of 64 k of the weights
     __host__ __device__ uint32_t slice() const { return input ? (uint32_t)((bn + 63) / 64) * kBlockBytes : (uint32_t)bn * 128; }
@@ -43,18 +43,19 @@ struct MmaLayout {
     __host__ __device__ uint32_t staging() const { return ring() + stages * kStage; }
     __host__ __device__ uint32_t bias() const { return staging() + kEpilogue * 32 * kPitch * 4; }
     __host__ __device__ uint32_t sums() const { return bias() + bn * 4; }
-    __host__ __device__ uint32_t barriers() const { return (sums() + 4 * bn * 4 + 7) / 8 * 8; }
+    __host__ __device__ uint32_t barriers() const { return (sums() + 4 * pair * bn * 4 + 7) / 8 * 8; }
     __host__ __device__ uint32_t bytes() const { return barriers() + (2 * stages + 5) * 8 + 8 + 1024; }
 };
 
-template <typename T, int MODE, int ACT, bool LAST, int CTAS>
-__global__ void __launch_bounds__(kThreads, CTAS) pointwise_mma_kernel(const __grid_constant__ MmaProduct q)
+template <typename T, int MODE, int ACT, bool LAST, int PAIR>
+__global__ void __launch_bounds__(32 * (kEpilogue * PAIR + 2), PAIR == 1 ? 2 : 1) pointwise_mma_kernel(const __grid_constant__ MmaProduct q)
 {
+    constexpr int WARPS = kEpilogue * PAIR, THREADS = 32 * (WARPS + 2), EACH = 4 / PAIR;
     extern __shared__ char raw_smem[];
     const uint32_t raw = smem_u32(raw_smem), base = (raw + 1023) & ~1023u;
     char *smem = raw_smem + (base - raw);
     const int chunks = (q.K + 63) / 64;
-    const MmaLayout lay{q.bn, q.stages, chunks, MODE == INPUT};
+    const MmaLayout lay{q.bn, q.stages, chunks, PAIR, MODE == INPUT};
     float *bias_smem = reinterpret_cast<float *>(smem + lay.bias()), *sums_smem = reinterpret_cast<float *>(smem + lay.sums());
     const uint32_t full = base + lay.barriers(), empty = full + 8 * q.stages, ready = empty + 8 * q.stages, drained = ready + 16,
                    weights_full = drained + 16;
@@ -71,7 +72,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) pointwise_mma_kernel(const __g
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(ready + 8 * i, 1);
-            mbar_init(drained + 8 * i, kEpilogue);
+            mbar_init(drained + 8 * i, WARPS);
         }
         mbar_init(weights_full, 1);
         fence_mbar_init();
@@ -79,17 +80,17 @@ __global__ void __launch_bounds__(kThreads, CTAS) pointwise_mma_kernel(const __g
         map_prefetch(&q.w);
     }
     grid_dependency_wait();
-    if (warp == kEpilogue + 1) tmem_alloc(tmem_slot, 2 * q.columns);
-    for (int i = threadIdx.x; i < q.bn; i += kThreads)
+    if (warp == WARPS + 1) tmem_alloc(tmem_slot, 2 * q.columns);
+    for (int i = threadIdx.x; i < q.bn; i += THREADS)
         bias_smem[i] = MODE != INPUT && q.bias && n0 + i < q.Cn ? to_float(static_cast<const T *>(q.bias)[n0 + i]) : 0.f;
-    for (int i = threadIdx.x; i < 4 * q.bn; i += kThreads) sums_smem[i] = 0.f;
+    for (int i = threadIdx.x; i < 4 * PAIR * q.bn; i += THREADS) sums_smem[i] = 0.f;
     tmem_release();
     __syncthreads();
     tmem_acquire();
     const uint32_t tmem = *tmem_slot;
     Waiter wait;
 
-    if (warp == kEpilogue) {
+    if (warp == WARPS) {
         if (lane == 0) {
             mbar_expect(weights_full, chunks * lay.slice());
             for (int c = 0; c < chunks; ++c) {
@@ -120,7 +121,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) pointwise_mma_kernel(const __g
                 if (wait.lost) break;
             }
         }
-    } else if (warp == kEpilogue + 1) {
+    } else if (warp == WARPS + 1) {
         if (lane == 0) {
             wait(weights_full, 0);
             uint32_t stage = 0, phase = 0, set = 0, set_phase = 0;
@@ -147,17 +148,21 @@ __global__ void __launch_bounds__(kThreads, CTAS) pointwise_mma_kernel(const __g
             }
         }
     } else {
-        float *staging = reinterpret_cast<float *>(smem + lay.staging()) + warp * 32 * kPitch;
-        const int quarter = warp & 3, half = warp >> 2, blocks = (q.bn + 31) / 32;
-        // A lane's four vectors of a block: planes, channel 8 i + outer and pixels from inner; last, that pixel and channels from
-        // inner.  Warps in pairs take every second block.
-        const int outer = lane >> 2, inner = 8 * (lane & 3);
+        const int quarter = warp & 3, member = PAIR == 2 ? warp >> 2 & 1 : 0, half = warp / (4 * PAIR), blocks = (q.bn + 31) / 32;
+        float *staging = reinterpret_cast<float *>(smem + lay.staging()) + (4 * half + quarter) * 32 * kPitch;
+        auto together = [&] {      // whoever shares the staging rows
+            if (PAIR == 2) asm volatile("bar.sync %0, 64;" ::"r"(1 + 4 * half + quarter) : "memory");
+            else __syncwarp();
+        };
+        // A lane's vectors of a block: planes, channel 8 i + outer and pixels from inner; last, that pixel and channels from
+        // inner.  Every second block is a warp's, or two warps', two of the four vectors each.
+        const int outer = (lane >> 2) + 8 * EACH * member, inner = 8 * (lane & 3);
         const T *residual = static_cast<const T *>(q.residual), *grad = static_cast<const T *>(q.grad);
         T *out = static_cast<T *>(q.out);
         struct Block {
             int64_t at;
             int there;                // bits
-            uint4 res[MODE == INPUT ? 1 : 4], grad[MODE == SLOPE ? 4 : 1];
+            uint4 res[MODE == INPUT ? 1 : EACH], grad[MODE == SLOPE ? EACH : 1];
         };
         uint32_t set = 0, set_phase = 0;
         for (int64_t tile = walker; tile < tiles; tile += walkers) {
@@ -169,7 +174,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) pointwise_mma_kernel(const __g
                 v.at = LAST ? p * q.Cn + c : ((int64_t)sample * q.Cn + c) * q.P + p;
                 v.there = 0;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < EACH; ++i) {
                     const bool there = LAST ? p + 8 * i < q.P && c < q.Cn && column < q.bn : p < q.P && c + 8 * i < q.Cn && column + 8 * i < q.bn;
                     const int64_t at = v.at + 8 * i * (LAST ? (int64_t)q.Cn : q.P);
                     v.there |= (int)there << i;
@@ -179,16 +184,16 @@ __global__ void __launch_bounds__(kThreads, CTAS) pointwise_mma_kernel(const __g
             };
             auto finish = [&](int b, const Block &now) {
 #pragma unroll
-                for (int part = 0; part < 2; ++part) {
+                for (int part = member; part < 2; part += PAIR) {
                     float v[16];
                     accumulators16(tmem + set * q.columns + 32 * b + 16 * part + ((uint32_t)quarter << 21), v);
 #pragma unroll
                     for (int j = 0; j < 16; ++j) staging[lane * kPitch + 16 * part + j] = v[j];
                 }
-                __syncwarp();
+                together();
                 float total[8] = {};
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < EACH; ++i) {
                     const int row = 8 * i + outer;
                     const bool there = now.there >> i & 1;
                     f2_t z[4];
@@ -224,7 +229,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) pointwise_mma_kernel(const __g
                                 float t = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
                                 t += __shfl_xor_sync(0xffffffffu, t, 1);
                                 t += __shfl_xor_sync(0xffffffffu, t, 2);
-                                if ((lane & 3) == 0 && 32 * b + row < q.bn) sums_smem[quarter * q.bn + 32 * b + row] += t;
+                                if ((lane & 3) == 0 && 32 * b + row < q.bn) sums_smem[(quarter + 4 * member) * q.bn + 32 * b + row] += t;
                             }
                         }
                     } else if (MODE == FORWARD) {
@@ -238,9 +243,9 @@ __global__ void __launch_bounds__(kThreads, CTAS) pointwise_mma_kernel(const __g
                     fold(total, lane, 8, 2);
                     fold(total, lane, 16, 1);
                     const int c = 32 * b + inner + (lane & 4 ? 4 : 0) + (lane & 8 ? 2 : 0) + (lane & 16 ? 1 : 0);
-                    if (c < q.bn) sums_smem[quarter * q.bn + c] += total[0];
+                    if (c < q.bn) sums_smem[(quarter + 4 * member) * q.bn + c] += total[0];
                 }
-                __syncwarp();
+                together();
             };
             Block one, two;
             fetch(half, one);
@@ -248,13 +253,13 @@ __global__ void __launch_bounds__(kThreads, CTAS) pointwise_mma_kernel(const __g
             __syncwarp();
             tmem_acquire();
             for (int b = half; b < blocks; b += 4) {
-                if (CTAS == 1) fetch(b + 2, two);
+                if (PAIR == 2) fetch(b + 2, two);
                 finish(b, one);
                 if (b + 2 >= blocks) break;
-                if (CTAS == 1) fetch(b + 4, one);
+                if (PAIR == 2) fetch(b + 4, one);
                 else fetch(b + 2, two);
                 finish(b + 2, two);
-                if (CTAS != 1 && b + 4 < blocks) fetch(b + 4, one);
+                if (PAIR == 1 && b + 4 < blocks) fetch(b + 4, one);
             }
             tmem_release();
             __syncwarp();
@@ -267,12 +272,13 @@ __global__ void __launch_bounds__(kThreads, CTAS) pointwise_mma_kernel(const __g
     __syncwarp();
     tmem_release();
     __syncthreads();
-    if (warp == kEpilogue + 1) tmem_free(tmem, 2 * q.columns);
+    if (warp == WARPS + 1) tmem_free(tmem, 2 * q.columns);
     if (MODE == SLOPE && q.sums)
-        for (int i = threadIdx.x; i < q.bn; i += kThreads)
+        for (int i = threadIdx.x; i < q.bn; i += THREADS)
             if (n0 + i < q.Cn) {
-                const float *t = sums_smem + i;
-                q.sums[(int64_t)walker * q.Cn + n0 + i] = (t[0] + t[q.bn]) + (t[2 * q.bn] + t[3 * q.bn]);
+                float t = 0.f;
+                for (int w = 0; w < 4 * PAIR; ++w) t += sums_smem[w * q.bn + i];
+                q.sums[(int64_t)walker * q.Cn + n0 + i] = t;
             }
 }
 
@@ -468,13 +474,16 @@ bool plan_product(const PointwiseShape &s, int K, int Cn, bool input, Plan *plan
     while (r.columns < r.bn) r.columns *= 2;
     r.tiles_p = ceil_div(P, 128);
     const int64_t tiles = r.tiles_p * samples;
-    for (r.stages = 4; r.stages >= 2; --r.stages) {
-        r.smem = MmaLayout{r.bn, r.stages, chunks, input}.bytes();
-        if (r.smem <= kMostShared) break;
+    if (tiles > INT32_MAX || P > INT32_MAX - 256 || P * std::max(s.Ci, s.Co) >= (int64_t)1 << 38) return false;      // (coordinates, strides)
+    // two CTAs an SM where both find room, or one with pairs of warps
+    r.stages = 4;
+    r.per_sm = 2;
+    r.smem = MmaLayout{r.bn, r.stages, chunks, 1, input}.bytes();
+    if (r.columns > 128 || 2 * (r.smem + 1024) > 228 << 10) {
+        r.per_sm = 1;
+        while ((r.smem = MmaLayout{r.bn, r.stages, chunks, 2, input}.bytes()) > kMostShared)
+            if (--r.stages < 2) return false;
     }
-    // (coordinates of 32 bits, strides below 2^40 bytes)
-    if (r.stages < 2 || tiles > INT32_MAX || P > INT32_MAX - 256 || P * std::max(s.Ci, s.Co) >= (int64_t)1 << 38) return false;
-    r.per_sm = r.columns <= 128 && 2 * (r.smem + 1024) <= 228 << 10 ? 2 : 1;
     r.walkers = (unsigned)std::min<int64_t>(tiles, std::max<int64_t>(1, 148 * r.per_sm / r.tiles_n));
     *plan = r;
     return true;
@@ -507,16 +516,16 @@ int launch_mma(const PointwiseShape &s, const Plan &plan, MmaProduct q, const vo
         auto go = [&](auto kernel) {
             if (const int e = raise_smem_limit((const void *)kernel, kMostShared)) return e;
             const LaunchScope scope(KID_POINTWISE_MMA, stream);
-            launch_overlapped(kernel, plan.walkers * plan.tiles_n, kThreads, plan.smem, stream, q);
+            launch_overlapped(kernel, plan.walkers * plan.tiles_n, 32 * (kEpilogue * (plan.per_sm == 1 ? 2 : 1) + 2), plan.smem, stream, q);
             return check_launch("pointwise_mma_kernel");
         };
-        auto of_type = [&](auto t, auto ctas) {
+        auto of_type = [&](auto t, auto pair) {
             using T = decltype(t);
-            constexpr int CTAS = decltype(ctas)::value;
-            return s.last ? go(pointwise_mma_kernel<T, MODE, ACT, true, CTAS>) : go(pointwise_mma_kernel<T, MODE, ACT, false, CTAS>);
+            constexpr int PAIR = decltype(pair)::value;
+            return s.last ? go(pointwise_mma_kernel<T, MODE, ACT, true, PAIR>) : go(pointwise_mma_kernel<T, MODE, ACT, false, PAIR>);
         };
-        auto run = [&](auto ctas) { return bf16 ? of_type(__nv_bfloat16(), ctas) : of_type(__half(), ctas); };
-        return plan.per_sm == 1 ? run(std::integral_constant<int, 1>()) : run(std::integral_constant<int, 2>());
+        auto run = [&](auto pair) { return bf16 ? of_type(__nv_bfloat16(), pair) : of_type(__half(), pair); };
+        return plan.per_sm == 1 ? run(std::integral_constant<int, 2>()) : run(std::integral_constant<int, 1>());
     });
 }
 
