@@ -283,6 +283,8 @@ int launch_pointwise_split_forward(const PointwiseShape &s, const void *x, const
 int launch_pointwise_split_slope(const PointwiseShape &s, const void *x, const void *weight, const void *bias, const void *residual,
                                  const void *grad, void *dz, float *sums, cudaStream_t stream);
 int launch_pointwise_split_input(const PointwiseShape &s, const void *dz, const void *weight, void *grad_input, cudaStream_t stream);
+int pointwise_split_weight_splits(const PointwiseShape &s);
+int launch_pointwise_split_weight(const PointwiseShape &s, const void *dz, const void *x, float *partial, bool sums, cudaStream_t stream);
 int read_wait_timeouts_split(int *count);
 
 size_t pointwise_workspace(const PointwiseShape &s, int need_mask);

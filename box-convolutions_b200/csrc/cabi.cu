@@ -815,6 +815,7 @@ const char *bc_kernel_name(int kernel_id)
         case KID_POINTWISE_MMA: return "pointwise_mma_kernel";
         case KID_POINTWISE_WEIGHT_MMA: return "pointwise_weight_mma_kernel";
         case KID_POINTWISE_SPLIT: return "pointwise_split_kernel";
+        case KID_POINTWISE_WEIGHT_SPLIT: return "pointwise_weight_split_kernel";
         case KID_NORM_FORWARD: return "norm_forward_kernel";
         case KID_NORM_BACKWARD: return "norm_backward_kernel";
         case KID_NORM_FINISH: return "norm_finish_kernel";

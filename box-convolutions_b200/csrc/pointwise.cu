@@ -463,8 +463,8 @@ Splits splits_of(const PointwiseShape &s)
 
 size_t partial_bytes(const PointwiseShape &s)
 {
-    // (either kernel's: the query does not know the arrays)
-    return align_up((size_t)std::max(splits_of(s).splits, pointwise_mma_weight_splits(s)) * pointwise_partial_stride(s.Co, s.Ci) * sizeof(float));
+    // (whichever kernel's: the query does not know the arrays)
+    return align_up((size_t)std::max({splits_of(s).splits, pointwise_mma_weight_splits(s), pointwise_split_weight_splits(s)}) * pointwise_partial_stride(s.Co, s.Ci) * sizeof(float));
 }
 // Which kernel a product with pixels in the rows takes.
 enum { BY_TMA, BY_SPLIT, BY_FMA };
@@ -547,6 +547,8 @@ int launch_pointwise_backward(const PointwiseShape &s, const void *x, const void
         int splits = pointwise_mma_weight_splits(s), e;
         if (splits && pointwise_mma_aligned(dz, x)) {
             e = launch_pointwise_mma_weight(s, dz, x, partial, want_bias && !sums, stream);
+        } else if ((splits = pointwise_split_weight_splits(s))) {
+            e = launch_pointwise_split_weight(s, dz, x, partial, want_bias && !sums, stream);
         } else {
             const Splits v = splits_of(s);
             splits = v.splits;

@@ -71,6 +71,59 @@ __device__ __forceinline__ void split8(const float (&v)[8], uint4 (&part)[3])
     for (int p = 0; p < 3; ++p) part[p] = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
 }
 
+// Eight values from `from` on, of which `n` are there (zeros beyond); VEC: whole vectors, aligned.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load8(const T *from, int n, uint4 (&v)[kParts<T> == 3 ? 2 : 1])
+{
+    if constexpr (VEC) {
+        constexpr int EACH = 16 / sizeof(T);
+#pragma unroll
+        for (int i = 0; i < 8 / EACH; ++i) v[i] = n > i * EACH ? *reinterpret_cast<const uint4 *>(from + i * EACH) : make_uint4(0, 0, 0, 0);
+    } else if constexpr (sizeof(T) == 4) {
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = i < n ? from[i] : 0.f;
+        v[0] = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+        v[1] = make_uint4(__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]), __float_as_uint(f[7]));
+    } else {
+        const unsigned short *bits = reinterpret_cast<const unsigned short *>(from);
+        uint32_t f[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = i < n ? bits[i] : 0;
+        v[0] = make_uint4(f[0] | f[1] << 16, f[2] | f[3] << 16, f[4] | f[5] << 16, f[6] | f[7] << 16);
+    }
+}
+template <typename T>
+__device__ __forceinline__ void floats8(const uint4 (&v)[kParts<T> == 3 ? 2 : 1], float (&f)[8])
+{
+    if constexpr (sizeof(T) == 4) {
+        float g[4];
+        unpack<float>(v[0], g);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = g[i];
+        unpack<float>(v[1], g);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[4 + i] = g[i];
+    } else {
+        unpack<T>(v[0], f);
+    }
+}
+// Into their place of every part, `part` bytes apart.
+template <typename T>
+__device__ __forceinline__ void place8(char *to, uint32_t part, const uint4 (&v)[kParts<T> == 3 ? 2 : 1])
+{
+    if constexpr (sizeof(T) == 4) {
+        float f[8];
+        uint4 parts[3];
+        floats8<T>(v, f);
+        split8(f, parts);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) *reinterpret_cast<uint4 *>(to + p * part) = parts[p];
+    } else {
+        *reinterpret_cast<uint4 *>(to) = v[0];
+    }
+}
+
 template <typename T, int MODE, int ACT, bool LAST, bool VEC>
 __global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const SplitProduct q)
 {
@@ -153,24 +206,7 @@ __global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const Spli
                 const int e = t + 128 * j, in = 8 * (LAST ? e & 7 : e & 15), outer = LAST ? e >> 3 : e >> 4;
                 const int inner = outer < (LAST ? pixels : k_left) ? (LAST ? k_left : pixels) - in : 0;
                 const T *from = a + outer * (LAST ? (int64_t)q.K : q.P) + in;
-                if constexpr (VEC) {
-                    constexpr int EACH = 16 / sizeof(T);
-#pragma unroll
-                    for (int i = 0; i < 8 / EACH; ++i)
-                        raw_v[j][i] = inner > i * EACH ? *reinterpret_cast<const uint4 *>(from + i * EACH) : make_uint4(0, 0, 0, 0);
-                } else if constexpr (PARTS == 3) {
-                    float v[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] = i < inner ? to_float(from[i]) : 0.f;
-                    raw_v[j][0] = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-                    raw_v[j][1] = make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7]));
-                } else {
-                    const unsigned short *bits = reinterpret_cast<const unsigned short *>(from);
-                    uint32_t v[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] = i < inner ? bits[i] : 0;
-                    raw_v[j][0] = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
-                }
+                load8<T, VEC>(from, inner, raw_v[j]);
             }
             if (!wait(empty + 8 * stage, phase ^ 1)) break;
             char *to = smem + lay.ring() + stage * PARTS * kPart;
@@ -180,17 +216,7 @@ __global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const Spli
                 const uint32_t at = LAST ? (e >> 3) * 128 + (((e & 7) ^ (e >> 3 & 7)) << 4)
                                          : (e >> 3 & 1) * kBlockBytes + (e >> 4) * 128 + (((e & 7) ^ (e >> 4 & 7)) << 4);
                 if ((LAST ? 8 * (e & 7) : e >> 4) >= k_used) continue;
-                if constexpr (PARTS == 3) {
-                    const uint4 &u = raw_v[j][0], &v = raw_v[j][1];
-                    const float f[8] = {__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w),
-                                        __uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w)};
-                    uint4 part[3];
-                    split8(f, part);
-#pragma unroll
-                    for (int p = 0; p < 3; ++p) *reinterpret_cast<uint4 *>(to + p * kPart + at) = part[p];
-                } else {
-                    *reinterpret_cast<uint4 *>(to + at) = raw_v[j][0];
-                }
+                place8<T>(to + at, kPart, raw_v[j]);
             }
             fence_proxy_async();
             __syncwarp();
@@ -347,6 +373,231 @@ __global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const Spli
                 q.sums[(int64_t)walker * q.Cn + n0 + i] = (sums_smem[i] + sums_smem[q.bn + i]) + (sums_smem[2 * q.bn + i] + sums_smem[3 * q.bn + i]);
 }
 
+// ---- grad_weight, D[o, i] = sum_p dz[o, p] x[i, p]: 128 x up to 256 (float 128) weights, split over the pixels; built like
+// pointwise_weight_mma_kernel, slices of 64 pixels.  Planes are K-major operands, rows of 64 pixels; channels last MN-major.
+
+constexpr int kWeightEpilogue = 4, kWeightThreads = 32 * (kWeightEpilogue + kGroups * kGroupWarps + 1);
+
+struct WeightSplit {
+    const void *dz, *x;
+    float *partial;          // a row a split: Co * Ci sums, then Co sums of dz
+    int64_t P;
+    int64_t per, slices;     // slices of a split; of a sample
+    int samples, Ci, Co;
+    int tiles_i;
+    int rows, bn, stages, columns;      // output and input channels of a tile
+    bool sums;
+    uint32_t instruction;
+};
+
+struct WeightSplitLayout {
+    int rows, bn, stages, parts;
+    bool last;
+    __host__ __device__ uint32_t bytes_of(int channels) const { return last ? (uint32_t)((channels + 63) / 64) * kBlockBytes : (uint32_t)channels * 128; }
+    // (M is 128 whatever there is of dz: what lies behind its rows is read as well, and leads nowhere)
+    __host__ __device__ uint32_t dz_part() const { return bytes_of(rows); }
+    __host__ __device__ uint32_t x_part() const { return bytes_of(bn); }
+    __host__ __device__ uint32_t stage() const { return (parts * (dz_part() + x_part()) + 1023) / 1024 * 1024; }
+    __host__ __device__ uint32_t barriers() const { return stages * stage() + 2 * kBlockBytes; }
+    __host__ __device__ uint32_t bytes() const { return barriers() + (2 * stages + 1) * 8 + 8 + 1024; }
+};
+
+template <typename T, bool LAST, bool VEC>
+__global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kernel(const WeightSplit q)
+{
+    constexpr int PARTS = kParts<T>;
+    extern __shared__ char raw_smem[];
+    __shared__ float sums_smem[kGroups][128];
+    const uint32_t raw = smem_u32(raw_smem), base = (raw + 1023) & ~1023u;
+    char *smem = raw_smem + (base - raw);
+    const WeightSplitLayout lay{q.rows, q.bn, q.stages, PARTS, LAST};
+    const uint32_t full = base + lay.barriers(), empty = full + 8 * q.stages, ready = empty + 8 * q.stages;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + lay.barriers() + (2 * q.stages + 1) * 8);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int tiles_o = (q.Co + q.rows - 1) / q.rows, tiles = tiles_o * q.tiles_i;
+    const int split = (int)(blockIdx.x / (unsigned)tiles), t = (int)blockIdx.x - split * tiles;
+    const int o0 = t / q.tiles_i * q.rows, i0 = (t - t / q.tiles_i * q.tiles_i) * q.bn;
+    const int64_t first = split * q.per, last = min((int64_t)q.samples * q.slices, first + q.per);
+    const bool sums = q.sums && i0 == 0;
+    const uint32_t columns = (PARTS > 1 ? 2 : 1) * q.columns;
+    const T *dz_all = static_cast<const T *>(q.dz), *x_all = static_cast<const T *>(q.x);
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < q.stages; ++i) {
+            mbar_init(full + 8 * i, kGroupWarps);
+            mbar_init(empty + 8 * i, 1);
+        }
+        mbar_init(ready, 1);
+        fence_mbar_init();
+    }
+    grid_dependency_wait();
+    if (warp == kWeightEpilogue + kGroups * kGroupWarps) tmem_alloc(tmem_slot, columns);
+    tmem_release();
+    __syncthreads();
+    tmem_acquire();
+    const uint32_t tmem = *tmem_slot;
+    Waiter wait;
+
+    if (warp >= kWeightEpilogue && warp < kWeightEpilogue + kGroups * kGroupWarps) {
+        const int group = (warp - kWeightEpilogue) / kGroupWarps, me = threadIdx.x - 32 * (kWeightEpilogue + group * kGroupWarps);
+        const int of_dz = q.rows * 8, total = of_dz + q.bn * 8;      // vectors of a slice
+        float sum[8] = {};      // planes: of the channel of vector me + 128 j; last: of the channels of every vector of dz
+        for (int64_t slice = first + group; slice < last; slice += kGroups) {
+            const int64_t nth = slice - first;
+            const int stage = (int)(nth % q.stages);
+            const uint32_t phase = (uint32_t)(nth / q.stages) & 1;
+            const int64_t sample = slice / q.slices, p0 = (slice - sample * q.slices) * 64;
+            const int pixels = (int)min((int64_t)64, q.P - p0);
+            char *const dz_to = smem + stage * lay.stage(), *const x_to = dz_to + PARTS * lay.dz_part();
+            bool waited = false;
+            for (int v0 = me; v0 < total; v0 += 8 * 128) {
+                uint4 v[8][PARTS == 3 ? 2 : 1];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int e = v0 + 128 * j;
+                    if (e >= total) break;
+                    const bool dz = e < of_dz;
+                    const int f = dz ? e : e - of_dz, C = dz ? q.Co : q.Ci, c0 = dz ? o0 : i0, wide = (dz ? q.rows : q.bn) / 8;
+                    const T *from = dz ? dz_all : x_all;
+                    if (LAST) {      // eight channels of a pixel
+                        const int p = f / wide, c = c0 + 8 * (f - p * wide);
+                        load8<T, VEC>(from + (p0 + p) * C + c, p < pixels ? C - c : 0, v[j]);
+                    } else {         // eight pixels of a channel
+                        const int c = c0 + (f >> 3), p = 8 * (f & 7);
+                        load8<T, VEC>(from + (sample * C + c) * q.P + p0 + p, c < C ? pixels - p : 0, v[j]);
+                    }
+                }
+                if (!waited) {
+                    waited = true;
+                    if (!wait(empty + 8 * stage, phase ^ 1)) break;
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int e = v0 + 128 * j;
+                    if (e >= total) break;
+                    const bool dz = e < of_dz;
+                    const int f = dz ? e : e - of_dz, wide = (dz ? q.rows : q.bn) / 8;
+                    const int outer = LAST ? f / wide : f >> 3, chunk = LAST ? f - outer * wide : f & 7;
+                    char *to = (dz ? dz_to : x_to) + (LAST ? (chunk >> 3) * kBlockBytes : 0) + outer * 128 + (((chunk & 7) ^ (outer & 7)) << 4);
+                    place8<T>(to, dz ? lay.dz_part() : lay.x_part(), v[j]);
+                    if (sums && dz) {
+                        float g[8];
+                        floats8<T>(v[j], g);
+                        if (LAST) {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) sum[i] += g[i];
+                        } else {
+                            sum[j] += ((g[0] + g[1]) + (g[2] + g[3])) + ((g[4] + g[5]) + (g[6] + g[7]));
+                        }
+                    }
+                }
+            }
+            if (wait.lost) break;
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(full + 8 * stage);
+        }
+        if (sums) {
+            // (rows are a power of two: a thread's vectors of dz are all at one place among the channels, or eight lanes' of a channel)
+            if (LAST) {
+                // the threads of a place, in order, one at a time
+                const int wide = q.rows / 8, place = me % wide;
+                for (int turn = 0; turn < 128 / wide; ++turn) {
+                    if (me / wide == turn)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) sums_smem[group][8 * place + i] = turn ? sums_smem[group][8 * place + i] + sum[i] : sum[i];
+                    asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    float g = sum[j];
+                    g += __shfl_xor_sync(0xffffffffu, g, 1);
+                    g += __shfl_xor_sync(0xffffffffu, g, 2);
+                    g += __shfl_xor_sync(0xffffffffu, g, 4);
+                    const int c = (me + 128 * j) >> 3;
+                    if ((lane & 7) == 0 && c < q.rows) sums_smem[group][c] = g;
+                }
+            }
+        }
+    } else if (warp == kWeightEpilogue + kGroups * kGroupWarps) {
+        if (lane == 0) {
+            uint32_t stage = 0, phase = 0;
+            for (int64_t slice = first; slice < last; ++slice) {
+                if (!wait(full + 8 * stage, phase)) break;
+                tmem_acquire();
+                const uint32_t a = base + stage * lay.stage(), b = a + PARTS * lay.dz_part();
+#pragma unroll
+                for (int k = 0; k < 64; k += 16)
+#pragma unroll
+                    for (int i = 0; i < PARTS; ++i)
+#pragma unroll
+                        for (int j = 0; j < PARTS - i; ++j) {
+                            const uint32_t ai = a + i * lay.dz_part(), bj = b + j * lay.x_part();
+                            mma(tmem + (i + j ? q.columns : 0), LAST ? mn_major(ai, k, kBlockBytes) : k_major(ai, k),
+                                LAST ? mn_major(bj, k, kBlockBytes) : k_major(bj, k), q.instruction, slice > first || k || i + j > 1 || i > 0);
+                        }
+                mma_commit(empty + 8 * stage);
+                if (++stage == (uint32_t)q.stages) {
+                    stage = 0;
+                    phase ^= 1;
+                }
+            }
+            if (!wait.lost) mma_commit(ready);
+        }
+    } else {
+        float *partial = q.partial + split * pointwise_partial_stride(q.Co, q.Ci);
+        wait(ready, 0);
+        __syncwarp();
+        tmem_acquire();
+        const int row = warp * 32 + lane, o = o0 + row;
+        const bool mine = row < q.rows && o < q.Co;
+        for (int b = 0; b < q.bn; b += 16) {
+            float v[16];
+            accumulators16(tmem + b + ((uint32_t)warp << 21), v);
+            if constexpr (PARTS == 3) {
+                float u[16], finite = 0.f;
+                accumulators16(tmem + q.columns + b + ((uint32_t)warp << 21), u);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    v[j] += u[j];
+                    if (i0 + b + j < q.Ci) finite = fmaf(v[j], 0.f, finite);
+                }
+                if (finite != 0.f && mine) {      // (a NaN: some value is not finite)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) u[j] = 0.f;
+                    for (int64_t slice = first; slice < last; ++slice) {
+                        const int64_t sample = slice / q.slices, p0 = (slice - sample * q.slices) * 64;
+                        for (int64_t p = p0; p < min(p0 + 64, q.P); ++p) {
+                            const float g = to_float(dz_all[LAST ? p * q.Co + o : (sample * q.Co + o) * q.P + p]);
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) {
+                                const int c = i0 + b + j;
+                                if (c < q.Ci) u[j] = fmaf(g, to_float(x_all[LAST ? p * q.Ci + c : (sample * q.Ci + c) * q.P + p]), u[j]);
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                        if (!(fabsf(v[j]) < INFINITY)) v[j] = u[j];
+                }
+                __syncwarp();
+            }
+            if (mine)
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    if (i0 + b + j < q.Ci) partial[(int64_t)o * q.Ci + i0 + b + j] = v[j];
+        }
+    }
+    __syncwarp();
+    tmem_release();
+    __syncthreads();
+    if (warp == kWeightEpilogue + kGroups * kGroupWarps) tmem_free(tmem, columns);
+    if (sums && (int)threadIdx.x < q.rows && o0 + (int)threadIdx.x < q.Co)
+        q.partial[split * pointwise_partial_stride(q.Co, q.Ci) + (int64_t)q.Co * q.Ci + o0 + threadIdx.x] =
+            last - first > 1 ? sums_smem[0][threadIdx.x] + sums_smem[1][threadIdx.x] : sums_smem[0][threadIdx.x];
+}
+
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 struct SplitPlan {
@@ -440,6 +691,83 @@ int launch_pointwise_split_input(const PointwiseShape &s, const void *dz, const 
     SplitPlan plan;
     plan_split(s, s.Co, s.Ci, &plan);
     return launch_split<INPUT>(s, plan, {dz, weight, nullptr, nullptr, nullptr, grad_input, nullptr, 0, s.Co, s.Ci, 0, 1, s.Ci}, stream);
+}
+
+// ---- grad_weight: rows of pointwise_partial_stride() floats, to be added
+namespace {
+struct WeightSplitPlan {
+    int rows, tiles_o, tiles_i, bn, stages, columns, splits;
+    int64_t slices, per;
+    uint32_t smem;
+};
+bool plan_weight_split(const PointwiseShape &s, WeightSplitPlan *plan)
+{
+    if (s.Ci < 1 || s.Co < 1) return false;
+    const int parts = s.io_kind == BC_IO_F32 ? 3 : 1, most = parts == 3 ? 128 : 256;
+    const int64_t P = s.last ? s.N * s.P : s.P, samples = s.last ? 1 : s.N;
+    WeightSplitPlan r{};
+    r.rows = 16;
+    while (r.rows < s.Co && r.rows < 128) r.rows *= 2;
+    r.tiles_o = (int)ceil_div(s.Co, r.rows);
+    r.tiles_i = (int)ceil_div(s.Ci, most);
+    r.bn = (int)ceil_div(ceil_div(s.Ci, r.tiles_i), 16) * 16;
+    r.tiles_i = (int)ceil_div(s.Ci, r.bn);
+    r.columns = 32;
+    while (r.columns < r.bn) r.columns *= 2;
+    for (r.stages = 4; r.stages >= 2; --r.stages) {
+        r.smem = WeightSplitLayout{r.rows, r.bn, r.stages, parts, s.last}.bytes();
+        if (r.smem <= kMostShared - 2048) break;
+    }
+    if (r.stages < 2) return false;
+    r.slices = ceil_div(P, 64);
+    const int64_t all = r.slices * samples, tiles = (int64_t)r.tiles_o * r.tiles_i;
+    r.per = std::max<int64_t>(std::min<int64_t>(4, all), ceil_div(all, std::max<int64_t>(1, 148 / tiles)));
+    r.splits = (int)ceil_div(all, r.per);
+    if (r.splits * tiles > INT32_MAX) return false;
+    *plan = r;
+    return true;
+}
+}  // namespace
+
+int pointwise_split_weight_splits(const PointwiseShape &s)
+{
+    WeightSplitPlan plan;
+    return plan_weight_split(s, &plan) ? plan.splits : 0;
+}
+int launch_pointwise_split_weight(const PointwiseShape &s, const void *dz, const void *x, float *partial, bool sums, cudaStream_t stream)
+{
+    WeightSplitPlan plan;
+    plan_weight_split(s, &plan);
+    WeightSplit q{};
+    q.dz = dz;
+    q.x = x;
+    q.partial = partial;
+    q.P = s.last ? s.N * s.P : s.P;
+    q.per = plan.per;
+    q.slices = plan.slices;
+    q.samples = s.last ? 1 : s.N;
+    q.Ci = s.Ci;
+    q.Co = s.Co;
+    q.tiles_i = plan.tiles_i;
+    q.rows = plan.rows;
+    q.bn = plan.bn;
+    q.stages = plan.stages;
+    q.columns = plan.columns;
+    q.sums = sums;
+    q.instruction = mma_instruction(s.io_kind != BC_IO_F16, s.last, s.last, plan.bn);
+    const int each = 16 / io_size(s.io_kind);
+    const bool vec = (s.last ? s.Ci % each == 0 && s.Co % each == 0 : s.P % each == 0) && pointwise_mma_aligned(dz, x);
+    return with_type(s.io_kind, [&](auto t) {
+        using T = decltype(t);
+        auto go = [&](auto kernel) {
+            if (const int e = raise_smem_limit((const void *)kernel, kMostShared - 2048)) return e;
+            const LaunchScope scope(KID_POINTWISE_WEIGHT_SPLIT, stream);
+            launch_overlapped(kernel, (unsigned)(plan.splits * plan.tiles_o * plan.tiles_i), kWeightThreads, plan.smem, stream, q);
+            return check_launch("pointwise_weight_split_kernel");
+        };
+        if (s.last) return vec ? go(pointwise_weight_split_kernel<T, true, true>) : go(pointwise_weight_split_kernel<T, true, false>);
+        return vec ? go(pointwise_weight_split_kernel<T, false, true>) : go(pointwise_weight_split_kernel<T, false, false>);
+    });
 }
 
 int read_wait_timeouts_split(int *count) { return read_wait_timeouts_here(count); }
