@@ -18,6 +18,8 @@ constexpr int kEpilogue = 8, kGroups = 2, kGroupWarps = 4;
 constexpr int kThreads = 32 * (kEpilogue + kGroups * kGroupWarps + 1);
 constexpr int kPitch = 17;
 constexpr uint32_t kPart = 16384;      // 128 pixels x 64 k
+constexpr uint32_t kCopies = 32768;    // the same in floats
+constexpr int kProducers = 32 * kGroups * kGroupWarps;
 constexpr uint32_t kMostShared = 227 << 10;
 
 template <typename T>
@@ -41,30 +43,27 @@ struct SplitLayout {
     bool last;
     __host__ __device__ uint32_t slice() const { return (uint32_t)bn * 128; }      // 64 k of one part of the weights
     __host__ __device__ uint32_t ring() const { return parts * chunks * slice(); }
-    __host__ __device__ uint32_t staging() const { return ring() + stages * parts * kPart; }
+    __host__ __device__ uint32_t copies() const { return ring() + stages * parts * kPart; }      // two slices of floats as they come
+    __host__ __device__ uint32_t staging() const { return copies() + (parts == 3 ? 2 * kCopies : 0); }
     __host__ __device__ uint32_t bias() const { return staging() + (last ? kEpilogue * 32 * kPitch * 4 : 0); }
     __host__ __device__ uint32_t sums() const { return bias() + bn * 4; }
     __host__ __device__ uint32_t barriers() const { return (sums() + 4 * bn * 4 + 7) / 8 * 8; }
     __host__ __device__ uint32_t bytes() const { return barriers() + (2 * stages + 4) * 8 + 8 + 1024; }
 };
 
-__device__ __forceinline__ float upper(float v) { return __uint_as_float(__float_as_uint(v) & 0xffff0000u); }
-// What is left of v without its upper part; nothing of an infinity.
-__device__ __forceinline__ float rest(float v, float u) { return v == u ? 0.f : v - u; }
-__device__ __forceinline__ uint32_t halves(float lo, float hi) { return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632); }
-
-// Eight floats as three vectors of bf16.
+// Eight floats as three vectors of bf16.  (An infinity leaves a NaN behind: what comes of it is computed again.)
 __device__ __forceinline__ void split8(const float (&v)[8], uint4 (&part)[3])
 {
     uint32_t w[3][4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        float x[2] = {v[2 * i], v[2 * i + 1]};
+        f2_t x = pack2(v[2 * i], v[2 * i + 1]);
 #pragma unroll
         for (int p = 0; p < 3; ++p) {
-            w[p][i] = halves(x[0], x[1]);
-            x[0] = rest(x[0], upper(x[0]));
-            x[1] = rest(x[1], upper(x[1]));
+            float lo, hi;
+            unpack2(x, lo, hi);
+            w[p][i] = __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632);
+            if (p < 2) x = sub2(x, pack2(__uint_as_float(__float_as_uint(lo) & 0xffff0000u), __uint_as_float(__float_as_uint(hi) & 0xffff0000u)));
         }
     }
 #pragma unroll
@@ -73,7 +72,7 @@ __device__ __forceinline__ void split8(const float (&v)[8], uint4 (&part)[3])
 
 // Eight values from `from` on, of which `n` are there (zeros beyond); VEC: whole vectors, aligned.
 template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T *from, int n, uint4 (&v)[kParts<T> == 3 ? 2 : 1])
+__device__ __forceinline__ void load8(const T *from, int n, uint4 (&v)[2])
 {
     if constexpr (VEC) {
         constexpr int EACH = 16 / sizeof(T);
@@ -93,8 +92,32 @@ __device__ __forceinline__ void load8(const T *from, int n, uint4 (&v)[kParts<T>
         v[0] = make_uint4(f[0] | f[1] << 16, f[2] | f[3] << 16, f[4] | f[5] << 16, f[6] | f[7] << 16);
     }
 }
+// Floats on their way into the thread's own place in shared memory, two vectors `half` bytes apart; zeros beyond n.
+template <bool VEC>
+__device__ __forceinline__ void copy8(uint32_t to, uint32_t half, const float *from, int n, const float *base)
+{
+    if (VEC) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + i * half), "l"(n > 4 * i ? from + 4 * i : base), "r"(n > 4 * i ? 16 : 0)
+                         : "memory");
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;"
+                         ::"r"(to + i / 4 * half + i % 4 * 4), "l"(n > i ? from + i : base), "r"(n > i ? 4 : 0) : "memory");
+    }
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// All of the thread's but the newest `slots - 1` groups have arrived.
+__device__ __forceinline__ void copies_wait(int slots)
+{
+    if (slots > 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
+    else asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
 template <typename T>
-__device__ __forceinline__ void floats8(const uint4 (&v)[kParts<T> == 3 ? 2 : 1], float (&f)[8])
+__device__ __forceinline__ void floats8(const uint4 (&v)[2], float (&f)[8])
 {
     if constexpr (sizeof(T) == 4) {
         float g[4];
@@ -110,7 +133,7 @@ __device__ __forceinline__ void floats8(const uint4 (&v)[kParts<T> == 3 ? 2 : 1]
 }
 // Into their place of every part, `part` bytes apart.
 template <typename T>
-__device__ __forceinline__ void place8(char *to, uint32_t part, const uint4 (&v)[kParts<T> == 3 ? 2 : 1])
+__device__ __forceinline__ void place8(char *to, uint32_t part, const uint4 (&v)[2])
 {
     if constexpr (sizeof(T) == 4) {
         float f[8];
@@ -145,7 +168,7 @@ __global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const Spli
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < q.stages; ++i) {
-            mbar_init(full + 8 * i, kGroupWarps);
+            mbar_init(full + 8 * i, PARTS == 3 ? kGroups * kGroupWarps : kGroupWarps);
             mbar_init(empty + 8 * i, 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -186,12 +209,64 @@ __global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const Spli
     const uint32_t tmem = *tmem_slot;
     Waiter wait;
 
-    if (warp >= kEpilogue && warp < kEpilogue + kGroups * kGroupWarps) {
+    const int64_t my_slices = walker < tiles ? (tiles - walker + walkers - 1) / walkers * chunks : 0;
+    if (PARTS == 3 && warp >= kEpilogue && warp < kEpilogue + kGroups * kGroupWarps) {
+        // Every thread has four vectors of a slice: it copies them to a place of its own, two slices ahead, and splits them from there.
+        const int t = threadIdx.x - 32 * kEpilogue;
+        const float *all = reinterpret_cast<const float *>(q.a);
+        const char *own = smem + lay.copies() + 16 * t;
+        auto copy = [&](int64_t slice) {
+            if (slice < my_slices) {
+                const int64_t nth = slice / chunks, tile = walker + nth * walkers;
+                const int c = (int)(slice - nth * chunks), sample = (int)(tile / q.tiles_p);
+                const int64_t p0 = (tile - (int64_t)sample * q.tiles_p) * 128;
+                const int pixels = (int)min((int64_t)128, q.P - p0), k_left = q.K - 64 * c;
+                const float *a = all + (LAST ? p0 * q.K + 64 * c : ((int64_t)sample * q.K + 64 * c) * q.P + p0);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int e = t + kProducers * j, in = 8 * (LAST ? e & 7 : e & 15), outer = LAST ? e >> 3 : e >> 4;
+                    const int inner = outer < (LAST ? pixels : k_left) ? (LAST ? k_left : pixels) - in : 0;
+                    copy8<VEC>(smem_u32(own) + (uint32_t)(slice & 1) * kCopies + 8192 * j, 4096, a + outer * (LAST ? (int64_t)q.K : q.P) + in, inner, all);
+                }
+            }
+            copies_commit();
+        };
+        copy(0);
+        copy(1);
+        uint32_t stage = 0, phase = 0;
+        int c = 0;
+        for (int64_t slice = 0; slice < my_slices; ++slice) {
+            copies_wait(2);
+            if (!wait(empty + 8 * stage, phase ^ 1)) break;
+            const int k_used = (q.K - 64 * c + 15) / 16 * 16;
+            char *to = smem + lay.ring() + stage * PARTS * kPart;
+            const char *from = own + (uint32_t)(slice & 1) * kCopies;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int e = t + kProducers * j;
+                const uint32_t at = LAST ? (e >> 3) * 128 + (((e & 7) ^ (e >> 3 & 7)) << 4)
+                                         : (e >> 3 & 1) * kBlockBytes + (e >> 4) * 128 + (((e & 7) ^ (e >> 4 & 7)) << 4);
+                if ((LAST ? 8 * (e & 7) : e >> 4) >= k_used) continue;
+                const uint4 v[2] = {*reinterpret_cast<const uint4 *>(from + 8192 * j),
+                                                         *reinterpret_cast<const uint4 *>(from + 8192 * j + 4096)};
+                place8<T>(to + at, kPart, v);
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(full + 8 * stage);
+            copy(slice + 2);
+            if (++c == chunks) c = 0;
+            if (++stage == (uint32_t)q.stages) {
+                stage = 0;
+                phase ^= 1;
+            }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+    } else if (warp >= kEpilogue && warp < kEpilogue + kGroups * kGroupWarps) {
         // group g brings every second slice: while one waits for memory the other writes
         const int group = (warp - kEpilogue) / kGroupWarps, t = threadIdx.x - 32 * (kEpilogue + group * kGroupWarps);
         int64_t slice = group;      // counts this CTA's slices
-        const int64_t my_tiles = walker < tiles ? (tiles - walker + walkers - 1) / walkers : 0;
-        for (; slice < my_tiles * chunks; slice += kGroups) {
+        for (; slice < my_slices; slice += kGroups) {
             const int64_t nth = slice / chunks, tile = walker + nth * walkers;
             const int c = (int)(slice - nth * chunks), stage = (int)(slice % q.stages);
             const uint32_t phase = (uint32_t)(slice / q.stages) & 1;
@@ -200,7 +275,7 @@ __global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const Spli
             const int pixels = (int)min((int64_t)128, q.P - p0), k_left = q.K - 64 * c, k_used = (k_left + 15) / 16 * 16;
             const T *a = a_all + (LAST ? p0 * q.K + 64 * c : ((int64_t)sample * q.K + 64 * c) * q.P + p0);
             // a vector: planes, eight pixels of a k; last, eight k of a pixel.  `inner` of it are there.
-            uint4 raw_v[8][PARTS == 3 ? 2 : 1];
+            uint4 raw_v[8][2];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int e = t + 128 * j, in = 8 * (LAST ? e & 7 : e & 15), outer = LAST ? e >> 3 : e >> 4;
@@ -385,20 +460,22 @@ struct WeightSplit {
     int64_t per, slices;     // slices of a split; of a sample
     int samples, Ci, Co;
     int tiles_i;
-    int rows, bn, stages, columns;      // output and input channels of a tile
+    int rows, bn, stages, slots, columns;      // output and input channels of a tile; ring; floats' slices on their way
     bool sums;
     uint32_t instruction;
 };
 
 struct WeightSplitLayout {
-    int rows, bn, stages, parts;
+    int rows, bn, stages, slots, parts;
     bool last;
     __host__ __device__ uint32_t bytes_of(int channels) const { return last ? (uint32_t)((channels + 63) / 64) * kBlockBytes : (uint32_t)channels * 128; }
     // (M is 128 whatever there is of dz: what lies behind its rows is read as well, and leads nowhere)
     __host__ __device__ uint32_t dz_part() const { return bytes_of(rows); }
     __host__ __device__ uint32_t x_part() const { return bytes_of(bn); }
     __host__ __device__ uint32_t stage() const { return (parts * (dz_part() + x_part()) + 1023) / 1024 * 1024; }
-    __host__ __device__ uint32_t barriers() const { return stages * stage() + 2 * kBlockBytes; }
+    __host__ __device__ uint32_t copies() const { return stages * stage() + 2 * kBlockBytes; }
+    __host__ __device__ int each() const { return ((rows + bn) * 8 + kProducers - 1) / kProducers; }      // vectors of a thread
+    __host__ __device__ uint32_t barriers() const { return copies() + slots * each() * 32 * kProducers; }
     __host__ __device__ uint32_t bytes() const { return barriers() + (2 * stages + 1) * 8 + 8 + 1024; }
 };
 
@@ -410,7 +487,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
     __shared__ float sums_smem[kGroups][128];
     const uint32_t raw = smem_u32(raw_smem), base = (raw + 1023) & ~1023u;
     char *smem = raw_smem + (base - raw);
-    const WeightSplitLayout lay{q.rows, q.bn, q.stages, PARTS, LAST};
+    const WeightSplitLayout lay{q.rows, q.bn, q.stages, q.slots, PARTS, LAST};
     const uint32_t full = base + lay.barriers(), empty = full + 8 * q.stages, ready = empty + 8 * q.stages;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + lay.barriers() + (2 * q.stages + 1) * 8);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -424,7 +501,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < q.stages; ++i) {
-            mbar_init(full + 8 * i, kGroupWarps);
+            mbar_init(full + 8 * i, PARTS == 3 ? kGroups * kGroupWarps : kGroupWarps);
             mbar_init(empty + 8 * i, 1);
         }
         mbar_init(ready, 1);
@@ -438,7 +515,95 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
     const uint32_t tmem = *tmem_slot;
     Waiter wait;
 
-    if (warp >= kWeightEpilogue && warp < kWeightEpilogue + kGroups * kGroupWarps) {
+    if (PARTS == 3 && warp >= kWeightEpilogue && warp < kWeightEpilogue + kGroups * kGroupWarps) {
+        // as in the product's kernel: a thread's own vectors, copied `slots` slices ahead
+        const int t = threadIdx.x - 32 * kWeightEpilogue;
+        const int of_dz = q.rows * 8, total = of_dz + q.bn * 8;
+        const uint32_t slot_bytes = lay.each() * 32 * kProducers;
+        const char *own = smem + lay.copies() + 16 * t;
+        auto copy = [&](int64_t slice) {
+            if (slice < last) {
+                const int64_t sample = slice / q.slices, p0 = (slice - sample * q.slices) * 64;
+                const int pixels = (int)min((int64_t)64, q.P - p0);
+                const uint32_t to = smem_u32(own) + (q.slots > 1 ? (uint32_t)(slice - first & 1) * slot_bytes : 0);
+                for (int j = 0, e = t; e < total; ++j, e += kProducers) {
+                    const bool dz = e < of_dz;
+                    const int f = dz ? e : e - of_dz, C = dz ? q.Co : q.Ci, c0 = dz ? o0 : i0, wide = (dz ? q.rows : q.bn) / 8;
+                    const float *from = reinterpret_cast<const float *>(dz ? q.dz : q.x);
+                    if (LAST) {      // eight channels of a pixel
+                        const int p = f / wide, c = c0 + 8 * (f - p * wide);
+                        copy8<VEC>(to + 8192 * j, 4096, from + (p0 + p) * C + c, p < pixels ? C - c : 0, from);
+                    } else {         // eight pixels of a channel
+                        const int c = c0 + (f >> 3), p = 8 * (f & 7);
+                        copy8<VEC>(to + 8192 * j, 4096, from + (sample * C + c) * q.P + p0 + p, c < C ? pixels - p : 0, from);
+                    }
+                }
+            }
+            copies_commit();
+        };
+        for (int i = 0; i < q.slots; ++i) copy(first + i);
+        float sum[8] = {};      // planes: of the channel of vector t + 256 j; last: of the channels of every vector of dz
+        uint32_t stage = 0, phase = 0;
+        for (int64_t slice = first; slice < last; ++slice) {
+            copies_wait(q.slots);
+            if (!wait(empty + 8 * stage, phase ^ 1)) break;
+            char *const dz_to = smem + stage * lay.stage(), *const x_to = dz_to + PARTS * lay.dz_part();
+            const char *from = own + (q.slots > 1 ? (uint32_t)(slice - first & 1) * slot_bytes : 0);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int e = t + kProducers * j;
+                if (e >= total) break;
+                const bool dz = e < of_dz;
+                const int f = dz ? e : e - of_dz, wide = (dz ? q.rows : q.bn) / 8;
+                const int outer = LAST ? f / wide : f >> 3, chunk = LAST ? f - outer * wide : f & 7;
+                char *to = (dz ? dz_to : x_to) + (LAST ? (chunk >> 3) * kBlockBytes : 0) + outer * 128 + (((chunk & 7) ^ (outer & 7)) << 4);
+                const uint4 v[2] = {*reinterpret_cast<const uint4 *>(from + 8192 * j),
+                                                         *reinterpret_cast<const uint4 *>(from + 8192 * j + 4096)};
+                place8<T>(to, dz ? lay.dz_part() : lay.x_part(), v);
+                if (sums && dz) {
+                    float g[8];
+                    floats8<T>(v, g);
+                    if (LAST) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) sum[i] += g[i];
+                    } else {
+                        sum[j] += ((g[0] + g[1]) + (g[2] + g[3])) + ((g[4] + g[5]) + (g[6] + g[7]));
+                    }
+                }
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(full + 8 * stage);
+            copy(slice + q.slots);
+            if (++stage == (uint32_t)q.stages) {
+                stage = 0;
+                phase ^= 1;
+            }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        if (sums) {
+            // (rows are a power of two: a thread's vectors of dz are all at one place among the channels, or eight lanes' of a channel)
+            if (LAST) {
+                const int wide = q.rows / 8, place = t % wide;
+                for (int turn = 0; turn < kProducers / wide; ++turn) {
+                    if (t / wide == turn)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) sums_smem[0][8 * place + i] = turn ? sums_smem[0][8 * place + i] + sum[i] : sum[i];
+                    asm volatile("bar.sync 1, 256;" ::: "memory");
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float g = sum[j];
+                    g += __shfl_xor_sync(0xffffffffu, g, 1);
+                    g += __shfl_xor_sync(0xffffffffu, g, 2);
+                    g += __shfl_xor_sync(0xffffffffu, g, 4);
+                    const int c = (t + kProducers * j) >> 3;
+                    if ((lane & 7) == 0 && c < q.rows) sums_smem[0][c] = g;
+                }
+            }
+        }
+    } else if (warp >= kWeightEpilogue && warp < kWeightEpilogue + kGroups * kGroupWarps) {
         const int group = (warp - kWeightEpilogue) / kGroupWarps, me = threadIdx.x - 32 * (kWeightEpilogue + group * kGroupWarps);
         const int of_dz = q.rows * 8, total = of_dz + q.bn * 8;      // vectors of a slice
         float sum[8] = {};      // planes: of the channel of vector me + 128 j; last: of the channels of every vector of dz
@@ -451,7 +616,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
             char *const dz_to = smem + stage * lay.stage(), *const x_to = dz_to + PARTS * lay.dz_part();
             bool waited = false;
             for (int v0 = me; v0 < total; v0 += 8 * 128) {
-                uint4 v[8][PARTS == 3 ? 2 : 1];
+                uint4 v[8][2];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const int e = v0 + 128 * j;
@@ -595,7 +760,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
     if (warp == kWeightEpilogue + kGroups * kGroupWarps) tmem_free(tmem, columns);
     if (sums && (int)threadIdx.x < q.rows && o0 + (int)threadIdx.x < q.Co)
         q.partial[split * pointwise_partial_stride(q.Co, q.Ci) + (int64_t)q.Co * q.Ci + o0 + threadIdx.x] =
-            last - first > 1 ? sums_smem[0][threadIdx.x] + sums_smem[1][threadIdx.x] : sums_smem[0][threadIdx.x];
+            PARTS == 1 && last - first > 1 ? sums_smem[0][threadIdx.x] + sums_smem[1][threadIdx.x] : sums_smem[0][threadIdx.x];
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -696,29 +861,35 @@ int launch_pointwise_split_input(const PointwiseShape &s, const void *dz, const 
 // ---- grad_weight: rows of pointwise_partial_stride() floats, to be added
 namespace {
 struct WeightSplitPlan {
-    int rows, tiles_o, tiles_i, bn, stages, columns, splits;
+    int rows, tiles_o, tiles_i, bn, stages, slots, columns, splits;
     int64_t slices, per;
     uint32_t smem;
 };
 bool plan_weight_split(const PointwiseShape &s, WeightSplitPlan *plan)
 {
     if (s.Ci < 1 || s.Co < 1) return false;
-    const int parts = s.io_kind == BC_IO_F32 ? 3 : 1, most = parts == 3 ? 128 : 256;
+    const int parts = s.io_kind == BC_IO_F32 ? 3 : 1;
     const int64_t P = s.last ? s.N * s.P : s.P, samples = s.last ? 1 : s.N;
     WeightSplitPlan r{};
     r.rows = 16;
     while (r.rows < s.Co && r.rows < 128) r.rows *= 2;
     r.tiles_o = (int)ceil_div(s.Co, r.rows);
-    r.tiles_i = (int)ceil_div(s.Ci, most);
-    r.bn = (int)ceil_div(ceil_div(s.Ci, r.tiles_i), 16) * 16;
-    r.tiles_i = (int)ceil_div(s.Ci, r.bn);
+    // the widest tile that shared memory holds: 16-bit with a ring of two to four, float with two and one or two slices of copies
+    for (int most = parts == 3 ? 128 : 256;; most /= 2) {
+        if (most < 32) return false;
+        r.tiles_i = (int)ceil_div(s.Ci, most);
+        r.bn = (int)ceil_div(ceil_div(s.Ci, r.tiles_i), 16) * 16;
+        r.tiles_i = (int)ceil_div(s.Ci, r.bn);
+        auto fits = [&](int stages, int slots) {
+            r.stages = stages;
+            r.slots = slots;
+            r.smem = WeightSplitLayout{r.rows, r.bn, stages, slots, parts, s.last}.bytes();
+            return r.smem <= kMostShared - 2048;
+        };
+        if (parts == 3 ? fits(2, 2) || fits(2, 1) : fits(4, 0) || fits(3, 0) || fits(2, 0)) break;
+    }
     r.columns = 32;
     while (r.columns < r.bn) r.columns *= 2;
-    for (r.stages = 4; r.stages >= 2; --r.stages) {
-        r.smem = WeightSplitLayout{r.rows, r.bn, r.stages, parts, s.last}.bytes();
-        if (r.smem <= kMostShared - 2048) break;
-    }
-    if (r.stages < 2) return false;
     r.slices = ceil_div(P, 64);
     const int64_t all = r.slices * samples, tiles = (int64_t)r.tiles_o * r.tiles_i;
     r.per = std::max<int64_t>(std::min<int64_t>(4, all), ceil_div(all, std::max<int64_t>(1, 148 / tiles)));
@@ -752,6 +923,7 @@ int launch_pointwise_split_weight(const PointwiseShape &s, const void *dz, const
     q.rows = plan.rows;
     q.bn = plan.bn;
     q.stages = plan.stages;
+    q.slots = plan.slots;
     q.columns = plan.columns;
     q.sums = sums;
     q.instruction = mma_instruction(s.io_kind != BC_IO_F16, s.last, s.last, plan.bn);
