@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(32 * (kEpilogue * PAIR + 2), PAIR == 1 ? 2 : 1
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const unsigned walkers = gridDim.x / (unsigned)q.tiles_n, walker = blockIdx.x / (unsigned)q.tiles_n;
     const int n0 = (int)(blockIdx.x - walker * q.tiles_n) * q.bn;
-    const int64_t tiles = (int64_t)q.samples * q.tiles_p;
+    const unsigned tiles = (unsigned)q.samples * (unsigned)q.tiles_p;      // (below 2^31)
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < q.stages; ++i) {
@@ -100,9 +100,9 @@ __global__ void __launch_bounds__(32 * (kEpilogue * PAIR + 2), PAIR == 1 ? 2 : 1
                 else tile_load(base + c * lay.slice(), &q.w, 64 * c, n0, weights_full);
             }
             uint32_t stage = 0, phase = 0;
-            for (int64_t tile = walker; tile < tiles; tile += walkers) {
-                const int sample = (int)(tile / q.tiles_p);
-                const int64_t p0 = (tile - (int64_t)sample * q.tiles_p) * 128;
+            for (unsigned tile = walker; tile < tiles; tile += walkers) {
+                const unsigned sample = tile / (unsigned)q.tiles_p;
+                const int64_t p0 = (int64_t)(tile - sample * q.tiles_p) * 128;
                 for (int c = 0; c < chunks; ++c) {
                     if (!wait(empty + 8 * stage, phase ^ 1)) break;
                     const uint32_t to = base + lay.ring() + stage * kStage, bar = full + 8 * stage;
@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(32 * (kEpilogue * PAIR + 2), PAIR == 1 ? 2 : 1
         if (lane == 0) {
             wait(weights_full, 0);
             uint32_t stage = 0, phase = 0, set = 0, set_phase = 0;
-            for (int64_t tile = walker; tile < tiles; tile += walkers) {
+            for (unsigned tile = walker; tile < tiles; tile += walkers) {
                 if (!wait(drained + 8 * set, set_phase ^ 1)) break;
                 tmem_acquire();
                 for (int c = 0; c < chunks; ++c) {
@@ -165,9 +165,9 @@ __global__ void __launch_bounds__(32 * (kEpilogue * PAIR + 2), PAIR == 1 ? 2 : 1
             uint4 res[MODE == INPUT ? 1 : EACH], grad[MODE == SLOPE ? EACH : 1];
         };
         uint32_t set = 0, set_phase = 0;
-        for (int64_t tile = walker; tile < tiles; tile += walkers) {
-            const int sample = (int)(tile / q.tiles_p);
-            const int64_t p0 = (tile - (int64_t)sample * q.tiles_p) * 128 + quarter * 32;
+        for (unsigned tile = walker; tile < tiles; tile += walkers) {
+            const unsigned sample = tile / (unsigned)q.tiles_p;
+            const int64_t p0 = (int64_t)(tile - sample * q.tiles_p) * 128 + quarter * 32;
             auto fetch = [&](int b, Block &v) {
                 const int64_t p = p0 + (LAST ? outer : inner);
                 const int column = 32 * b + (LAST ? inner : outer), c = n0 + column;

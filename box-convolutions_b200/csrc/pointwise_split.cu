@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const Spli
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const unsigned walkers = gridDim.x / (unsigned)q.tiles_n, walker = blockIdx.x / (unsigned)q.tiles_n;
     const int n0 = (int)(blockIdx.x - walker * q.tiles_n) * q.bn;
-    const int64_t tiles = (int64_t)q.samples * q.tiles_p;
+    const unsigned tiles = (unsigned)q.samples * (unsigned)q.tiles_p;      // (below 2^31)
     const uint32_t set_columns = (PARTS > 1 ? 2 : 1) * q.columns;
     const T *w_all = static_cast<const T *>(q.w), *a_all = static_cast<const T *>(q.a);
 
@@ -209,53 +209,65 @@ __global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const Spli
     const uint32_t tmem = *tmem_slot;
     Waiter wait;
 
-    const int64_t my_slices = walker < tiles ? (tiles - walker + walkers - 1) / walkers * chunks : 0;
+    // A producer's way through this CTA's slices.
+    struct Cursor {
+        unsigned tile;
+        int c;
+    };
+    auto advance = [&](Cursor &at) {
+        if (++at.c == chunks) {
+            at.c = 0;
+            at.tile += walkers;
+        }
+    };
     if (PARTS == 3 && warp >= kEpilogue && warp < kEpilogue + kGroups * kGroupWarps) {
         // Every thread has four vectors of a slice: it copies them to a place of its own, two slices ahead, and splits them from there.
         const int t = threadIdx.x - 32 * kEpilogue;
         const float *all = reinterpret_cast<const float *>(q.a);
         const char *own = smem + lay.copies() + 16 * t;
-        auto copy = [&](int64_t slice) {
-            if (slice < my_slices) {
-                const int64_t nth = slice / chunks, tile = walker + nth * walkers;
-                const int c = (int)(slice - nth * chunks), sample = (int)(tile / q.tiles_p);
-                const int64_t p0 = (tile - (int64_t)sample * q.tiles_p) * 128;
-                const int pixels = (int)min((int64_t)128, q.P - p0), k_left = q.K - 64 * c;
-                const float *a = all + (LAST ? p0 * q.K + 64 * c : ((int64_t)sample * q.K + 64 * c) * q.P + p0);
+        Cursor ahead{walker, 0};
+        uint32_t to_slot = 0;
+        auto copy = [&] {
+            if (ahead.tile < tiles) {
+                const unsigned sample = ahead.tile / (unsigned)q.tiles_p;
+                const int64_t p0 = (int64_t)(ahead.tile - sample * q.tiles_p) * 128;
+                const int pixels = (int)min((int64_t)128, q.P - p0), k_left = q.K - 64 * ahead.c;
+                const float *a = all + (LAST ? p0 * q.K + 64 * ahead.c : ((int64_t)sample * q.K + 64 * ahead.c) * q.P + p0);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int e = t + kProducers * j, in = 8 * (LAST ? e & 7 : e & 15), outer = LAST ? e >> 3 : e >> 4;
                     const int inner = outer < (LAST ? pixels : k_left) ? (LAST ? k_left : pixels) - in : 0;
-                    copy8<VEC>(smem_u32(own) + (uint32_t)(slice & 1) * kCopies + 8192 * j, 4096, a + outer * (LAST ? (int64_t)q.K : q.P) + in, inner, all);
+                    copy8<VEC>(smem_u32(own) + to_slot + 8192 * j, 4096, a + outer * (LAST ? (int64_t)q.K : q.P) + in, inner, all);
                 }
+                advance(ahead);
+                to_slot ^= kCopies;
             }
             copies_commit();
         };
-        copy(0);
-        copy(1);
-        uint32_t stage = 0, phase = 0;
-        int c = 0;
-        for (int64_t slice = 0; slice < my_slices; ++slice) {
+        copy();
+        copy();
+        uint32_t stage = 0, phase = 0, from_slot = 0;
+        for (Cursor at{walker, 0}; at.tile < tiles; advance(at)) {
             copies_wait(2);
             if (!wait(empty + 8 * stage, phase ^ 1)) break;
-            const int k_used = (q.K - 64 * c + 15) / 16 * 16;
+            const int k_used = (q.K - 64 * at.c + 15) / 16 * 16;
             char *to = smem + lay.ring() + stage * PARTS * kPart;
-            const char *from = own + (uint32_t)(slice & 1) * kCopies;
+            const char *from = own + from_slot;
+            from_slot ^= kCopies;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const int e = t + kProducers * j;
-                const uint32_t at = LAST ? (e >> 3) * 128 + (((e & 7) ^ (e >> 3 & 7)) << 4)
-                                         : (e >> 3 & 1) * kBlockBytes + (e >> 4) * 128 + (((e & 7) ^ (e >> 4 & 7)) << 4);
+                const uint32_t place = LAST ? (e >> 3) * 128 + (((e & 7) ^ (e >> 3 & 7)) << 4)
+                                            : (e >> 3 & 1) * kBlockBytes + (e >> 4) * 128 + (((e & 7) ^ (e >> 4 & 7)) << 4);
                 if ((LAST ? 8 * (e & 7) : e >> 4) >= k_used) continue;
                 const uint4 v[2] = {*reinterpret_cast<const uint4 *>(from + 8192 * j),
                                                          *reinterpret_cast<const uint4 *>(from + 8192 * j + 4096)};
-                place8<T>(to + at, kPart, v);
+                place8<T>(to + place, kPart, v);
             }
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(full + 8 * stage);
-            copy(slice + 2);
-            if (++c == chunks) c = 0;
+            copy();
             if (++stage == (uint32_t)q.stages) {
                 stage = 0;
                 phase ^= 1;
@@ -265,13 +277,13 @@ __global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const Spli
     } else if (warp >= kEpilogue && warp < kEpilogue + kGroups * kGroupWarps) {
         // group g brings every second slice: while one waits for memory the other writes
         const int group = (warp - kEpilogue) / kGroupWarps, t = threadIdx.x - 32 * (kEpilogue + group * kGroupWarps);
-        int64_t slice = group;      // counts this CTA's slices
-        for (; slice < my_slices; slice += kGroups) {
-            const int64_t nth = slice / chunks, tile = walker + nth * walkers;
-            const int c = (int)(slice - nth * chunks), stage = (int)(slice % q.stages);
-            const uint32_t phase = (uint32_t)(slice / q.stages) & 1;
-            const int sample = (int)(tile / q.tiles_p);
-            const int64_t p0 = (tile - (int64_t)sample * q.tiles_p) * 128;
+        uint32_t stage = group, phase = 0;
+        Cursor at{walker, 0};
+        if (group) advance(at);
+        for (; at.tile < tiles; advance(at), advance(at)) {
+            const int c = at.c;
+            const unsigned sample = at.tile / (unsigned)q.tiles_p;
+            const int64_t p0 = (int64_t)(at.tile - sample * q.tiles_p) * 128;
             const int pixels = (int)min((int64_t)128, q.P - p0), k_left = q.K - 64 * c, k_used = (k_left + 15) / 16 * 16;
             const T *a = a_all + (LAST ? p0 * q.K + 64 * c : ((int64_t)sample * q.K + 64 * c) * q.P + p0);
             // a vector: planes, eight pixels of a k; last, eight k of a pixel.  `inner` of it are there.
@@ -288,19 +300,23 @@ __global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const Spli
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int e = t + 128 * j;
-                const uint32_t at = LAST ? (e >> 3) * 128 + (((e & 7) ^ (e >> 3 & 7)) << 4)
-                                         : (e >> 3 & 1) * kBlockBytes + (e >> 4) * 128 + (((e & 7) ^ (e >> 4 & 7)) << 4);
+                const uint32_t place = LAST ? (e >> 3) * 128 + (((e & 7) ^ (e >> 3 & 7)) << 4)
+                                            : (e >> 3 & 1) * kBlockBytes + (e >> 4) * 128 + (((e & 7) ^ (e >> 4 & 7)) << 4);
                 if ((LAST ? 8 * (e & 7) : e >> 4) >= k_used) continue;
-                place8<T>(to + at, kPart, raw_v[j]);
+                place8<T>(to + place, kPart, raw_v[j]);
             }
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(full + 8 * stage);
+            if ((stage += kGroups) >= (uint32_t)q.stages) {
+                stage -= q.stages;
+                phase ^= 1;
+            }
         }
     } else if (warp == kEpilogue + kGroups * kGroupWarps) {
         if (lane == 0) {
             uint32_t stage = 0, phase = 0, set = 0, set_phase = 0;
-            for (int64_t tile = walker; tile < tiles; tile += walkers) {
+            for (unsigned tile = walker; tile < tiles; tile += walkers) {
                 if (!wait(drained + 8 * set, set_phase ^ 1)) break;
                 tmem_acquire();
                 for (int c = 0; c < chunks; ++c) {
@@ -335,9 +351,9 @@ __global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const Spli
         const T *residual = static_cast<const T *>(q.residual), *grad = static_cast<const T *>(q.grad);
         T *out = static_cast<T *>(q.out);
         uint32_t set = 0, set_phase = 0;
-        for (int64_t tile = walker; tile < tiles; tile += walkers) {
-            const int sample = (int)(tile / q.tiles_p);
-            const int64_t p0 = (tile - (int64_t)sample * q.tiles_p) * 128 + quarter * 32;
+        for (unsigned tile = walker; tile < tiles; tile += walkers) {
+            const unsigned sample = tile / (unsigned)q.tiles_p;
+            const int64_t p0 = (int64_t)(tile - sample * q.tiles_p) * 128 + quarter * 32;
             const int rows = (int)max((int64_t)0, min((int64_t)32, q.P - p0));
             // Blocks of 16 channels, 16 values a lane, coalesced: planes, the lane's pixel and channel i; last, pixel
             // 2 i + (lane >> 4) and channel lane & 15.  What the block reads is on its way before its sums are there.
@@ -457,7 +473,7 @@ struct WeightSplit {
     const void *dz, *x;
     float *partial;          // a row a split: Co * Ci sums, then Co sums of dz
     int64_t P;
-    int64_t per, slices;     // slices of a split; of a sample
+    int per, slices;         // slices of a split; of a sample
     int samples, Ci, Co;
     int tiles_i;
     int rows, bn, stages, slots, columns;      // output and input channels of a tile; ring; floats' slices on their way
@@ -494,7 +510,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
     const int tiles_o = (q.Co + q.rows - 1) / q.rows, tiles = tiles_o * q.tiles_i;
     const int split = (int)(blockIdx.x / (unsigned)tiles), t = (int)blockIdx.x - split * tiles;
     const int o0 = t / q.tiles_i * q.rows, i0 = (t - t / q.tiles_i * q.tiles_i) * q.bn;
-    const int64_t first = split * q.per, last = min((int64_t)q.samples * q.slices, first + q.per);
+    const int first = split * q.per, last = min(q.samples * q.slices, first + q.per);      // (all of them below 2^30)
     const bool sums = q.sums && i0 == 0;
     const uint32_t columns = (PARTS > 1 ? 2 : 1) * q.columns;
     const T *dz_all = static_cast<const T *>(q.dz), *x_all = static_cast<const T *>(q.x);
@@ -521,17 +537,27 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
         const int of_dz = q.rows * 8, total = of_dz + q.bn * 8;
         const uint32_t slot_bytes = lay.each() * 32 * kProducers;
         const char *own = smem + lay.copies() + 16 * t;
-        auto copy = [&](int64_t slice) {
+        int outer_of[8], chunk_of[8];      // last: pixels and places among the channels of the thread's vectors
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int e = t + kProducers * j, f = e < of_dz ? e : e - of_dz, wide = (e < of_dz ? q.rows : q.bn) / 8;
+            outer_of[j] = (unsigned)f / (unsigned)wide;
+            chunk_of[j] = f - outer_of[j] * wide;
+        }
+        auto copy = [&](int slice) {
             if (slice < last) {
-                const int64_t sample = slice / q.slices, p0 = (slice - sample * q.slices) * 64;
+                const int64_t sample = (unsigned)slice / (unsigned)q.slices, p0 = (slice - sample * q.slices) * 64;
                 const int pixels = (int)min((int64_t)64, q.P - p0);
                 const uint32_t to = smem_u32(own) + (q.slots > 1 ? (uint32_t)(slice - first & 1) * slot_bytes : 0);
-                for (int j = 0, e = t; e < total; ++j, e += kProducers) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int e = t + kProducers * j;
+                    if (e >= total) break;
                     const bool dz = e < of_dz;
-                    const int f = dz ? e : e - of_dz, C = dz ? q.Co : q.Ci, c0 = dz ? o0 : i0, wide = (dz ? q.rows : q.bn) / 8;
+                    const int f = dz ? e : e - of_dz, C = dz ? q.Co : q.Ci, c0 = dz ? o0 : i0;
                     const float *from = reinterpret_cast<const float *>(dz ? q.dz : q.x);
                     if (LAST) {      // eight channels of a pixel
-                        const int p = f / wide, c = c0 + 8 * (f - p * wide);
+                        const int p = outer_of[j], c = c0 + 8 * chunk_of[j];
                         copy8<VEC>(to + 8192 * j, 4096, from + (p0 + p) * C + c, p < pixels ? C - c : 0, from);
                     } else {         // eight pixels of a channel
                         const int c = c0 + (f >> 3), p = 8 * (f & 7);
@@ -544,7 +570,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
         for (int i = 0; i < q.slots; ++i) copy(first + i);
         float sum[8] = {};      // planes: of the channel of vector t + 256 j; last: of the channels of every vector of dz
         uint32_t stage = 0, phase = 0;
-        for (int64_t slice = first; slice < last; ++slice) {
+        for (int slice = first; slice < last; ++slice) {
             copies_wait(q.slots);
             if (!wait(empty + 8 * stage, phase ^ 1)) break;
             char *const dz_to = smem + stage * lay.stage(), *const x_to = dz_to + PARTS * lay.dz_part();
@@ -554,8 +580,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
                 const int e = t + kProducers * j;
                 if (e >= total) break;
                 const bool dz = e < of_dz;
-                const int f = dz ? e : e - of_dz, wide = (dz ? q.rows : q.bn) / 8;
-                const int outer = LAST ? f / wide : f >> 3, chunk = LAST ? f - outer * wide : f & 7;
+                const int f = dz ? e : e - of_dz, outer = LAST ? outer_of[j] : f >> 3, chunk = LAST ? chunk_of[j] : f & 7;
                 char *to = (dz ? dz_to : x_to) + (LAST ? (chunk >> 3) * kBlockBytes : 0) + outer * 128 + (((chunk & 7) ^ (outer & 7)) << 4);
                 const uint4 v[2] = {*reinterpret_cast<const uint4 *>(from + 8192 * j),
                                                          *reinterpret_cast<const uint4 *>(from + 8192 * j + 4096)};
@@ -607,11 +632,9 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
         const int group = (warp - kWeightEpilogue) / kGroupWarps, me = threadIdx.x - 32 * (kWeightEpilogue + group * kGroupWarps);
         const int of_dz = q.rows * 8, total = of_dz + q.bn * 8;      // vectors of a slice
         float sum[8] = {};      // planes: of the channel of vector me + 128 j; last: of the channels of every vector of dz
-        for (int64_t slice = first + group; slice < last; slice += kGroups) {
-            const int64_t nth = slice - first;
-            const int stage = (int)(nth % q.stages);
-            const uint32_t phase = (uint32_t)(nth / q.stages) & 1;
-            const int64_t sample = slice / q.slices, p0 = (slice - sample * q.slices) * 64;
+        for (int slice = first + group; slice < last; slice += kGroups) {
+            const unsigned nth = slice - first, stage = nth % (unsigned)q.stages, phase = nth / (unsigned)q.stages & 1;
+            const int64_t sample = (unsigned)slice / (unsigned)q.slices, p0 = (slice - sample * q.slices) * 64;
             const int pixels = (int)min((int64_t)64, q.P - p0);
             char *const dz_to = smem + stage * lay.stage(), *const x_to = dz_to + PARTS * lay.dz_part();
             bool waited = false;
@@ -625,7 +648,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
                     const int f = dz ? e : e - of_dz, C = dz ? q.Co : q.Ci, c0 = dz ? o0 : i0, wide = (dz ? q.rows : q.bn) / 8;
                     const T *from = dz ? dz_all : x_all;
                     if (LAST) {      // eight channels of a pixel
-                        const int p = f / wide, c = c0 + 8 * (f - p * wide);
+                        const int p = (unsigned)f / (unsigned)wide, c = c0 + 8 * (f - p * wide);
                         load8<T, VEC>(from + (p0 + p) * C + c, p < pixels ? C - c : 0, v[j]);
                     } else {         // eight pixels of a channel
                         const int c = c0 + (f >> 3), p = 8 * (f & 7);
@@ -642,7 +665,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
                     if (e >= total) break;
                     const bool dz = e < of_dz;
                     const int f = dz ? e : e - of_dz, wide = (dz ? q.rows : q.bn) / 8;
-                    const int outer = LAST ? f / wide : f >> 3, chunk = LAST ? f - outer * wide : f & 7;
+                    const int outer = LAST ? (unsigned)f / (unsigned)wide : f >> 3, chunk = LAST ? f - outer * wide : f & 7;
                     char *to = (dz ? dz_to : x_to) + (LAST ? (chunk >> 3) * kBlockBytes : 0) + outer * 128 + (((chunk & 7) ^ (outer & 7)) << 4);
                     place8<T>(to, dz ? lay.dz_part() : lay.x_part(), v[j]);
                     if (sums && dz) {
@@ -688,7 +711,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
     } else if (warp == kWeightEpilogue + kGroups * kGroupWarps) {
         if (lane == 0) {
             uint32_t stage = 0, phase = 0;
-            for (int64_t slice = first; slice < last; ++slice) {
+            for (int slice = first; slice < last; ++slice) {
                 if (!wait(full + 8 * stage, phase)) break;
                 tmem_acquire();
                 const uint32_t a = base + stage * lay.stage(), b = a + PARTS * lay.dz_part();
@@ -731,8 +754,8 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
                 if (finite != 0.f && mine) {      // (a NaN: some value is not finite)
 #pragma unroll
                     for (int j = 0; j < 16; ++j) u[j] = 0.f;
-                    for (int64_t slice = first; slice < last; ++slice) {
-                        const int64_t sample = slice / q.slices, p0 = (slice - sample * q.slices) * 64;
+                    for (int slice = first; slice < last; ++slice) {
+                        const int64_t sample = (unsigned)slice / (unsigned)q.slices, p0 = (slice - sample * q.slices) * 64;
                         for (int64_t p = p0; p < min(p0 + 64, q.P); ++p) {
                             const float g = to_float(dz_all[LAST ? p * q.Co + o : (sample * q.Co + o) * q.P + p]);
 #pragma unroll
@@ -894,7 +917,7 @@ bool plan_weight_split(const PointwiseShape &s, WeightSplitPlan *plan)
     const int64_t all = r.slices * samples, tiles = (int64_t)r.tiles_o * r.tiles_i;
     r.per = std::max<int64_t>(std::min<int64_t>(4, all), ceil_div(all, std::max<int64_t>(1, 148 / tiles)));
     r.splits = (int)ceil_div(all, r.per);
-    if (r.splits * tiles > INT32_MAX) return false;
+    if (all >= 1 << 30 || r.splits * tiles > INT32_MAX) return false;
     *plan = r;
     return true;
 }
@@ -914,8 +937,8 @@ int launch_pointwise_split_weight(const PointwiseShape &s, const void *dz, const
     q.x = x;
     q.partial = partial;
     q.P = s.last ? s.N * s.P : s.P;
-    q.per = plan.per;
-    q.slices = plan.slices;
+    q.per = (int)plan.per;
+    q.slices = (int)plan.slices;
     q.samples = s.last ? 1 : s.N;
     q.Ci = s.Ci;
     q.Co = s.Co;
