@@ -26,6 +26,10 @@ __device__ __forceinline__ uint64_t k_major(uint32_t addr, int k) { return opera
 // MN-major: blocks `block` bytes apart; 8 k are an atom of 1024 bytes.
 __device__ __forceinline__ uint64_t mn_major(uint32_t addr, int k, uint32_t block) { return operand(addr + 128 * k, block, 1024); }
 
+// The same operand `bytes` further on.  (The issuing thread is alone on its scheduler slot: what it computes for every
+// instruction, the tensor cores wait for.)
+__device__ __forceinline__ uint64_t further(uint64_t operand, uint32_t bytes) { return operand + (bytes >> 4); }
+
 // 16-bit operands of one type, float accumulators, M 128.
 __host__ __device__ inline uint32_t mma_instruction(bool bf16, bool a_mn, bool b_mn, int n)
 {

@@ -124,6 +124,8 @@ __global__ void __launch_bounds__(32 * (kEpilogue * PAIR + 2), PAIR == 1 ? 2 : 1
     } else if (warp == WARPS + 1) {
         if (lane == 0) {
             wait(weights_full, 0);
+            const uint64_t ring = LAST ? k_major(base + lay.ring(), 0) : mn_major(base + lay.ring(), 0, kBlockBytes);
+            const uint64_t weights = MODE == INPUT ? mn_major(base, 0, kBlockBytes) : k_major(base, 0);
             uint32_t stage = 0, phase = 0, set = 0, set_phase = 0;
             for (unsigned tile = walker; tile < tiles; tile += walkers) {
                 if (!wait(drained + 8 * set, set_phase ^ 1)) break;
@@ -131,11 +133,12 @@ __global__ void __launch_bounds__(32 * (kEpilogue * PAIR + 2), PAIR == 1 ? 2 : 1
                 for (int c = 0; c < chunks; ++c) {
                     if (!wait(full + 8 * stage, phase)) break;
                     tmem_acquire();
-                    const uint32_t a = base + lay.ring() + stage * kStage, w = base + c * lay.slice();
-                    const int steps = (min(64, q.K - 64 * c) + 15) / 16;
-                    for (int k = 0; k < 16 * steps; k += 16)
-                        mma(tmem + set * q.columns, LAST ? k_major(a, k) : mn_major(a, k, kBlockBytes),
-                            MODE == INPUT ? mn_major(w, k, kBlockBytes) : k_major(w, k), q.instruction, c || k);
+                    const uint64_t a = further(ring, stage * kStage), w = further(weights, c * lay.slice());
+                    const int k_used = q.K - 64 * c;
+#pragma unroll
+                    for (int k = 0; k < 64; k += 16)
+                        if (k < k_used)
+                            mma(tmem + set * q.columns, further(a, (LAST ? 2 : 128) * k), further(w, (MODE == INPUT ? 128 : 2) * k), q.instruction, c || k);
                     mma_commit(empty + 8 * stage);
                     if (++stage == (uint32_t)q.stages) {
                         stage = 0;

@@ -315,6 +315,9 @@ __global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const Spli
         }
     } else if (warp == kEpilogue + kGroups * kGroupWarps) {
         if (lane == 0) {
+            const uint64_t ring = LAST ? k_major(base + lay.ring(), 0) : mn_major(base + lay.ring(), 0, kBlockBytes);
+            uint64_t weights[PARTS];
+            for (int j = 0; j < PARTS; ++j) weights[j] = k_major(base + j * chunks * lay.slice(), 0);
             uint32_t stage = 0, phase = 0, set = 0, set_phase = 0;
             for (unsigned tile = walker; tile < tiles; tile += walkers) {
                 if (!wait(drained + 8 * set, set_phase ^ 1)) break;
@@ -322,18 +325,21 @@ __global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const Spli
                 for (int c = 0; c < chunks; ++c) {
                     if (!wait(full + 8 * stage, phase)) break;
                     tmem_acquire();
-                    const uint32_t a = base + lay.ring() + stage * PARTS * kPart, w = base + c * lay.slice();
-                    const int steps = (min(64, q.K - 64 * c) + 15) / 16;
-                    for (int k = 0; k < 16 * steps; k += 16) {
+                    const uint64_t a = further(ring, stage * PARTS * kPart);
+                    uint64_t w[PARTS];
 #pragma unroll
-                        for (int i = 0; i < PARTS; ++i)
+                    for (int j = 0; j < PARTS; ++j) w[j] = further(weights[j], c * lay.slice());
+                    const int k_used = q.K - 64 * c;
+                    const uint32_t d = tmem + set * set_columns;
 #pragma unroll
-                            for (int j = 0; j < PARTS - i; ++j) {
-                                const uint32_t ai = a + i * kPart, wj = w + j * chunks * lay.slice();
-                                mma(tmem + set * set_columns + (i + j ? q.columns : 0), LAST ? k_major(ai, k) : mn_major(ai, k, kBlockBytes), k_major(wj, k),
-                                    q.instruction, c || k || i + j > 1 || i > 0);
-                            }
-                    }
+                    for (int k = 0; k < 64; k += 16)
+                        if (k < k_used)
+#pragma unroll
+                            for (int i = 0; i < PARTS; ++i)
+#pragma unroll
+                                for (int j = 0; j < PARTS - i; ++j)
+                                    mma(i + j ? d + q.columns : d, further(a, i * kPart + (LAST ? 2 : 128) * k), further(w[j], 2 * k), q.instruction,
+                                        c || k || i + j > 1 || i > 0);
                     mma_commit(empty + 8 * stage);
                     if (++stage == (uint32_t)q.stages) {
                         stage = 0;
@@ -710,21 +716,25 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
         }
     } else if (warp == kWeightEpilogue + kGroups * kGroupWarps) {
         if (lane == 0) {
+            uint64_t a[PARTS], b[PARTS];
+            for (int i = 0; i < PARTS; ++i) {
+                const uint32_t dz = base + i * lay.dz_part(), x = base + PARTS * lay.dz_part() + i * lay.x_part();
+                a[i] = LAST ? mn_major(dz, 0, kBlockBytes) : k_major(dz, 0);
+                b[i] = LAST ? mn_major(x, 0, kBlockBytes) : k_major(x, 0);
+            }
             uint32_t stage = 0, phase = 0;
             for (int slice = first; slice < last; ++slice) {
                 if (!wait(full + 8 * stage, phase)) break;
                 tmem_acquire();
-                const uint32_t a = base + stage * lay.stage(), b = a + PARTS * lay.dz_part();
+                const uint32_t stage_at = stage * lay.stage();
 #pragma unroll
                 for (int k = 0; k < 64; k += 16)
 #pragma unroll
                     for (int i = 0; i < PARTS; ++i)
 #pragma unroll
-                        for (int j = 0; j < PARTS - i; ++j) {
-                            const uint32_t ai = a + i * lay.dz_part(), bj = b + j * lay.x_part();
-                            mma(tmem + (i + j ? q.columns : 0), LAST ? mn_major(ai, k, kBlockBytes) : k_major(ai, k),
-                                LAST ? mn_major(bj, k, kBlockBytes) : k_major(bj, k), q.instruction, slice > first || k || i + j > 1 || i > 0);
-                        }
+                        for (int j = 0; j < PARTS - i; ++j)
+                            mma(i + j ? tmem + q.columns : tmem, further(a[i], stage_at + (LAST ? 128 : 2) * k), further(b[j], stage_at + (LAST ? 128 : 2) * k),
+                                q.instruction, slice > first || k || i + j > 1 || i > 0);
                 mma_commit(empty + 8 * stage);
                 if (++stage == (uint32_t)q.stages) {
                     stage = 0;
