@@ -34,6 +34,7 @@ struct SplitProduct {
     int wn, wk;              // strides of W along the output's and the operand's channels
     int tiles_p, tiles_n;
     int bn, stages, columns;
+    bool merged;             // float: the weights' three parts are one operand, and three sets of sums lie side by side
     uint32_t instruction;
 };
 
@@ -43,69 +44,45 @@ struct SplitLayout {
     bool last;
     __host__ __device__ uint32_t slice() const { return (uint32_t)bn * 128; }      // 64 k of one part of the weights
     __host__ __device__ uint32_t ring() const { return parts * chunks * slice(); }
-    __host__ __device__ uint32_t copies() const { return ring() + stages * parts * kPart; }      // two slices of floats as they come
-    __host__ __device__ uint32_t staging() const { return copies() + (parts == 3 ? 2 * kCopies : 0); }
+    __host__ __device__ uint32_t copies() const { return ring() + stages * parts * kPart; }      // a slice of floats as they come
+    __host__ __device__ uint32_t staging() const { return copies() + (parts == 3 ? kCopies : 0); }
     __host__ __device__ uint32_t bias() const { return staging() + (last ? kEpilogue * 32 * kPitch * 4 : 0); }
     __host__ __device__ uint32_t sums() const { return bias() + bn * 4; }
     __host__ __device__ uint32_t barriers() const { return (sums() + 4 * bn * 4 + 7) / 8 * 8; }
     __host__ __device__ uint32_t bytes() const { return barriers() + (2 * stages + 4) * 8 + 8 + 1024; }
 };
 
-// Eight floats as three vectors of bf16.  (An infinity leaves a NaN behind: what comes of it is computed again.)
-__device__ __forceinline__ void split8(const float (&v)[8], uint4 (&part)[3])
+// Floats, two and four of them, as bf16 parts.  (An infinity leaves a NaN behind: what comes of it is computed again.)
+__device__ __forceinline__ void split2(float a, float b, uint32_t (&part)[3])
 {
-    uint32_t w[3][4];
+    f2_t x = pack2(a, b);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        f2_t x = pack2(v[2 * i], v[2 * i + 1]);
-#pragma unroll
-        for (int p = 0; p < 3; ++p) {
-            float lo, hi;
-            unpack2(x, lo, hi);
-            w[p][i] = __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632);
-            if (p < 2) x = sub2(x, pack2(__uint_as_float(__float_as_uint(lo) & 0xffff0000u), __uint_as_float(__float_as_uint(hi) & 0xffff0000u)));
-        }
-    }
-#pragma unroll
-    for (int p = 0; p < 3; ++p) part[p] = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
-}
-
-// Eight values from `from` on, of which `n` are there (zeros beyond); VEC: whole vectors, aligned.
-template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T *from, int n, uint4 (&v)[2])
-{
-    if constexpr (VEC) {
-        constexpr int EACH = 16 / sizeof(T);
-#pragma unroll
-        for (int i = 0; i < 8 / EACH; ++i) v[i] = n > i * EACH ? *reinterpret_cast<const uint4 *>(from + i * EACH) : make_uint4(0, 0, 0, 0);
-    } else if constexpr (sizeof(T) == 4) {
-        float f[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = i < n ? from[i] : 0.f;
-        v[0] = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
-        v[1] = make_uint4(__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]), __float_as_uint(f[7]));
-    } else {
-        const unsigned short *bits = reinterpret_cast<const unsigned short *>(from);
-        uint32_t f[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = i < n ? bits[i] : 0;
-        v[0] = make_uint4(f[0] | f[1] << 16, f[2] | f[3] << 16, f[4] | f[5] << 16, f[6] | f[7] << 16);
+    for (int p = 0; p < 3; ++p) {
+        float lo, hi;
+        unpack2(x, lo, hi);
+        part[p] = __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632);
+        if (p < 2) x = sub2(x, pack2(__uint_as_float(__float_as_uint(lo) & 0xffff0000u), __uint_as_float(__float_as_uint(hi) & 0xffff0000u)));
     }
 }
-// Floats on their way into the thread's own place in shared memory, two vectors `half` bytes apart; zeros beyond n.
+// Into their place of every part, `part` bytes apart.
+__device__ __forceinline__ void place4(char *to, uint32_t part, const float4 &v)
+{
+    uint32_t lo[3], hi[3];
+    split2(v.x, v.y, lo);
+    split2(v.z, v.w, hi);
+#pragma unroll
+    for (int p = 0; p < 3; ++p) *reinterpret_cast<uint2 *>(to + p * part) = make_uint2(lo[p], hi[p]);
+}
+// Four of them on their way into the thread's own place in shared memory, zeros beyond n.
 template <bool VEC>
-__device__ __forceinline__ void copy8(uint32_t to, uint32_t half, const float *from, int n, const float *base)
+__device__ __forceinline__ void copy4(uint32_t to, const float *from, int n, const float *base)
 {
     if (VEC) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + i * half), "l"(n > 4 * i ? from + 4 * i : base), "r"(n > 4 * i ? 16 : 0)
-                         : "memory");
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(n > 0 ? from : base), "r"(n > 0 ? 16 : 0) : "memory");
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;"
-                         ::"r"(to + i / 4 * half + i % 4 * 4), "l"(n > i ? from + i : base), "r"(n > i ? 4 : 0) : "memory");
+        for (int i = 0; i < 4; ++i)
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + 4 * i), "l"(n > i ? from + i : base), "r"(n > i ? 4 : 0) : "memory");
     }
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -116,35 +93,16 @@ __device__ __forceinline__ void copies_wait(int slots)
     else asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-template <typename T>
-__device__ __forceinline__ void floats8(const uint4 (&v)[2], float (&f)[8])
+// Eight 16-bit values from `from` on, of which `n` are there (zeros beyond); VEC: whole vectors, aligned.
+template <typename T, bool VEC>
+__device__ __forceinline__ uint4 load8(const T *from, int n)
 {
-    if constexpr (sizeof(T) == 4) {
-        float g[4];
-        unpack<float>(v[0], g);
+    if constexpr (VEC) return n > 0 ? *reinterpret_cast<const uint4 *>(from) : make_uint4(0, 0, 0, 0);
+    const unsigned short *bits = reinterpret_cast<const unsigned short *>(from);
+    uint32_t f[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) f[i] = g[i];
-        unpack<float>(v[1], g);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) f[4 + i] = g[i];
-    } else {
-        unpack<T>(v[0], f);
-    }
-}
-// Into their place of every part, `part` bytes apart.
-template <typename T>
-__device__ __forceinline__ void place8(char *to, uint32_t part, const uint4 (&v)[2])
-{
-    if constexpr (sizeof(T) == 4) {
-        float f[8];
-        uint4 parts[3];
-        floats8<T>(v, f);
-        split8(f, parts);
-#pragma unroll
-        for (int p = 0; p < 3; ++p) *reinterpret_cast<uint4 *>(to + p * part) = parts[p];
-    } else {
-        *reinterpret_cast<uint4 *>(to) = v[0];
-    }
+    for (int i = 0; i < 8; ++i) f[i] = i < n ? bits[i] : 0;
+    return make_uint4(f[0] | f[1] << 16, f[2] | f[3] << 16, f[4] | f[5] << 16, f[6] | f[7] << 16);
 }
 
 template <typename T, int MODE, int ACT, bool LAST, bool VEC>
@@ -163,7 +121,7 @@ __global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const Spli
     const unsigned walkers = gridDim.x / (unsigned)q.tiles_n, walker = blockIdx.x / (unsigned)q.tiles_n;
     const int n0 = (int)(blockIdx.x - walker * q.tiles_n) * q.bn;
     const unsigned tiles = (unsigned)q.samples * (unsigned)q.tiles_p;      // (below 2^31)
-    const uint32_t set_columns = (PARTS > 1 ? 2 : 1) * q.columns;
+    const uint32_t set_columns = q.merged ? q.columns : (PARTS > 1 ? 2 : 1) * q.columns;
     const T *w_all = static_cast<const T *>(q.w), *a_all = static_cast<const T *>(q.a);
 
     if (threadIdx.x == 0) {
@@ -189,17 +147,21 @@ __global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const Spli
             // (along the weights' rows: k forward, channels for grad_input)
             const int n = MODE == INPUT ? e % q.bn : e / (chunks * 8), k8 = MODE == INPUT ? e / q.bn : e % (chunks * 8);
             float v[8];
-            uint4 part[3];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int k = 8 * k8 + j;
                 v[j] = k < q.K && n0 + n < q.Cn ? to_float(w_all[(int64_t)(n0 + n) * q.wn + (int64_t)k * q.wk]) : 0.f;
             }
-            if constexpr (PARTS == 3) split8(v, part);
-            else part[0] = pack<T>(v);
-            char *to = smem + (k8 >> 3) * lay.slice() + n * 128 + (((k8 & 7) ^ (n & 7)) << 4);
+            char *to = smem + (k8 >> 3) * PARTS * lay.slice() + n * 128 + (((k8 & 7) ^ (n & 7)) << 4);
+            if constexpr (PARTS == 3) {
+                place4(to, lay.slice(), make_float4(v[0], v[1], v[2], v[3]));
+                place4(to + 8, lay.slice(), make_float4(v[4], v[5], v[6], v[7]));
+            } else {
+                uint32_t h[4];
 #pragma unroll
-            for (int p = 0; p < PARTS; ++p) *reinterpret_cast<uint4 *>(to + p * chunks * lay.slice()) = part[p];
+                for (int j = 0; j < 4; ++j) h[j] = narrow2(v[2 * j], v[2 * j + 1], T());
+                *reinterpret_cast<uint4 *>(to) = make_uint4(h[0], h[1], h[2], h[3]);
+            }
         }
     }
     fence_proxy_async();
@@ -221,53 +183,47 @@ __global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const Spli
         }
     };
     if (PARTS == 3 && warp >= kEpilogue && warp < kEpilogue + kGroups * kGroupWarps) {
-        // Every thread has four vectors of a slice: it copies them to a place of its own, two slices ahead, and splits them from there.
+        // A thread has eight vectors of four floats of a slice: it copies them to a place of its own and splits them from
+        // there, the next slice's on their way.
         const int t = threadIdx.x - 32 * kEpilogue;
         const float *all = reinterpret_cast<const float *>(q.a);
         const char *own = smem + lay.copies() + 16 * t;
+        // planes: four pixels of a k; last: four k of a pixel
+        const int in = 4 * (LAST ? t & 15 : t & 31), outer0 = LAST ? t >> 4 : t >> 5, outer_step = LAST ? kProducers / 16 : kProducers / 32;
+        const int64_t pitch = LAST ? (int64_t)q.K : q.P;
         Cursor ahead{walker, 0};
-        uint32_t to_slot = 0;
         auto copy = [&] {
             if (ahead.tile < tiles) {
                 const unsigned sample = ahead.tile / (unsigned)q.tiles_p;
                 const int64_t p0 = (int64_t)(ahead.tile - sample * q.tiles_p) * 128;
                 const int pixels = (int)min((int64_t)128, q.P - p0), k_left = q.K - 64 * ahead.c;
-                const float *a = all + (LAST ? p0 * q.K + 64 * ahead.c : ((int64_t)sample * q.K + 64 * ahead.c) * q.P + p0);
+                const float *a = all + (LAST ? p0 * q.K + 64 * ahead.c : ((int64_t)sample * q.K + 64 * ahead.c) * q.P + p0) + outer0 * pitch + in;
+                const int inner = (LAST ? k_left : pixels) - in, outers = (LAST ? pixels : k_left) - outer0;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int e = t + kProducers * j, in = 8 * (LAST ? e & 7 : e & 15), outer = LAST ? e >> 3 : e >> 4;
-                    const int inner = outer < (LAST ? pixels : k_left) ? (LAST ? k_left : pixels) - in : 0;
-                    copy8<VEC>(smem_u32(own) + to_slot + 8192 * j, 4096, a + outer * (LAST ? (int64_t)q.K : q.P) + in, inner, all);
-                }
+                for (int j = 0; j < 8; ++j)
+                    copy4<VEC>(smem_u32(own) + 4096 * j, a + j * outer_step * pitch, j * outer_step < outers ? inner : 0, all);
                 advance(ahead);
-                to_slot ^= kCopies;
             }
             copies_commit();
         };
         copy();
-        copy();
-        uint32_t stage = 0, phase = 0, from_slot = 0;
+        uint32_t stage = 0, phase = 0;
         for (Cursor at{walker, 0}; at.tile < tiles; advance(at)) {
-            copies_wait(2);
-            if (!wait(empty + 8 * stage, phase ^ 1)) break;
-            const int k_used = (q.K - 64 * at.c + 15) / 16 * 16;
-            char *to = smem + lay.ring() + stage * PARTS * kPart;
-            const char *from = own + from_slot;
-            from_slot ^= kCopies;
+            copies_wait(1);
+            float4 v[8];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int e = t + kProducers * j;
-                const uint32_t place = LAST ? (e >> 3) * 128 + (((e & 7) ^ (e >> 3 & 7)) << 4)
-                                            : (e >> 3 & 1) * kBlockBytes + (e >> 4) * 128 + (((e & 7) ^ (e >> 4 & 7)) << 4);
-                if ((LAST ? 8 * (e & 7) : e >> 4) >= k_used) continue;
-                const uint4 v[2] = {*reinterpret_cast<const uint4 *>(from + 8192 * j),
-                                                         *reinterpret_cast<const uint4 *>(from + 8192 * j + 4096)};
-                place8<T>(to + place, kPart, v);
+            for (int j = 0; j < 8; ++j) v[j] = *reinterpret_cast<const float4 *>(own + 4096 * j);
+            copy();
+            if (!wait(empty + 8 * stage, phase ^ 1)) break;
+            char *to = smem + lay.ring() + stage * PARTS * kPart + (in & 4) * 2;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int outer = outer0 + j * outer_step;
+                place4(to + (LAST ? 0 : (in >> 6) * kBlockBytes) + outer * 128 + ((((in >> 3) & 7) ^ (outer & 7)) << 4), kPart, v[j]);
             }
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(full + 8 * stage);
-            copy();
             if (++stage == (uint32_t)q.stages) {
                 stage = 0;
                 phase ^= 1;
@@ -287,13 +243,13 @@ __global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const Spli
             const int pixels = (int)min((int64_t)128, q.P - p0), k_left = q.K - 64 * c, k_used = (k_left + 15) / 16 * 16;
             const T *a = a_all + (LAST ? p0 * q.K + 64 * c : ((int64_t)sample * q.K + 64 * c) * q.P + p0);
             // a vector: planes, eight pixels of a k; last, eight k of a pixel.  `inner` of it are there.
-            uint4 raw_v[8][2];
+            uint4 raw_v[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int e = t + 128 * j, in = 8 * (LAST ? e & 7 : e & 15), outer = LAST ? e >> 3 : e >> 4;
                 const int inner = outer < (LAST ? pixels : k_left) ? (LAST ? k_left : pixels) - in : 0;
                 const T *from = a + outer * (LAST ? (int64_t)q.K : q.P) + in;
-                load8<T, VEC>(from, inner, raw_v[j]);
+                if constexpr (PARTS == 1) raw_v[j] = load8<T, VEC>(from, inner);
             }
             if (!wait(empty + 8 * stage, phase ^ 1)) break;
             char *to = smem + lay.ring() + stage * PARTS * kPart;
@@ -303,7 +259,7 @@ __global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const Spli
                 const uint32_t place = LAST ? (e >> 3) * 128 + (((e & 7) ^ (e >> 3 & 7)) << 4)
                                             : (e >> 3 & 1) * kBlockBytes + (e >> 4) * 128 + (((e & 7) ^ (e >> 4 & 7)) << 4);
                 if ((LAST ? 8 * (e & 7) : e >> 4) >= k_used) continue;
-                place8<T>(to + place, kPart, raw_v[j]);
+                *reinterpret_cast<uint4 *>(to + place) = raw_v[j];
             }
             fence_proxy_async();
             __syncwarp();
@@ -316,8 +272,7 @@ __global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const Spli
     } else if (warp == kEpilogue + kGroups * kGroupWarps) {
         if (lane == 0) {
             const uint64_t ring = LAST ? k_major(base + lay.ring(), 0) : mn_major(base + lay.ring(), 0, kBlockBytes);
-            uint64_t weights[PARTS];
-            for (int j = 0; j < PARTS; ++j) weights[j] = k_major(base + j * chunks * lay.slice(), 0);
+            const uint64_t weights = k_major(base, 0);
             uint32_t stage = 0, phase = 0, set = 0, set_phase = 0;
             for (unsigned tile = walker; tile < tiles; tile += walkers) {
                 if (!wait(drained + 8 * set, set_phase ^ 1)) break;
@@ -326,20 +281,27 @@ __global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const Spli
                     if (!wait(full + 8 * stage, phase)) break;
                     tmem_acquire();
                     const uint64_t a = further(ring, stage * PARTS * kPart);
-                    uint64_t w[PARTS];
-#pragma unroll
-                    for (int j = 0; j < PARTS; ++j) w[j] = further(weights[j], c * lay.slice());
+                    const uint64_t w = further(weights, c * PARTS * lay.slice());
                     const int k_used = q.K - 64 * c;
                     const uint32_t d = tmem + set * set_columns;
 #pragma unroll
                     for (int k = 0; k < 64; k += 16)
-                        if (k < k_used)
+                        if (k < k_used) {
+                            const uint64_t ak = further(a, (LAST ? 2 : 128) * k), wk = further(w, 2 * k);
+                            if (PARTS == 3 && q.merged) {
+                                // the weights' parts in a row are one operand: an instruction takes some 90 cycles at any width here
+                                mma(d, ak, wk, q.instruction, c || k);
+                                mma(d + q.bn, further(ak, kPart), wk, q.instruction - (q.bn >> 3 << 17), true);
+                                mma(d + 2 * q.bn, further(ak, 2 * kPart), wk, q.instruction - (2 * q.bn >> 3 << 17), true);
+                            } else {
 #pragma unroll
-                            for (int i = 0; i < PARTS; ++i)
+                                for (int i = 0; i < PARTS; ++i)
 #pragma unroll
-                                for (int j = 0; j < PARTS - i; ++j)
-                                    mma(i + j ? d + q.columns : d, further(a, i * kPart + (LAST ? 2 : 128) * k), further(w[j], 2 * k), q.instruction,
-                                        c || k || i + j > 1 || i > 0);
+                                    for (int j = 0; j < PARTS - i; ++j)
+                                        mma(i + j ? d + q.columns : d, further(ak, i * kPart), further(wk, j * lay.slice()), q.instruction,
+                                            c || k || i + j > 1 || i > 0);
+                            }
+                        }
                     mma_commit(empty + 8 * stage);
                     if (++stage == (uint32_t)q.stages) {
                         stage = 0;
@@ -389,7 +351,15 @@ __global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const Spli
                 accumulators16(from, v);
                 if constexpr (PARTS == 3) {
                     float u[16], finite = 0.f;
-                    accumulators16(from + q.columns, u);
+                    if (q.merged) {
+                        float u2[16];
+                        accumulators16(from + q.bn, u);
+                        accumulators16(from + 2 * q.bn, u2);
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) u[j] += u2[j];
+                    } else {
+                        accumulators16(from + q.columns, u);
+                    }
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
                         v[j] += u[j];
@@ -496,8 +466,8 @@ struct WeightSplitLayout {
     __host__ __device__ uint32_t x_part() const { return bytes_of(bn); }
     __host__ __device__ uint32_t stage() const { return (parts * (dz_part() + x_part()) + 1023) / 1024 * 1024; }
     __host__ __device__ uint32_t copies() const { return stages * stage() + 2 * kBlockBytes; }
-    __host__ __device__ int each() const { return ((rows + bn) * 8 + kProducers - 1) / kProducers; }      // vectors of a thread
-    __host__ __device__ uint32_t barriers() const { return copies() + slots * each() * 32 * kProducers; }
+    __host__ __device__ int each() const { return ((rows + bn) * 16 + kProducers - 1) / kProducers; }      // vectors of a thread
+    __host__ __device__ uint32_t barriers() const { return copies() + slots * each() * 16 * kProducers; }
     __host__ __device__ uint32_t bytes() const { return barriers() + (2 * stages + 1) * 8 + 8 + 1024; }
 };
 
@@ -538,43 +508,41 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
     Waiter wait;
 
     if (PARTS == 3 && warp >= kWeightEpilogue && warp < kWeightEpilogue + kGroups * kGroupWarps) {
-        // as in the product's kernel: a thread's own vectors, copied `slots` slices ahead
+        // as in the product's kernel: a thread's own vectors of four, copied `slots` slices ahead, eight of them at a time
         const int t = threadIdx.x - 32 * kWeightEpilogue;
-        const int of_dz = q.rows * 8, total = of_dz + q.bn * 8;
-        const uint32_t slot_bytes = lay.each() * 32 * kProducers;
+        const int of_dz = q.rows * 16, total = of_dz + q.bn * 16;
+        const uint32_t slot_bytes = lay.each() * 16 * kProducers;
         const char *own = smem + lay.copies() + 16 * t;
-        int outer_of[8], chunk_of[8];      // last: pixels and places among the channels of the thread's vectors
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int e = t + kProducers * j, f = e < of_dz ? e : e - of_dz, wide = (e < of_dz ? q.rows : q.bn) / 8;
-            outer_of[j] = (unsigned)f / (unsigned)wide;
-            chunk_of[j] = f - outer_of[j] * wide;
-        }
+        // vector e of an operand of `wide` vectors a row: planes, four pixels of a channel; last, four channels of a pixel
+        struct Spot {
+            bool dz;
+            int outer, in;
+        };
+        auto spot = [&](int e) {
+            Spot v;
+            v.dz = e < of_dz;
+            const int f = v.dz ? e : e - of_dz, wide = LAST ? (v.dz ? q.rows : q.bn) / 4 : 16;
+            v.outer = LAST ? (int)((unsigned)f / (unsigned)wide) : f >> 4;
+            v.in = 4 * (LAST ? f - v.outer * wide : f & 15);
+            return v;
+        };
         auto copy = [&](int slice) {
             if (slice < last) {
                 const int64_t sample = (unsigned)slice / (unsigned)q.slices, p0 = (slice - sample * q.slices) * 64;
                 const int pixels = (int)min((int64_t)64, q.P - p0);
                 const uint32_t to = smem_u32(own) + (q.slots > 1 ? (uint32_t)(slice - first & 1) * slot_bytes : 0);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int e = t + kProducers * j;
-                    if (e >= total) break;
-                    const bool dz = e < of_dz;
-                    const int f = dz ? e : e - of_dz, C = dz ? q.Co : q.Ci, c0 = dz ? o0 : i0;
-                    const float *from = reinterpret_cast<const float *>(dz ? q.dz : q.x);
-                    if (LAST) {      // eight channels of a pixel
-                        const int p = outer_of[j], c = c0 + 8 * chunk_of[j];
-                        copy8<VEC>(to + 8192 * j, 4096, from + (p0 + p) * C + c, p < pixels ? C - c : 0, from);
-                    } else {         // eight pixels of a channel
-                        const int c = c0 + (f >> 3), p = 8 * (f & 7);
-                        copy8<VEC>(to + 8192 * j, 4096, from + (sample * C + c) * q.P + p0 + p, c < C ? pixels - p : 0, from);
-                    }
+                for (int j = 0, e = t; e < total; ++j, e += kProducers) {
+                    const Spot v = spot(e);
+                    const int C = v.dz ? q.Co : q.Ci, c = (v.dz ? o0 : i0) + (LAST ? v.in : v.outer), p = LAST ? v.outer : v.in;
+                    const float *from = reinterpret_cast<const float *>(v.dz ? q.dz : q.x);
+                    copy4<VEC>(to + 4096 * j, from + (LAST ? (p0 + p) * C + c : (sample * C + c) * q.P + p0 + p),
+                               LAST ? (p < pixels ? C - c : 0) : (c < C ? pixels - p : 0), from);
                 }
             }
             copies_commit();
         };
         for (int i = 0; i < q.slots; ++i) copy(first + i);
-        float sum[8] = {};      // planes: of the channel of vector t + 256 j; last: of the channels of every vector of dz
+        float sum[8] = {};      // planes: of the channel of vector t + 256 j; last: of the four channels of every vector of dz
         uint32_t stage = 0, phase = 0;
         for (int slice = first; slice < last; ++slice) {
             copies_wait(q.slots);
@@ -582,23 +550,28 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
             char *const dz_to = smem + stage * lay.stage(), *const x_to = dz_to + PARTS * lay.dz_part();
             const char *from = own + (q.slots > 1 ? (uint32_t)(slice - first & 1) * slot_bytes : 0);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int e = t + kProducers * j;
-                if (e >= total) break;
-                const bool dz = e < of_dz;
-                const int f = dz ? e : e - of_dz, outer = LAST ? outer_of[j] : f >> 3, chunk = LAST ? chunk_of[j] : f & 7;
-                char *to = (dz ? dz_to : x_to) + (LAST ? (chunk >> 3) * kBlockBytes : 0) + outer * 128 + (((chunk & 7) ^ (outer & 7)) << 4);
-                const uint4 v[2] = {*reinterpret_cast<const uint4 *>(from + 8192 * j),
-                                                         *reinterpret_cast<const uint4 *>(from + 8192 * j + 4096)};
-                place8<T>(to, dz ? lay.dz_part() : lay.x_part(), v);
-                if (sums && dz) {
-                    float g[8];
-                    floats8<T>(v, g);
-                    if (LAST) {
+            for (int half = 0; half < 2; ++half) {
+                float4 v[8];
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) sum[i] += g[i];
-                    } else {
-                        sum[j] += ((g[0] + g[1]) + (g[2] + g[3])) + ((g[4] + g[5]) + (g[6] + g[7]));
+                for (int j = 0; j < 8; ++j)
+                    if (t + kProducers * (8 * half + j) < total) v[j] = *reinterpret_cast<const float4 *>(from + 4096 * (8 * half + j));
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int e = t + kProducers * (8 * half + j);
+                    if (e >= total) break;
+                    const Spot w = spot(e);
+                    char *to = (w.dz ? dz_to : x_to) + (LAST ? (w.in >> 6) * kBlockBytes : 0) + w.outer * 128 + ((((w.in >> 3) & 7) ^ (w.outer & 7)) << 4) +
+                               (w.in & 4) * 2;
+                    place4(to, w.dz ? lay.dz_part() : lay.x_part(), v[j]);
+                    if (half == 0 && sums && w.dz) {      // (dz has 2048 vectors at most)
+                        if (LAST) {
+                            sum[0] += v[j].x;
+                            sum[1] += v[j].y;
+                            sum[2] += v[j].z;
+                            sum[3] += v[j].w;
+                        } else {
+                            sum[j] += (v[j].x + v[j].y) + (v[j].z + v[j].w);
+                        }
                     }
                 }
             }
@@ -615,22 +588,23 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
         if (sums) {
             // (rows are a power of two: a thread's vectors of dz are all at one place among the channels, or eight lanes' of a channel)
             if (LAST) {
-                const int wide = q.rows / 8, place = t % wide;
+                const int wide = q.rows / 4, place = t % wide;
                 for (int turn = 0; turn < kProducers / wide; ++turn) {
                     if (t / wide == turn)
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) sums_smem[0][8 * place + i] = turn ? sums_smem[0][8 * place + i] + sum[i] : sum[i];
+                        for (int i = 0; i < 4; ++i) sums_smem[0][4 * place + i] = turn ? sums_smem[0][4 * place + i] + sum[i] : sum[i];
                     asm volatile("bar.sync 1, 256;" ::: "memory");
                 }
             } else {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
+                for (int j = 0; j < 8; ++j) {
                     float g = sum[j];
                     g += __shfl_xor_sync(0xffffffffu, g, 1);
                     g += __shfl_xor_sync(0xffffffffu, g, 2);
                     g += __shfl_xor_sync(0xffffffffu, g, 4);
-                    const int c = (t + kProducers * j) >> 3;
-                    if ((lane & 7) == 0 && c < q.rows) sums_smem[0][c] = g;
+                    g += __shfl_xor_sync(0xffffffffu, g, 8);
+                    const int c = (t + kProducers * j) >> 4;
+                    if ((lane & 15) == 0 && c < q.rows) sums_smem[0][c] = g;
                 }
             }
         }
@@ -645,7 +619,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
             char *const dz_to = smem + stage * lay.stage(), *const x_to = dz_to + PARTS * lay.dz_part();
             bool waited = false;
             for (int v0 = me; v0 < total; v0 += 8 * 128) {
-                uint4 v[8][2];
+                uint4 v[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const int e = v0 + 128 * j;
@@ -655,10 +629,10 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
                     const T *from = dz ? dz_all : x_all;
                     if (LAST) {      // eight channels of a pixel
                         const int p = (unsigned)f / (unsigned)wide, c = c0 + 8 * (f - p * wide);
-                        load8<T, VEC>(from + (p0 + p) * C + c, p < pixels ? C - c : 0, v[j]);
+                        if constexpr (PARTS == 1) v[j] = load8<T, VEC>(from + (p0 + p) * C + c, p < pixels ? C - c : 0);
                     } else {         // eight pixels of a channel
                         const int c = c0 + (f >> 3), p = 8 * (f & 7);
-                        load8<T, VEC>(from + (sample * C + c) * q.P + p0 + p, c < C ? pixels - p : 0, v[j]);
+                        if constexpr (PARTS == 1) v[j] = load8<T, VEC>(from + (sample * C + c) * q.P + p0 + p, c < C ? pixels - p : 0);
                     }
                 }
                 if (!waited) {
@@ -673,10 +647,10 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
                     const int f = dz ? e : e - of_dz, wide = (dz ? q.rows : q.bn) / 8;
                     const int outer = LAST ? (unsigned)f / (unsigned)wide : f >> 3, chunk = LAST ? f - outer * wide : f & 7;
                     char *to = (dz ? dz_to : x_to) + (LAST ? (chunk >> 3) * kBlockBytes : 0) + outer * 128 + (((chunk & 7) ^ (outer & 7)) << 4);
-                    place8<T>(to, dz ? lay.dz_part() : lay.x_part(), v[j]);
+                    *reinterpret_cast<uint4 *>(to) = v[j];
                     if (sums && dz) {
-                        float g[8];
-                        floats8<T>(v[j], g);
+                        float g[8] = {};
+                        if constexpr (PARTS == 1) unpack<T>(v[j], g);
                         if (LAST) {
 #pragma unroll
                             for (int i = 0; i < 8; ++i) sum[i] += g[i];
@@ -800,6 +774,7 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 struct SplitPlan {
     int bn, tiles_n, stages, columns;
+    bool merged;
     int64_t tiles_p;
     unsigned walkers;
     uint32_t smem;
@@ -814,12 +789,14 @@ bool plan_split(const PointwiseShape &s, int K, int Cn, SplitPlan *plan)
     // channels of a tile: what shared memory holds of the weights, and tensor memory of the sums
     const uint32_t others = SplitLayout{16, r.stages, 0, parts, s.last}.bytes() + 8192;
     const int64_t most = std::min<int64_t>(parts == 3 ? 128 : 256, (int64_t)(kMostShared - others) / (parts * chunks * 128) / 16 * 16);
+    if (most < 32 && Cn > most) return false;      // (every tile splits the operand again: multiply-adds are as fast)
     if (most < 16) return false;
     r.tiles_n = (int)ceil_div(Cn, most);
     r.bn = (int)ceil_div(ceil_div(Cn, r.tiles_n), 16) * 16;
     r.tiles_n = (int)ceil_div(Cn, r.bn);
+    r.merged = parts == 3 && 3 * r.bn <= 256;
     r.columns = 32;
-    while (r.columns < r.bn) r.columns *= 2;
+    while (r.columns < (r.merged ? 3 : 1) * r.bn) r.columns *= 2;
     r.smem = SplitLayout{r.bn, r.stages, chunks, parts, s.last}.bytes();
     r.tiles_p = ceil_div(P, 128);
     const int64_t tiles = r.tiles_p * samples;
@@ -839,7 +816,8 @@ int launch_split(const PointwiseShape &s, const SplitPlan &plan, SplitProduct q,
     q.bn = plan.bn;
     q.stages = plan.stages;
     q.columns = plan.columns;
-    q.instruction = mma_instruction(s.io_kind != BC_IO_F16, !s.last, false, plan.bn);
+    q.merged = plan.merged;
+    q.instruction = mma_instruction(s.io_kind != BC_IO_F16, !s.last, false, (plan.merged ? 3 : 1) * plan.bn);
     const int each = 16 / io_size(s.io_kind);
     const bool vec = (s.last ? q.K : q.P) % each == 0 && pointwise_mma_aligned(q.a, nullptr);
     return with_type(s.io_kind, [&](auto t) {
