@@ -65,7 +65,7 @@ enum KernelId {
     KID_FORWARD_PLANE, KID_BACKWARD_PLANE, KID_SUM_CHUNKS, KID_BACKWARD_BAND, KID_INTEGRAL_BANDS, KID_FORWARD_BAND,
     KID_FORWARD_SLAB, KID_BACKWARD_SLAB, KID_FORWARD_QUAD, KID_BACKWARD_QUAD,
     KID_FORWARD_TMEM, KID_FORWARD_TMEM_STREAM, KID_BACKWARD_QUAD_PAIR, KID_BACKWARD_SQUARE, KID_FORWARD_FLAT,
-    KID_POINTWISE, KID_POINTWISE_WEIGHT, KID_POINTWISE_FINISH, KID_POINTWISE_MMA, KID_POINTWISE_WEIGHT_MMA, KID_POINTWISE_SPLIT, KID_POINTWISE_WEIGHT_SPLIT, KID_NORM_FORWARD, KID_NORM_BACKWARD, KID_NORM_FINISH, KID_COUNT
+    KID_POINTWISE, KID_POINTWISE_FINISH, KID_POINTWISE_MMA, KID_POINTWISE_WEIGHT_MMA, KID_POINTWISE_SPLIT, KID_POINTWISE_WEIGHT_SPLIT, KID_NORM_FORWARD, KID_NORM_BACKWARD, KID_NORM_FINISH, KID_COUNT
 };
 
 // Put around a kernel launch: counts it and, while profiling is enabled, records a CUDA event on

@@ -810,7 +810,6 @@ const char *bc_kernel_name(int kernel_id)
         case KID_BACKWARD_SQUARE: return "backward_square_kernel";
         case KID_FORWARD_FLAT: return "forward_flat_kernel";
         case KID_POINTWISE: return "pointwise_kernel";
-        case KID_POINTWISE_WEIGHT: return "pointwise_weight_kernel";
         case KID_POINTWISE_FINISH: return "pointwise_finish_kernel";
         case KID_POINTWISE_MMA: return "pointwise_mma_kernel";
         case KID_POINTWISE_WEIGHT_MMA: return "pointwise_weight_mma_kernel";

@@ -1,12 +1,13 @@
-// Pointwise convolution, out = act(W x + bias + residual) per pixel, and its gradients, with float multiply-adds:
-// every size, layout, alignment and type.
+// Pointwise convolution, out = act(W x + bias + residual) per pixel, and its gradients: which kernels serve a call, those of
+// float multiply-adds for weights that the tensor cores' kernels (pointwise_mma.cu, pointwise_split.cu) do not hold, and the
+// sums that end the weights' gradients.
 //
-// Three products, all of the form  D[m, n] = sum_k A[m, k] B[n, k]  with pixels and channels in turn:
+// The products are of the form  D[m, n] = sum_k A[m, k] B[n, k]  with pixels and channels in turn:
 //   forward      D[p, o] = sum_i x[i, p] W[o, i]           act(D + bias + residual) is stored
 //   slope        the same product; grad * act'(D + bias + residual) = dz is stored
 //   grad_input   D[p, i] = sum_o dz[o, p] W[o, i]
 //   grad_weight  D[o, i] = sum_p dz[o, p] x[i, p]          split over the pixels; partial sums added in order
-// A CTA makes a tile of D from slices of 16 k that pass through shared memory as floats; a thread keeps 8 x 8 (8 x 4)
+// By multiply-adds a CTA makes a tile of D from slices of 16 k that pass through shared memory as floats; a thread keeps 8 x 8 (8 x 4)
 // sums in registers.
 #include "bc_layers.cuh"
 
@@ -239,147 +240,6 @@ __global__ void __launch_bounds__(kThreads, BN == 64 ? 3 : 4) pointwise_kernel(P
     }
 }
 
-struct WeightProduct {
-    const void *dz, *x;
-    float *partial;          // a row a split: Co * Ci sums, then Co sums of dz
-    int N, Ci, Co;           // (N 1, channels last)
-    int64_t P;
-    int tiles_o, tiles_i;
-    int chunk, chunks;       // a piece is `chunk` pixels of a sample, which has `chunks` of them
-    int per;                 // pieces of a split
-    bool sums;               // the sums of dz too
-};
-
-// D's tile: BO x 2048 / BO * 2 weights (32 x 128 or 64 x 64), summed over a split's pixels; 8 x 4 sums a thread, two output
-// channels an instruction.  VEC: rows and arrays allow vectors of four values.
-template <typename T, bool LAST, int BO, bool VEC>
-__global__ void __launch_bounds__(kThreads, 4) pointwise_weight_kernel(WeightProduct q)
-{
-    constexpr int BI = 4096 / BO, NA = BO * kBK / kThreads, NB = BI * kBK / kThreads;
-    __shared__ __align__(16) float As[2][kBK][BO + 4];
-    __shared__ __align__(16) float2 Bs[2][kBK][BI + 2];
-    const int tid = threadIdx.x, tm = tid % (BO / 8), tn = tid / (BO / 8);
-    const int tiles = q.tiles_o * q.tiles_i, split = blockIdx.x / tiles, t = blockIdx.x - split * tiles;
-    const int o0 = t / q.tiles_i * BO, i0 = t % q.tiles_i * BI;
-    const T *dz = static_cast<const T *>(q.dz), *x = static_cast<const T *>(q.x);
-    grid_dependency_wait();
-    f2_t acc[4][4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = both(0.f);
-    float sum = 0.f;
-    const int64_t pieces = (int64_t)q.N * q.chunks, end = min(pieces, (int64_t)(split + 1) * q.per);
-    int64_t piece = (int64_t)split * q.per;
-    int pixels = 0, k0 = 0;
-    const T *a = nullptr, *b = nullptr;
-    auto enter = [&] {      // the piece's first slice
-        const int64_t sample = piece / q.chunks, p0 = (piece - sample * q.chunks) * q.chunk;
-        pixels = (int)min((int64_t)q.chunk, q.P - p0);
-        a = dz + (sample * q.Co * q.P + (LAST ? p0 * q.Co : p0));
-        b = x + (sample * q.Ci * q.P + (LAST ? p0 * q.Ci : p0));
-        k0 = 0;
-    };
-    float ra[NA], rb[NB];
-    // `n` values of one operand: channels c0 + {0 .. B - 1} of C
-    auto fetch = [&](auto size, const T *from, int c0, int C, auto &r) {
-        constexpr int B = decltype(size)::value;
-        if constexpr (VEC) {
-#pragma unroll
-            for (int j = 0; j < B * kBK / kThreads / 4; ++j) {
-                const int e = tid + kThreads * j, k = k0 + (LAST ? e / (B / 4) : 4 * (e & 3)), c = c0 + (LAST ? 4 * (e % (B / 4)) : e >> 2);
-                *reinterpret_cast<float4 *>(&r[4 * j]) =
-                    k < pixels && c < C ? load4(from + (LAST ? (int64_t)k * C + c : c * q.P + k)) : make_float4(0.f, 0.f, 0.f, 0.f);
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < B * kBK / kThreads; ++j) {
-                const int e = tid + kThreads * j, k = k0 + (LAST ? e / B : e & 15), c = c0 + (LAST ? e % B : e >> 4);
-                r[j] = k < pixels && c < C ? to_float(from[LAST ? (int64_t)k * C + c : c * q.P + k]) : 0.f;
-            }
-        }
-    };
-    auto place = [&](auto size, const auto &r, auto &&put) {      // put(k, channel, value)
-        constexpr int B = decltype(size)::value;
-#pragma unroll
-        for (int j = 0; j < B * kBK / kThreads; ++j) {
-            if constexpr (VEC) {
-                const int e = tid + kThreads * (j / 4);
-                put(LAST ? e / (B / 4) : 4 * (e & 3) + j % 4, LAST ? 4 * (e % (B / 4)) + j % 4 : e >> 2, r[j]);
-            } else {
-                const int e = tid + kThreads * j;
-                put(LAST ? e / B : e & 15, LAST ? e % B : e >> 4, r[j]);
-            }
-        }
-    };
-    auto load = [&] {
-        fetch(std::integral_constant<int, BO>(), a, o0, q.Co, ra);
-        fetch(std::integral_constant<int, BI>(), b, i0, q.Ci, rb);
-    };
-    auto store = [&](int s) {
-        place(std::integral_constant<int, BO>(), ra, [&](int k, int c, float v) { As[s][k][c] = v; });
-        place(std::integral_constant<int, BI>(), rb, [&](int k, int c, float v) { Bs[s][k][c] = make_float2(v, v); });
-    };
-    auto advance = [&] {      // to the next slice; false behind the last
-        k0 += kBK;
-        if (k0 < pixels) return true;
-        if (++piece >= end) return false;
-        enter();
-        return true;
-    };
-    if (piece < end) {
-        enter();
-        load();
-        store(0);
-        __syncthreads();
-        for (int s = 0;; s ^= 1) {
-            const bool more = advance();
-            if (more) load();
-#pragma unroll
-            for (int k = 0; k < kBK; ++k) {
-                f2_t av[4], bv[4];
-                ulonglong2 u = *reinterpret_cast<const ulonglong2 *>(&As[s][k][4 * tm]);
-                av[0] = u.x;
-                av[1] = u.y;
-                u = *reinterpret_cast<const ulonglong2 *>(&As[s][k][BO / 2 + 4 * tm]);
-                av[2] = u.x;
-                av[3] = u.y;
-#pragma unroll
-                for (int j = 0; j < 4; j += 2) {
-                    u = *reinterpret_cast<const ulonglong2 *>(&Bs[s][k][4 * tn + j]);
-                    bv[j] = u.x;
-                    bv[j + 1] = u.y;
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[i][j] = fma2(av[i], bv[j], acc[i][j]);
-            }
-            if (q.sums && i0 == 0 && tid < BO) {
-#pragma unroll
-                for (int k = 0; k < kBK; ++k) sum += As[s][k][tid];
-            }
-            if (!more) break;
-            store(s ^ 1);
-            __syncthreads();
-        }
-    }
-    float *partial = q.partial + split * pointwise_partial_stride(q.Co, q.Ci);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int o = o0 + BO / 2 * (i / 2) + 4 * tm + 2 * (i % 2);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            float v[2];
-            unpack2(acc[i][j], v[0], v[1]);
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-                if (o + h < q.Co && i0 + 4 * tn + j < q.Ci) partial[(int64_t)(o + h) * q.Ci + i0 + 4 * tn + j] = v[h];
-        }
-    }
-    if (q.sums && i0 == 0 && tid < BO && o0 + tid < q.Co) partial[(int64_t)q.Co * q.Ci + o0 + tid] = sum;
-}
-
 // Rows of partial sums, added in a fixed order, rounded once: `count` columns, `stride` floats from row to row.
 struct Partials {
     const float *from;
@@ -440,31 +300,10 @@ int launch_product(const PointwiseShape &s, Product q, cudaStream_t stream)
     });
 }
 
-// How grad_weight is cut: tiles, and the pixels in pieces of at most 256, about four CTAs an SM.
-struct Splits {
-    int chunk, chunks, per, splits;
-    int bo, tiles_o, tiles_i;
-};
-Splits splits_of(const PointwiseShape &s)
-{
-    const int64_t P = s.last ? s.N * s.P : s.P, samples = s.last ? 1 : s.N;
-    Splits v;
-    v.bo = s.Co <= 32 ? 32 : 64;
-    v.tiles_o = (int)ceil_div(s.Co, v.bo);
-    v.tiles_i = (int)ceil_div(s.Ci ? s.Ci : 1, 4096 / v.bo);
-    v.chunk = (int)(P < 256 ? P : 256);
-    v.chunks = (int)ceil_div(P, v.chunk);
-    const int64_t pieces = samples * v.chunks, tiles = (int64_t)v.tiles_o * v.tiles_i;
-    const int64_t wanted = tiles > 592 ? 1 : 592 / tiles;
-    v.per = (int)ceil_div(pieces, wanted);
-    v.splits = (int)ceil_div(pieces, v.per);
-    return v;
-}
-
 size_t partial_bytes(const PointwiseShape &s)
 {
     // (whichever kernel's: the query does not know the arrays)
-    return align_up((size_t)std::max({splits_of(s).splits, pointwise_mma_weight_splits(s), pointwise_split_weight_splits(s)}) * pointwise_partial_stride(s.Co, s.Ci) * sizeof(float));
+    return align_up((size_t)std::max(pointwise_mma_weight_splits(s), pointwise_split_weight_splits(s)) * pointwise_partial_stride(s.Co, s.Ci) * sizeof(float));
 }
 // Which kernel a product with pixels in the rows takes.
 enum { BY_TMA, BY_SPLIT, BY_FMA };
@@ -544,32 +383,10 @@ int launch_pointwise_backward(const PointwiseShape &s, const void *x, const void
     if (sums) of_sums = {sums, s.Co, s.Co, rows, grad_bias};
     if (want_weight || !sums) {
         float *partial = static_cast<float *>(take(partial_bytes(s)));
-        int splits = pointwise_mma_weight_splits(s), e;
-        if (splits && pointwise_mma_aligned(dz, x)) {
-            e = launch_pointwise_mma_weight(s, dz, x, partial, want_bias && !sums, stream);
-        } else if ((splits = pointwise_split_weight_splits(s))) {
-            e = launch_pointwise_split_weight(s, dz, x, partial, want_bias && !sums, stream);
-        } else {
-            const Splits v = splits_of(s);
-            splits = v.splits;
-            WeightProduct q{dz, x, partial, s.last ? 1 : s.N, s.Ci, s.Co, s.last ? s.N * s.P : s.P, v.tiles_o, v.tiles_i, v.chunk, v.chunks, v.per,
-                            want_bias && !sums};
-            const int64_t ctas = (int64_t)v.splits * q.tiles_o * q.tiles_i;
-            if (ctas > INT32_MAX) return BC_ERR_BAD_SHAPE;
-            const bool vec = (s.last ? s.Ci % 4 == 0 && s.Co % 4 == 0 : s.P % 4 == 0) && pointwise_mma_aligned(dz, x);
-            e = with_type(s.io_kind, [&](auto t) {
-                using T = decltype(t);
-                auto go = [&](auto last, auto aligned) {
-                    constexpr bool LAST = decltype(last)::value, VEC = decltype(aligned)::value;
-                    const LaunchScope scope(KID_POINTWISE_WEIGHT, stream);
-                    v.bo == 32 ? launch_overlapped(pointwise_weight_kernel<T, LAST, 32, VEC>, (unsigned)ctas, kThreads, 0, stream, q)
-                               : launch_overlapped(pointwise_weight_kernel<T, LAST, 64, VEC>, (unsigned)ctas, kThreads, 0, stream, q);
-                    return check_launch("pointwise_weight_kernel");
-                };
-                if (s.last) return vec ? go(std::true_type(), std::true_type()) : go(std::true_type(), std::false_type());
-                return vec ? go(std::false_type(), std::true_type()) : go(std::false_type(), std::false_type());
-            });
-        }
+        int splits = pointwise_mma_aligned(dz, x) ? pointwise_mma_weight_splits(s) : 0;
+        int e = BC_ERR_BAD_SHAPE;
+        if (splits) e = launch_pointwise_mma_weight(s, dz, x, partial, want_bias && !sums, stream);
+        else if ((splits = pointwise_split_weight_splits(s))) e = launch_pointwise_split_weight(s, dz, x, partial, want_bias && !sums, stream);
         if (e) return e;
         if (want_weight) of_weights = {partial, pointwise_partial_stride(s.Co, s.Ci), weights, splits, grad_weight};
         if (want_bias && !sums) of_sums = {partial + weights, pointwise_partial_stride(s.Co, s.Ci), s.Co, splits, grad_bias};

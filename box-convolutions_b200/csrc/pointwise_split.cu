@@ -878,8 +878,7 @@ struct WeightSplitPlan {
 };
 bool plan_weight_split(const PointwiseShape &s, WeightSplitPlan *plan)
 {
-    if (s.Ci < 1 || s.Co < 1) return false;
-    const int parts = s.io_kind == BC_IO_F32 ? 3 : 1;
+    const int parts = s.io_kind == BC_IO_F32 ? 3 : 1, Ci = std::max(1, s.Ci);      // (no input channels: the sums of dz alone)
     const int64_t P = s.last ? s.N * s.P : s.P, samples = s.last ? 1 : s.N;
     WeightSplitPlan r{};
     r.rows = 16;
@@ -888,9 +887,9 @@ bool plan_weight_split(const PointwiseShape &s, WeightSplitPlan *plan)
     // the widest tile that shared memory holds: 16-bit with a ring of two to four, float with two and one or two slices of copies
     for (int most = parts == 3 ? 128 : 256;; most /= 2) {
         if (most < 32) return false;
-        r.tiles_i = (int)ceil_div(s.Ci, most);
-        r.bn = (int)ceil_div(ceil_div(s.Ci, r.tiles_i), 16) * 16;
-        r.tiles_i = (int)ceil_div(s.Ci, r.bn);
+        r.tiles_i = (int)ceil_div(Ci, most);
+        r.bn = (int)ceil_div(ceil_div(Ci, r.tiles_i), 16) * 16;
+        r.tiles_i = (int)ceil_div(Ci, r.bn);
         auto fits = [&](int stages, int slots) {
             r.stages = stages;
             r.slots = slots;

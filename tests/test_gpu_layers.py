@@ -118,6 +118,8 @@ POINTWISE = [
     (1, 1, 1, 1, 1), (2, 3, 5, 1, 1), (300, 24, 40, 1, 1), (1, 16, 16, 1, 128), (2, 17, 33, 3, 43), (3, 64, 16, 9, 15),
     (2, 32, 128, 16, 24), (1, 128, 32, 40, 50), (2, 60, 20, 31, 37), (2, 65, 129, 11, 13), (1, 256, 256, 16, 16),
     (5, 8, 72, 7, 7), (1, 1, 64, 20, 20), (1, 64, 1, 20, 20), (2, 320, 24, 8, 16), (1, 40, 264, 10, 26), (1, 512, 320, 8, 24),
+    # more tiles than CTAs, aligned and not; more input channels than shared memory holds the weights of
+    (3, 72, 40, 136, 152), (2, 37, 19, 151, 203), (1, 4609, 24, 3, 7), (1, 2304, 40, 4, 10),
 ]
 
 
