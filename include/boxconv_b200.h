@@ -279,7 +279,7 @@ int bc_pointwise_backward(const void *input, const void *weight, const void *bia
 
 /* out = act( weight[c] * (input - mean) / sqrt(var + eps) + bias[c] ): mean and (biased) variance over the pixels of the
  * C / groups adjacent channels of a sample's group; weight and bias (C), each or both NULL for 1 and 0.  stats, which may be
- * NULL, receives 2 * N * groups floats, the mean and 1 / sqrt(var + eps) of every group: the backward pass reads them.
+ * NULL, receives 2 * N * groups floats (8-byte aligned), the mean and 1 / sqrt(var + eps) of every group: the backward pass reads them.
  * out overlaps no input. */
 size_t bc_group_norm_forward_workspace(int io_kind, int N, int C, int64_t pixels, int groups, int channels_last);
 int bc_group_norm_forward(const void *input, const void *weight, const void *bias, void *out, float *stats, int io_kind, int N, int C,
