@@ -2,9 +2,9 @@
 // ones whose rows TMA does not take (odd planes, channels that are no multiple of eight).  The products of pointwise.cu with
 // pixels in the rows, built like pointwise_mma_kernel: persistent CTAs, weights in shared memory, two sets of accumulators.
 //
-// A float is the sum of three bf16 values, its upper, middle and lower eight bits, so a product of floats is that of nine
-// pairs; the six that reach above 2^-24 of it are made: the upper ones into one accumulator, the others into a second, added at
-// the end.  (An accumulator's additions round towards zero: the second stays 2^-8 of the first, and the first sees a
+// A float is the sum of three bf16 values: itself rounded, what is left rounded, and what is left then.  A product of floats is that
+// of nine pairs; the six are made that reach above 2^-26 of it: the upper ones into one accumulator, the others into a second or a
+// third, added at the end.  (An accumulator's additions round towards zero: the others stay 2^-8 of the first, which sees a
 // sixth of the additions.)  Measured against multiply-adds, which wait for shared memory here ((16,128->32,64,128) planes: 38 us).
 // Infinities and NaN have no such sum: a result that is not finite is computed again by multiply-adds.
 #include "bc_mma.cuh"
@@ -60,8 +60,10 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t (&part)[3])
     for (int p = 0; p < 3; ++p) {
         float lo, hi;
         unpack2(x, lo, hi);
-        part[p] = __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632);
-        if (p < 2) x = sub2(x, pack2(__uint_as_float(__float_as_uint(lo) & 0xffff0000u), __uint_as_float(__float_as_uint(hi) & 0xffff0000u)));
+        part[p] = narrow2(lo, hi, __nv_bfloat16());
+        if (p == 2) break;
+        widen2(part[p], lo, hi, __nv_bfloat16());
+        x = sub2(x, pack2(lo, hi));
     }
 }
 // Into their place of every part, `part` bytes apart.
