@@ -143,6 +143,42 @@ __global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const Spli
     for (int i = threadIdx.x; i < q.bn; i += kThreads)
         bias_smem[i] = MODE != INPUT && q.bias && n0 + i < q.Cn ? to_float(static_cast<const T *>(q.bias)[n0 + i]) : 0.f;
     for (int i = threadIdx.x; i < 4 * q.bn; i += kThreads) sums_smem[i] = 0.f;
+    // A producer's way through this CTA's slices.
+    struct Cursor {
+        unsigned tile;
+        int c;
+    };
+    auto advance = [&](Cursor &at) {
+        if (++at.c == chunks) {
+            at.c = 0;
+            at.tile += walkers;
+        }
+    };
+    // Producers of floats: a thread has eight vectors of four floats of a slice, copies them to a place of its own and splits them
+    // from there, the next slice's on their way.
+    const int t = (int)threadIdx.x - 32 * kEpilogue;
+    const float *all = reinterpret_cast<const float *>(q.a);
+    const char *own = smem + lay.copies() + 16 * t;
+    // planes: four pixels of a k; last: four k of a pixel
+    const int in = 4 * (LAST ? t & 15 : t & 31), outer0 = LAST ? t >> 4 : t >> 5, outer_step = LAST ? kProducers / 16 : kProducers / 32;
+    const int64_t pitch = LAST ? (int64_t)q.K : q.P;
+    Cursor ahead{walker, 0};
+    auto copy = [&] {
+        if (ahead.tile < tiles) {
+            const unsigned sample = ahead.tile / (unsigned)q.tiles_p;
+            const int64_t p0 = (int64_t)(ahead.tile - sample * q.tiles_p) * 128;
+            const int pixels = (int)min((int64_t)128, q.P - p0), k_left = q.K - 64 * ahead.c;
+            const float *a = all + (LAST ? p0 * q.K + 64 * ahead.c : ((int64_t)sample * q.K + 64 * ahead.c) * q.P + p0) + outer0 * pitch + in;
+            const int inner = (LAST ? k_left : pixels) - in, outers = (LAST ? pixels : k_left) - outer0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                copy4<VEC>(smem_u32(own) + 4096 * j, a + j * outer_step * pitch, j * outer_step < outers ? inner : 0, all);
+            advance(ahead);
+        }
+        copies_commit();
+    };
+    const bool produces = warp >= kEpilogue && warp < kEpilogue + kGroups * kGroupWarps;
+    if (PARTS == 3 && produces) copy();      // (the first slice is on its way while the weights are placed)
     // the weights, K-major, eight k a thread
     {
         for (int e = threadIdx.x; e < q.bn * chunks * 8; e += kThreads) {
@@ -173,42 +209,7 @@ __global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const Spli
     const uint32_t tmem = *tmem_slot;
     Waiter wait;
 
-    // A producer's way through this CTA's slices.
-    struct Cursor {
-        unsigned tile;
-        int c;
-    };
-    auto advance = [&](Cursor &at) {
-        if (++at.c == chunks) {
-            at.c = 0;
-            at.tile += walkers;
-        }
-    };
-    if (PARTS == 3 && warp >= kEpilogue && warp < kEpilogue + kGroups * kGroupWarps) {
-        // A thread has eight vectors of four floats of a slice: it copies them to a place of its own and splits them from
-        // there, the next slice's on their way.
-        const int t = threadIdx.x - 32 * kEpilogue;
-        const float *all = reinterpret_cast<const float *>(q.a);
-        const char *own = smem + lay.copies() + 16 * t;
-        // planes: four pixels of a k; last: four k of a pixel
-        const int in = 4 * (LAST ? t & 15 : t & 31), outer0 = LAST ? t >> 4 : t >> 5, outer_step = LAST ? kProducers / 16 : kProducers / 32;
-        const int64_t pitch = LAST ? (int64_t)q.K : q.P;
-        Cursor ahead{walker, 0};
-        auto copy = [&] {
-            if (ahead.tile < tiles) {
-                const unsigned sample = ahead.tile / (unsigned)q.tiles_p;
-                const int64_t p0 = (int64_t)(ahead.tile - sample * q.tiles_p) * 128;
-                const int pixels = (int)min((int64_t)128, q.P - p0), k_left = q.K - 64 * ahead.c;
-                const float *a = all + (LAST ? p0 * q.K + 64 * ahead.c : ((int64_t)sample * q.K + 64 * ahead.c) * q.P + p0) + outer0 * pitch + in;
-                const int inner = (LAST ? k_left : pixels) - in, outers = (LAST ? pixels : k_left) - outer0;
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    copy4<VEC>(smem_u32(own) + 4096 * j, a + j * outer_step * pitch, j * outer_step < outers ? inner : 0, all);
-                advance(ahead);
-            }
-            copies_commit();
-        };
-        copy();
+    if (PARTS == 3 && produces) {
         uint32_t stage = 0, phase = 0;
         for (Cursor at{walker, 0}; at.tile < tiles; advance(at)) {
             copies_wait(1);
