@@ -4,7 +4,7 @@
 // channels.  The weights stay in shared memory; persistent CTAs walk over the pixels.  One thread brings slices of 64 k by
 // TMA into a ring, one issues tcgen05.mma into one of two sets of accumulators in tensor memory, eight warps take the other set
 // out.  Planes are an MN-major operand and channels last a K-major one: no transposition in either.
-// A warp of the epilogue passes 32 x 32 sums through shared memory (rows of 33 words: no bank conflicts), so that it reads
+// A warp of the epilogue passes 32 x 32 sums through shared memory, so that it reads
 // residuals and gradients and writes results 16 bytes a lane, 64 bytes in a row, along whichever index runs in memory.  Where a
 // CTA has its SM to itself, the next block's are on their way while a block is dealt with.
 //
@@ -17,7 +17,7 @@ namespace {
 
 enum { FORWARD, SLOPE, INPUT };
 constexpr int kEpilogue = 8;      // warps of the epilogue, or pairs of them
-constexpr int kPitch = 33;
+constexpr int kPitch = 33, kPitchLast = 36;      // words: columns, or vectors of rows, without bank conflicts
 constexpr uint32_t kStage = 16384;      // 128 pixels x 64 k
 constexpr size_t kMostShared = 227 << 10;
 
@@ -41,7 +41,7 @@ struct MmaLayout {
     __host__ __device__ uint32_t slice() const { return input ? (uint32_t)((bn + 63) / 64) * kBlockBytes : (uint32_t)bn * 128; }
     __host__ __device__ uint32_t ring() const { return (chunks * slice() + 1023) / 1024 * 1024; }
     __host__ __device__ uint32_t staging() const { return ring() + stages * kStage; }
-    __host__ __device__ uint32_t bias() const { return staging() + kEpilogue * 32 * kPitch * 4; }
+    __host__ __device__ uint32_t bias() const { return staging() + kEpilogue * 32 * kPitchLast * 4; }
     __host__ __device__ uint32_t sums() const { return bias() + bn * 4; }
     __host__ __device__ uint32_t barriers() const { return (sums() + 4 * pair * bn * 4 + 7) / 8 * 8; }
     __host__ __device__ uint32_t bytes() const { return barriers() + (2 * stages + 5) * 8 + 8 + 1024; }
@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(32 * (kEpilogue * PAIR + 2), PAIR == 1 ? 2 : 1
         }
     } else {
         const int quarter = warp & 3, member = PAIR == 2 ? warp >> 2 & 1 : 0, half = warp / (4 * PAIR), blocks = (q.bn + 31) / 32;
-        float *staging = reinterpret_cast<float *>(smem + lay.staging()) + (4 * half + quarter) * 32 * kPitch;
+        float *staging = reinterpret_cast<float *>(smem + lay.staging()) + (4 * half + quarter) * 32 * kPitchLast;
         auto together = [&] {      // whoever shares the staging rows
             if (PAIR == 2) asm volatile("bar.sync %0, 64;" ::"r"(1 + 4 * half + quarter) : "memory");
             else __syncwarp();
@@ -191,7 +191,10 @@ __global__ void __launch_bounds__(32 * (kEpilogue * PAIR + 2), PAIR == 1 ? 2 : 1
                     float v[16];
                     accumulators16(tmem + set * q.columns + 32 * b + 16 * part + ((uint32_t)quarter << 21), v);
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) staging[lane * kPitch + 16 * part + j] = v[j];
+                    for (int j = 0; j < 16; j += LAST ? 4 : 1) {
+                        if (LAST) *reinterpret_cast<float4 *>(staging + lane * kPitchLast + 16 * part + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+                        else staging[lane * kPitch + 16 * part + j] = v[j];
+                    }
                 }
                 together();
                 float total[8] = {};
@@ -200,15 +203,25 @@ __global__ void __launch_bounds__(32 * (kEpilogue * PAIR + 2), PAIR == 1 ? 2 : 1
                     const int row = 8 * i + outer;
                     const bool there = now.there >> i & 1;
                     f2_t z[4];
+                    // four pairs, of a row or of a column
+                    auto pairs = [](const float *from, int pitch, f2_t (&v)[4]) {
+                        if (LAST) {
+                            const ulonglong2 lo = *reinterpret_cast<const ulonglong2 *>(from), hi = *reinterpret_cast<const ulonglong2 *>(from + 4);
+                            v[0] = lo.x;
+                            v[1] = lo.y;
+                            v[2] = hi.x;
+                            v[3] = hi.y;
+                        } else {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float *from = LAST ? staging + row * kPitch + inner + 2 * j : staging + (inner + 2 * j) * kPitch + row;
-                        z[j] = pack2(from[0], from[LAST ? 1 : kPitch]);
-                    }
+                            for (int j = 0; j < 4; ++j) v[j] = pack2(from[2 * j * pitch], from[(2 * j + 1) * pitch]);
+                        }
+                    };
+                    pairs(LAST ? staging + row * kPitchLast + inner : staging + inner * kPitch + row, kPitch, z);
                     if (MODE != INPUT && there) {
-                        const float *bias = bias_smem + 32 * b + (LAST ? inner : row);
+                        f2_t bias[4];
+                        pairs(bias_smem + 32 * b + (LAST ? inner : row), 0, bias);
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) z[j] = add2(z[j], pack2(bias[LAST ? 2 * j : 0], bias[LAST ? 2 * j + 1 : 0]));
+                        for (int j = 0; j < 4; ++j) z[j] = add2(z[j], bias[j]);
                         if (residual) {
                             f2_t r[4];
                             unpack_pairs<T>(now.res[i], r);
@@ -479,11 +492,15 @@ bool plan_product(const PointwiseShape &s, int K, int Cn, bool input, Plan *plan
     const int64_t tiles = r.tiles_p * samples;
     if (tiles > INT32_MAX || P > INT32_MAX - 256 || P * std::max(s.Ci, s.Co) >= (int64_t)1 << 38) return false;      // (coordinates, strides)
     // two CTAs an SM where both find room, or one with pairs of warps
-    r.stages = 4;
+    // ((32,32->128,64,128) f16 last with residual: 47 us alone with a ring of four, 43 with two CTAs and rings of three)
     r.per_sm = 2;
-    r.smem = MmaLayout{r.bn, r.stages, chunks, 1, input}.bytes();
-    if (r.columns > 128 || 2 * (r.smem + 1024) > 228 << 10) {
+    for (r.stages = 4; r.stages > 2; --r.stages) {
+        r.smem = MmaLayout{r.bn, r.stages, chunks, 1, input}.bytes();
+        if (2 * (r.smem + 1024) <= 228 << 10) break;
+    }
+    if (r.columns > 128 || r.stages == 2) {
         r.per_sm = 1;
+        r.stages = 4;
         while ((r.smem = MmaLayout{r.bn, r.stages, chunks, 2, input}.bytes()) > kMostShared)
             if (--r.stages < 2) return false;
     }
