@@ -475,10 +475,11 @@ struct Plan {
     unsigned walkers;
     uint32_t smem;
 };
-bool plan_product(const PointwiseShape &s, int K, int Cn, bool input, Plan *plan)
+bool plan_product(const PointwiseShape &s, int K, int Cn, int mode, Plan *plan)
 {
     const int samples = s.last ? 1 : s.N, chunks = (int)ceil_div(K, 64);
     const int64_t P = s.last ? s.N * s.P : s.P;
+    const bool input = mode == INPUT;
     Plan r{};
     // channels of a tile: all of them up to 256, with weights of at most 128 KB
     const int64_t most = std::min<int64_t>(256, (int64_t)(128 << 10) / (chunks * 128) / 16 * 16);
@@ -492,13 +493,14 @@ bool plan_product(const PointwiseShape &s, int K, int Cn, bool input, Plan *plan
     const int64_t tiles = r.tiles_p * samples;
     if (tiles > INT32_MAX || P > INT32_MAX - 256 || P * std::max(s.Ci, s.Co) >= (int64_t)1 << 38) return false;      // (coordinates, strides)
     // two CTAs an SM where both find room, or one with pairs of warps
-    // ((32,32->128,64,128) f16 last with residual: 47 us alone with a ring of four, 43 with two CTAs and rings of three)
+    // ((32,32->128,64,128) f16 last with residual: 47 us alone with a ring of four, 43 with two CTAs and rings of three).  The
+    // slope's epilogue does not fit the registers of two: alone ((32,128->64,64,128) bf16 last, SiLU: 43 us, 47 with two).
     r.per_sm = 2;
     for (r.stages = 4; r.stages > 2; --r.stages) {
         r.smem = MmaLayout{r.bn, r.stages, chunks, 1, input}.bytes();
         if (2 * (r.smem + 1024) <= 228 << 10) break;
     }
-    if (r.columns > 128 || r.stages == 2) {
+    if (r.columns > 128 || r.stages == 2 || mode == SLOPE) {
         r.per_sm = 1;
         r.stages = 4;
         while ((r.smem = MmaLayout{r.bn, r.stages, chunks, 2, input}.bytes()) > kMostShared)
@@ -545,7 +547,9 @@ int launch_mma(const PointwiseShape &s, const Plan &plan, MmaProduct q, const vo
             return s.last ? go(pointwise_mma_kernel<T, MODE, ACT, true, PAIR>) : go(pointwise_mma_kernel<T, MODE, ACT, false, PAIR>);
         };
         auto run = [&](auto pair) { return bf16 ? of_type(__nv_bfloat16(), pair) : of_type(__half(), pair); };
-        return plan.per_sm == 1 ? run(std::integral_constant<int, 2>()) : run(std::integral_constant<int, 1>());
+        if constexpr (MODE != SLOPE)
+            if (plan.per_sm == 2) return run(std::integral_constant<int, 1>());
+        return run(std::integral_constant<int, 2>());
     });
 }
 
@@ -562,7 +566,7 @@ bool rows_aligned(const PointwiseShape &s)
 bool pointwise_mma_suits(const PointwiseShape &s, bool input)
 {
     Plan plan;
-    return rows_aligned(s) && plan_product(s, input ? s.Co : s.Ci, input ? s.Ci : s.Co, input, &plan);
+    return rows_aligned(s) && plan_product(s, input ? s.Co : s.Ci, input ? s.Ci : s.Co, input ? INPUT : SLOPE, &plan);
 }
 bool pointwise_mma_aligned(const void *a, const void *b, const void *c, const void *d, const void *e)
 {
@@ -571,13 +575,13 @@ bool pointwise_mma_aligned(const void *a, const void *b, const void *c, const vo
 int pointwise_mma_sums_rows(const PointwiseShape &s)
 {
     Plan plan;
-    return plan_product(s, s.Ci, s.Co, false, &plan) ? (int)plan.walkers : 0;
+    return plan_product(s, s.Ci, s.Co, SLOPE, &plan) ? (int)plan.walkers : 0;
 }
 int launch_pointwise_mma_forward(const PointwiseShape &s, const void *x, const void *weight, const void *bias, const void *residual, void *out,
                                  cudaStream_t stream)
 {
     Plan plan;
-    plan_product(s, s.Ci, s.Co, false, &plan);
+    plan_product(s, s.Ci, s.Co, FORWARD, &plan);
     MmaProduct q{};
     q.bias = bias;
     q.residual = residual;
@@ -590,7 +594,7 @@ int launch_pointwise_mma_slope(const PointwiseShape &s, const void *x, const voi
                                const void *grad, void *dz, float *sums, cudaStream_t stream)
 {
     Plan plan;
-    plan_product(s, s.Ci, s.Co, false, &plan);
+    plan_product(s, s.Ci, s.Co, SLOPE, &plan);
     MmaProduct q{};
     q.bias = bias;
     q.residual = residual;
@@ -604,7 +608,7 @@ int launch_pointwise_mma_slope(const PointwiseShape &s, const void *x, const voi
 int launch_pointwise_mma_input(const PointwiseShape &s, const void *dz, const void *weight, void *grad_input, cudaStream_t stream)
 {
     Plan plan;
-    plan_product(s, s.Co, s.Ci, true, &plan);
+    plan_product(s, s.Co, s.Ci, INPUT, &plan);
     MmaProduct q{};
     q.out = grad_input;
     q.K = s.Co;
