@@ -539,7 +539,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
                     const int C = v.dz ? q.Co : q.Ci, c = (v.dz ? o0 : i0) + (LAST ? v.in : v.outer), p = LAST ? v.outer : v.in;
                     const float *from = reinterpret_cast<const float *>(v.dz ? q.dz : q.x);
                     copy4<VEC>(to + 4096 * j, from + (LAST ? (p0 + p) * C + c : (sample * C + c) * q.P + p0 + p),
-                               LAST ? (p < pixels ? C - c : 0) : (c < C ? pixels - p : 0), from);
+                               LAST ? (p < pixels ? C - c : 0) : (c < C ? pixels - p : 0), reinterpret_cast<const float *>(q.dz));
                 }
             }
             copies_commit();

@@ -437,12 +437,14 @@ def test_same_bits_from_call_to_call_and_on_another_stream(bc):
                 assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(first, second, third)), name
 
 
-def test_two_captured_steps_replayed_at_once(bc):
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_two_captured_steps_replayed_at_once(bc, dtype):
     """Graphs of whole steps, gradients included, on two streams: each has workspaces of its own and computes on new data."""
     for name, f, params in _calls(bc):
         graphs = []
+        params = [p.to(dtype) for p in params]
         for k in range(2):
-            x, g = torch.randn(2, 24, 40, 48, device="cuda"), torch.randn(2, 40, 40, 48, device="cuda")
+            x, g = torch.randn(2, 24, 40, 48, device="cuda").to(dtype), torch.randn(2, 40, 40, 48, device="cuda").to(dtype)
             side = torch.cuda.Stream()
             side.wait_stream(torch.cuda.current_stream())
             with torch.cuda.stream(side):
