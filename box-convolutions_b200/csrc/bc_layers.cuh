@@ -90,6 +90,27 @@ __device__ __forceinline__ uint4 pack_pairs(const f2_t (&v)[kVec<T> / 2])
 }
 __device__ __forceinline__ f2_t both(float v) { return pack2(v, v); }
 
+// What a rounding to 16 bits leaves of a value; of one whose rounding is not finite, nothing.
+template <typename T>
+__device__ __forceinline__ float left_by_rounding(float v, T rounded)
+{
+    const float left = v - to_float(rounded);
+    return fabsf(left) < INFINITY ? left : 0.f;
+}
+template <typename T>
+__device__ __forceinline__ uint4 left_by_rounding(const f2_t (&v)[kVec<T> / 2], const uint4 &rounded)
+{
+    f2_t r[kVec<T> / 2];
+    unpack_pairs<T>(rounded, r);
+#pragma unroll
+    for (int j = 0; j < kVec<T> / 2; ++j) {
+        float a, b;
+        unpack2(sub2(v[j], r[j]), a, b);
+        r[j] = pack2(fabsf(a) < INFINITY ? a : 0.f, fabsf(b) < INFINITY ? b : 0.f);
+    }
+    return pack_pairs<T>(r);
+}
+
 // ---- activations (BC_ACT_*), of two values at a time.  A NaN stays one in all of them; the ReLU's slope at zero and at NaN
 // is 0, as PyTorch's.  Exponentials and quotients are the hardware's powers of two and reciprocals (2^-22 and 2^-23): with
 // CUDA's own functions a normalisation of float planes with SiLU was bound by instructions, (256,32,64,128) forward 148 us.
@@ -258,6 +279,7 @@ struct PointwiseShape {
     bool last;
     int io_kind, act;
 };
+// A 16-bit dz = grad * slope is two tensors, its rounding and `rest`, the rounding of what that leaves (null: one tensor is all of dz).
 // The products on the tensor cores (pointwise_mma.cu): 16-bit types, rows and arrays on 16 bytes.
 bool pointwise_mma_suits(const PointwiseShape &s, bool input);
 bool pointwise_mma_aligned(const void *a, const void *b, const void *c = nullptr, const void *d = nullptr, const void *e = nullptr);
@@ -266,13 +288,15 @@ int launch_pointwise_mma_forward(const PointwiseShape &s, const void *x, const v
 // sums: pointwise_mma_sums_rows() rows of Co floats, sums of dz to be added, or null
 int pointwise_mma_sums_rows(const PointwiseShape &s);
 int launch_pointwise_mma_slope(const PointwiseShape &s, const void *x, const void *weight, const void *bias, const void *residual,
-                               const void *grad, void *dz, float *sums, cudaStream_t stream);
-int launch_pointwise_mma_input(const PointwiseShape &s, const void *dz, const void *weight, void *grad_input, cudaStream_t stream);
+                               const void *grad, void *dz, void *rest, float *sums, cudaStream_t stream);
+int launch_pointwise_mma_input(const PointwiseShape &s, const void *dz, const void *rest, const void *weight, void *grad_input,
+                               cudaStream_t stream);
 // Floats of a row of partial sums of grad_weight, Co * Ci and the Co of grad_bias: whole vectors, so that every row starts on one.
 __host__ __device__ inline int64_t pointwise_partial_stride(int Co, int Ci) { return ((int64_t)Co * Ci + Co + 3) / 4 * 4; }
 // rows of partial sums (0: not for this kernel)
 int pointwise_mma_weight_splits(const PointwiseShape &s);
-int launch_pointwise_mma_weight(const PointwiseShape &s, const void *dz, const void *x, float *partial, bool sums, cudaStream_t stream);
+int launch_pointwise_mma_weight(const PointwiseShape &s, const void *dz, const void *rest, const void *x, float *partial, bool sums,
+                                cudaStream_t stream);
 int read_wait_timeouts_mma(int *count);
 
 // The same with operands made by threads (pointwise_split.cu): floats as sums of bf16, rows of any alignment.
@@ -281,10 +305,12 @@ int pointwise_split_sums_rows(const PointwiseShape &s);
 int launch_pointwise_split_forward(const PointwiseShape &s, const void *x, const void *weight, const void *bias, const void *residual,
                                    void *out, cudaStream_t stream);
 int launch_pointwise_split_slope(const PointwiseShape &s, const void *x, const void *weight, const void *bias, const void *residual,
-                                 const void *grad, void *dz, float *sums, cudaStream_t stream);
-int launch_pointwise_split_input(const PointwiseShape &s, const void *dz, const void *weight, void *grad_input, cudaStream_t stream);
-int pointwise_split_weight_splits(const PointwiseShape &s);
-int launch_pointwise_split_weight(const PointwiseShape &s, const void *dz, const void *x, float *partial, bool sums, cudaStream_t stream);
+                                 const void *grad, void *dz, void *rest, float *sums, cudaStream_t stream);
+int launch_pointwise_split_input(const PointwiseShape &s, const void *dz, const void *rest, const void *weight, void *grad_input,
+                                 cudaStream_t stream);
+int pointwise_split_weight_splits(const PointwiseShape &s, bool rest);      // (no more with `rest` than without)
+int launch_pointwise_split_weight(const PointwiseShape &s, const void *dz, const void *rest, const void *x, float *partial, bool sums,
+                                  cudaStream_t stream);
 int read_wait_timeouts_split(int *count);
 
 size_t pointwise_workspace(const PointwiseShape &s, int need_mask);

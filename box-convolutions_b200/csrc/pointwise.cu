@@ -21,6 +21,7 @@ constexpr int kThreads = 128, kBM = 128, kBK = 16;
 struct Product {
     const void *a, *w, *bias, *residual, *grad;
     void *out;
+    void *rest;              // INPUT: null, or what `a` lacks of dz; SLOPE: where that goes, or null
     int K, Cn;               // channels of A and of the output
     int wn, wk;              // strides of W along them
     int64_t P;               // pixels of a sample (of all of them together, channels last)
@@ -69,6 +70,12 @@ __device__ __forceinline__ void finish4(const Product &q, int64_t at, float (&z)
         }
     }
     store4<T>(out, z);
+    if (MODE == SLOPE && q.rest) {
+        float left[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) left[i] = left_by_rounding(z[i], from_float<T>(z[i]));
+        store4<T>(static_cast<T *>(q.rest) + at, left);
+    }
 }
 
 // D's tile: kBM pixels of a sample x BN channels.  VEC: rows and arrays allow vectors of four values; a thread's pixels are
@@ -88,6 +95,7 @@ __global__ void __launch_bounds__(kThreads, BN == 64 ? 3 : 4) pointwise_kernel(P
     const int pixels = (int)min((int64_t)kBM, q.P - p0);
     const T *a = static_cast<const T *>(q.a) + sample * q.K * q.P + (LAST ? p0 * q.K : p0);
     const T *w = static_cast<const T *>(q.w);
+    const T *a_rest = MODE == INPUT && q.rest ? static_cast<const T *>(q.rest) + (a - static_cast<const T *>(q.a)) : nullptr;
     grid_dependency_wait();
 
     float ra[16], rb[BN / 8];
@@ -96,14 +104,21 @@ __global__ void __launch_bounds__(kThreads, BN == 64 ? 3 : 4) pointwise_kernel(P
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const int e = tid + kThreads * j, k = k0 + (LAST ? 4 * (e & 3) : e >> 5), m = LAST ? e >> 2 : 4 * (e & 31);
-                *reinterpret_cast<float4 *>(ra + 4 * j) =
-                    k < q.K && m < pixels ? load4(a + (LAST ? (int64_t)m * q.K + k : k * q.P + m)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                const int64_t at = LAST ? (int64_t)m * q.K + k : k * q.P + m;
+                const bool there = k < q.K && m < pixels;
+                float4 v = there ? load4(a + at) : make_float4(0.f, 0.f, 0.f, 0.f);
+                if (MODE == INPUT && a_rest && there) {
+                    const float4 u = load4(a_rest + at);
+                    v = make_float4(v.x + u.x, v.y + u.y, v.z + u.z, v.w + u.w);
+                }
+                *reinterpret_cast<float4 *>(ra + 4 * j) = v;
             }
         } else {
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
                 const int k = k0 + (LAST ? tid & 15 : j), m = LAST ? (tid >> 4) + 8 * j : tid;
-                ra[j] = k < q.K && m < pixels ? to_float(a[LAST ? (int64_t)m * q.K + k : k * q.P + m]) : 0.f;
+                const int64_t at = LAST ? (int64_t)m * q.K + k : k * q.P + m;
+                ra[j] = k < q.K && m < pixels ? to_float(a[at]) + (MODE == INPUT && a_rest ? to_float(a_rest[at]) : 0.f) : 0.f;
             }
         }
 #pragma unroll
@@ -232,7 +247,10 @@ __global__ void __launch_bounds__(kThreads, BN == 64 ? 3 : 4) pointwise_kernel(P
                         const int64_t at = base + (LAST ? (int64_t)m * q.Cn + n + j : (n + j) * q.P + m);
                         float v = z[h] + b4[j];
                         if (MODE != INPUT && residual) v += to_float(residual[at]);
-                        out[at] = from_float<T>(MODE == FORWARD ? activate<ACT, T>(v) : MODE == SLOPE ? times_slope<ACT, T>(to_float(grad[at]), v) : v);
+                        v = MODE == FORWARD ? activate<ACT, T>(v) : MODE == SLOPE ? times_slope<ACT, T>(to_float(grad[at]), v) : v;
+                        const T rounded = from_float<T>(v);
+                        out[at] = rounded;
+                        if (MODE == SLOPE && q.rest) static_cast<T *>(q.rest)[at] = from_float<T>(left_by_rounding(v, rounded));
                     }
                 }
             }
@@ -303,7 +321,7 @@ int launch_product(const PointwiseShape &s, Product q, cudaStream_t stream)
 size_t partial_bytes(const PointwiseShape &s)
 {
     // (whichever kernel's: the query does not know the arrays)
-    return align_up((size_t)std::max(pointwise_mma_weight_splits(s), pointwise_split_weight_splits(s)) * pointwise_partial_stride(s.Co, s.Ci) * sizeof(float));
+    return align_up((size_t)std::max(pointwise_mma_weight_splits(s), pointwise_split_weight_splits(s, false)) * pointwise_partial_stride(s.Co, s.Ci) * sizeof(float));
 }
 // Which kernel a product with pixels in the rows takes.
 enum { BY_TMA, BY_SPLIT, BY_FMA };
@@ -323,6 +341,14 @@ size_t sums_bytes(const PointwiseShape &s)
 }
 // dz in memory, where it is neither grad_output itself nor asked for.
 bool own_dz(const PointwiseShape &s, int need_mask) { return s.act != BC_ACT_NONE && !(need_mask & BC_NEED_PW_RESIDUAL); }
+// A 16-bit dz goes into its products as its rounding (grad_residual) and what that leaves, rounded: off by u^2 of it.  With
+// the rounding alone grad_input and grad_weight were 1.4 times as far from their definition as one rounding puts them; a step of
+// (64,256->256,64,128) bf16 last with GELU took 706 us, and takes 864.
+bool keeps_rest(const PointwiseShape &s, int need_mask)
+{
+    return s.act != BC_ACT_NONE && s.io_kind != BC_IO_F32 && (need_mask & (BC_NEED_PW_INPUT | BC_NEED_PW_WEIGHT | BC_NEED_PW_BIAS));
+}
+size_t dz_bytes(const PointwiseShape &s) { return align_up((size_t)io_size(s.io_kind) * s.N * s.Co * s.P); }
 
 }  // namespace
 
@@ -332,12 +358,12 @@ int launch_pointwise_forward(const PointwiseShape &s, const void *x, const void 
     const int way = way_of(s, false, pointwise_mma_aligned(x, weight, residual, out));
     if (way == BY_TMA) return launch_pointwise_mma_forward(s, x, weight, bias, residual, out, stream);
     if (way == BY_SPLIT) return launch_pointwise_split_forward(s, x, weight, bias, residual, out, stream);
-    return launch_product<FORWARD>(s, {x, weight, bias, residual, nullptr, out, s.Ci, s.Co, s.Ci, 1}, stream);
+    return launch_product<FORWARD>(s, {x, weight, bias, residual, nullptr, out, nullptr, s.Ci, s.Co, s.Ci, 1}, stream);
 }
 
 size_t pointwise_workspace(const PointwiseShape &s, int need_mask)
 {
-    size_t bytes = own_dz(s, need_mask) ? align_up((size_t)io_size(s.io_kind) * s.N * s.Co * s.P) : 0;
+    size_t bytes = ((own_dz(s, need_mask) ? 1 : 0) + (keeps_rest(s, need_mask) ? 1 : 0)) * dz_bytes(s);
     if (need_mask & (BC_NEED_PW_WEIGHT | BC_NEED_PW_BIAS)) bytes += partial_bytes(s);
     if ((need_mask & BC_NEED_PW_BIAS) && s.act != BC_ACT_NONE) bytes += sums_bytes(s);
     return bytes;
@@ -355,26 +381,28 @@ int launch_pointwise_backward(const PointwiseShape &s, const void *x, const void
     };
     const bool want_weight = need_mask & BC_NEED_PW_WEIGHT, want_bias = need_mask & BC_NEED_PW_BIAS;
     const void *dz = grad;
+    void *rest = nullptr;
     float *sums = nullptr;      // rows of sums of dz as it was before its rounding
     int rows = 0;
     if (s.act != BC_ACT_NONE) {
-        void *to = own_dz(s, need_mask) ? take(align_up((size_t)io_size(s.io_kind) * s.N * s.Co * s.P)) : grad_residual;
+        void *to = own_dz(s, need_mask) ? take(dz_bytes(s)) : grad_residual;
+        if (keeps_rest(s, need_mask)) rest = take(dz_bytes(s));
         const int way = way_of(s, false, pointwise_mma_aligned(x, weight, residual, grad, to));
         if (want_bias && way != BY_FMA) {
             sums = static_cast<float *>(take(sums_bytes(s)));
             rows = sums_rows(s, way);
         }
-        const int e = way == BY_TMA     ? launch_pointwise_mma_slope(s, x, weight, bias, residual, grad, to, sums, stream)
-                      : way == BY_SPLIT ? launch_pointwise_split_slope(s, x, weight, bias, residual, grad, to, sums, stream)
-                                        : launch_product<SLOPE>(s, {x, weight, bias, residual, grad, to, s.Ci, s.Co, s.Ci, 1}, stream);
+        const int e = way == BY_TMA     ? launch_pointwise_mma_slope(s, x, weight, bias, residual, grad, to, rest, sums, stream)
+                      : way == BY_SPLIT ? launch_pointwise_split_slope(s, x, weight, bias, residual, grad, to, rest, sums, stream)
+                                        : launch_product<SLOPE>(s, {x, weight, bias, residual, grad, to, rest, s.Ci, s.Co, s.Ci, 1}, stream);
         if (e) return e;
         dz = to;
     }
     if (need_mask & BC_NEED_PW_INPUT) {
         const int way = way_of(s, true, pointwise_mma_aligned(dz, weight, grad_input));
-        const int e = way == BY_TMA     ? launch_pointwise_mma_input(s, dz, weight, grad_input, stream)
-                      : way == BY_SPLIT ? launch_pointwise_split_input(s, dz, weight, grad_input, stream)
-                                        : launch_product<INPUT>(s, {dz, weight, nullptr, nullptr, nullptr, grad_input, s.Co, s.Ci, 1, s.Ci}, stream);
+        const int e = way == BY_TMA     ? launch_pointwise_mma_input(s, dz, rest, weight, grad_input, stream)
+                      : way == BY_SPLIT ? launch_pointwise_split_input(s, dz, rest, weight, grad_input, stream)
+                                        : launch_product<INPUT>(s, {dz, weight, nullptr, nullptr, nullptr, grad_input, rest, s.Co, s.Ci, 1, s.Ci}, stream);
         if (e) return e;
     }
     if (!want_weight && !want_bias) return BC_OK;
@@ -385,8 +413,8 @@ int launch_pointwise_backward(const PointwiseShape &s, const void *x, const void
         float *partial = static_cast<float *>(take(partial_bytes(s)));
         int splits = pointwise_mma_aligned(dz, x) ? pointwise_mma_weight_splits(s) : 0;
         int e = BC_ERR_BAD_SHAPE;
-        if (splits) e = launch_pointwise_mma_weight(s, dz, x, partial, want_bias && !sums, stream);
-        else if ((splits = pointwise_split_weight_splits(s))) e = launch_pointwise_split_weight(s, dz, x, partial, want_bias && !sums, stream);
+        if (splits) e = launch_pointwise_mma_weight(s, dz, rest, x, partial, want_bias && !sums, stream);
+        else if ((splits = pointwise_split_weight_splits(s, rest))) e = launch_pointwise_split_weight(s, dz, rest, x, partial, want_bias && !sums, stream);
         if (e) return e;
         if (want_weight) of_weights = {partial, pointwise_partial_stride(s.Co, s.Ci), weights, splits, grad_weight};
         if (want_bias && !sums) of_sums = {partial + weights, pointwise_partial_stride(s.Co, s.Ci), s.Co, splits, grad_bias};

@@ -9,7 +9,7 @@
 // CTA has its SM to itself, the next block's are on their way while a block is dealt with.
 //
 // Measured on B200, (64,256->256,64,128) bf16 last: grad_input 97 us, 5.4 TB/s or 0.83 of the copy bandwidth; forward with residual
-// and GELU 182, slope 249, bound by the epilogue's instructions.
+// and GELU 182, slope 249, bound by the epilogue's instructions (grad_input of one tensor; the slope without storing what its rounding leaves).
 //
 // pointwise_weight_mma_kernel: grad_weight, D[o, i] = sum_p dz[o, p] x[i, p], 128 x up to 256 weights, split over the pixels; 96 us there.
 #include "bc_mma.cuh"
@@ -25,14 +25,15 @@ constexpr uint32_t kStage = 16384;      // 128 pixels x 64 k
 constexpr size_t kMostShared = 227 << 10;
 
 struct MmaProduct {
-    CUtensorMap a, w;
+    CUtensorMap a, a_rest, w;      // INPUT: dz is the sum of two tensors
     const void *bias, *residual, *grad;
-    void *out;
+    void *out, *rest;        // rest: SLOPE, what the rounding of dz leaves, or null
     float *sums;             // SLOPE: [CTA / tiles_n][Cn] sums of dz over the CTA's pixels, or null
     int64_t P;               // pixels of a sample (of all of them together, channels last)
     int K, Cn, samples;
     int tiles_p, tiles_n;
     int bn, stages, columns; // channels of a tile; slices in the ring; columns of tensor memory for one set
+    int parts;               // tensors that A is the sum of
     uint32_t instruction;
 };
 
@@ -57,7 +58,7 @@ __global__ void __launch_bounds__(32 * (kEpilogue * PAIR + 2), PAIR == 1 ? 2 : 1
     extern __shared__ char raw_smem[];
     const uint32_t raw = smem_u32(raw_smem), base = (raw + 1023) & ~1023u;
     char *smem = raw_smem + (base - raw);
-    const int chunks = (q.K + 63) / 64;
+    const int chunks = (q.K + 63) / 64, parts = MODE == INPUT ? q.parts : 1;
     const MmaLayout lay{q.bn, q.stages, chunks, PAIR, MODE == INPUT};
     float *bias_smem = reinterpret_cast<float *>(smem + lay.bias()), *sums_smem = reinterpret_cast<float *>(smem + lay.sums());
     const uint32_t full = base + lay.barriers(), empty = full + 8 * q.stages, ready = empty + 8 * q.stages, drained = ready + 16,
@@ -106,15 +107,17 @@ __global__ void __launch_bounds__(32 * (kEpilogue * PAIR + 2), PAIR == 1 ? 2 : 1
             for (unsigned tile = walker; tile < tiles; tile += walkers) {
                 const unsigned sample = tile / (unsigned)q.tiles_p;
                 const int64_t p0 = (int64_t)(tile - sample * q.tiles_p) * 128;
-                for (int c = 0; c < chunks; ++c) {
+                for (int i = 0; i < parts * chunks; ++i) {      // (the parts of a slice in turn)
+                    const int c = MODE == INPUT && parts == 2 ? i >> 1 : i;
+                    const CUtensorMap *a = MODE == INPUT && parts == 2 && (i & 1) ? &q.a_rest : &q.a;
                     if (!wait(empty + 8 * stage, phase ^ 1)) break;
                     const uint32_t to = base + lay.ring() + stage * kStage, bar = full + 8 * stage;
                     mbar_expect(bar, kStage);
                     if (LAST) {
-                        tile_load(to, &q.a, 64 * c, (int)p0, bar);
+                        tile_load(to, a, 64 * c, (int)p0, bar);
                     } else {
-                        tile_load(to, &q.a, (int)p0, 64 * c, sample, bar);
-                        tile_load(to + kBlockBytes, &q.a, (int)p0 + 64, 64 * c, sample, bar);
+                        tile_load(to, a, (int)p0, 64 * c, sample, bar);
+                        tile_load(to + kBlockBytes, a, (int)p0 + 64, 64 * c, sample, bar);
                     }
                     if (++stage == (uint32_t)q.stages) {
                         stage = 0;
@@ -133,15 +136,16 @@ __global__ void __launch_bounds__(32 * (kEpilogue * PAIR + 2), PAIR == 1 ? 2 : 1
             for (unsigned tile = walker; tile < tiles; tile += walkers) {
                 if (!wait(drained + 8 * set, set_phase ^ 1)) break;
                 tmem_acquire();
-                for (int c = 0; c < chunks; ++c) {
+                for (int i = 0; i < parts * chunks; ++i) {
                     if (!wait(full + 8 * stage, phase)) break;
                     tmem_acquire();
+                    const int c = MODE == INPUT && parts == 2 ? i >> 1 : i;
                     const uint64_t a = further(ring, stage * kStage), w = further(weights, c * lay.slice());
                     const int k_used = q.K - 64 * c;
 #pragma unroll
                     for (int k = 0; k < 64; k += 16)
                         if (k < k_used)
-                            mma(tmem + set * q.columns, further(a, (LAST ? 2 : 128) * k), further(w, (MODE == INPUT ? 128 : 2) * k), q.instruction, c || k);
+                            mma(tmem + set * q.columns, further(a, (LAST ? 2 : 128) * k), further(w, (MODE == INPUT ? 128 : 2) * k), q.instruction, i || k);
                     mma_commit(empty + 8 * stage);
                     if (++stage == (uint32_t)q.stages) {
                         stage = 0;
@@ -164,7 +168,7 @@ __global__ void __launch_bounds__(32 * (kEpilogue * PAIR + 2), PAIR == 1 ? 2 : 1
         // inner.  Every second block is a warp's, or two warps', two of the four vectors each.
         const int outer = (lane >> 2) + 8 * EACH * member, inner = 8 * (lane & 3);
         const T *residual = static_cast<const T *>(q.residual), *grad = static_cast<const T *>(q.grad);
-        T *out = static_cast<T *>(q.out);
+        T *out = static_cast<T *>(q.out), *rest = static_cast<T *>(q.rest);
         struct Block {
             int64_t at;
             int there;                // bits
@@ -255,7 +259,12 @@ __global__ void __launch_bounds__(32 * (kEpilogue * PAIR + 2), PAIR == 1 ? 2 : 1
 #pragma unroll
                         for (int j = 0; j < 4; ++j) z[j] = activate2<ACT, T>(z[j]);
                     }
-                    if (there) *reinterpret_cast<uint4 *>(out + now.at + 8 * i * (LAST ? (int64_t)q.Cn : q.P)) = pack_pairs<T>(z);
+                    if (there) {
+                        const int64_t at = now.at + 8 * i * (LAST ? (int64_t)q.Cn : q.P);
+                        const uint4 rounded = pack_pairs<T>(z);
+                        *reinterpret_cast<uint4 *>(out + at) = rounded;
+                        if (MODE == SLOPE && rest) *reinterpret_cast<uint4 *>(rest + at) = left_by_rounding<T>(z, rounded);
+                    }
                 }
                 if (MODE == SLOPE && LAST && q.sums) {      // eight channels over the eight lanes of their vectors
                     fold(total, lane, 4, 4);
@@ -306,23 +315,25 @@ __global__ void __launch_bounds__(32 * (kEpilogue * PAIR + 2), PAIR == 1 ? 2 : 1
 constexpr int kWeightThreads = 32 * 6, kMostStages = 8;
 
 struct WeightMma {
-    CUtensorMap dz, x;
+    CUtensorMap dz, dz_rest, x;
     float *partial;          // a row a split: Co * Ci sums, then Co sums of dz
     int64_t per;             // slices of 64 pixels of a split
     int64_t slices;          // of a sample
     int samples, Ci, Co;
     int tiles_i;
     int bn, rows, stages, columns;      // input channels of a tile; rows of dz that are loaded (planes); ring; tensor memory
+    int parts;               // tensors that dz is the sum of
     bool sums;
     uint32_t instruction;
 };
 
-// Shared memory from a 1024-byte boundary on: slices of dz (128 channels) and x (bn), then barriers.
+// Shared memory from a 1024-byte boundary on: slices of dz (128 channels of each part) and x (bn), then barriers.
 struct WeightLayout {
-    int bn, stages;
+    int bn, stages, parts;
     bool last;
     __host__ __device__ uint32_t x_bytes() const { return last ? (uint32_t)((bn + 63) / 64) * kBlockBytes : (uint32_t)bn * 128; }
-    __host__ __device__ uint32_t stage() const { return 2 * kBlockBytes + x_bytes(); }
+    __host__ __device__ uint32_t x_at() const { return parts * 2 * kBlockBytes; }
+    __host__ __device__ uint32_t stage() const { return x_at() + x_bytes(); }
     __host__ __device__ uint32_t barriers() const { return stages * stage(); }
     __host__ __device__ uint32_t bytes() const { return barriers() + (2 * stages + 1) * 8 + 8 + 1024; }
 };
@@ -335,7 +346,7 @@ __global__ void __launch_bounds__(kWeightThreads) pointwise_weight_mma_kernel(co
     __shared__ float part[128][9];
     const uint32_t raw = smem_u32(raw_smem), base = (raw + 1023) & ~1023u;
     char *smem = raw_smem + (base - raw);
-    const WeightLayout lay{q.bn, q.stages, LAST};
+    const WeightLayout lay{q.bn, q.stages, q.parts, LAST};
     const uint32_t full = base + lay.barriers(), empty = full + 8 * q.stages, ready = empty + 8 * q.stages;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + lay.barriers() + (2 * q.stages + 1) * 8);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -366,20 +377,23 @@ __global__ void __launch_bounds__(kWeightThreads) pointwise_weight_mma_kernel(co
     if (warp == 4) {
         if (lane == 0) {
             const int a_blocks = LAST ? (o0 + 64 < q.Co ? 2 : 1) : 0, b_blocks = (q.bn + 63) / 64;
-            const uint32_t bytes = (LAST ? a_blocks * kBlockBytes : (uint32_t)q.rows * 128) + lay.x_bytes();
+            const uint32_t bytes = q.parts * (LAST ? a_blocks * kBlockBytes : (uint32_t)q.rows * 128) + lay.x_bytes();
             uint32_t stage = 0, phase = 0;
             for (int64_t slice = first; slice < last; ++slice) {
                 if (!wait(empty + 8 * stage, phase ^ 1)) break;
                 const int sample = (int)(slice / q.slices), p0 = (int)(slice - sample * q.slices) * 64;
-                const uint32_t a = base + stage * lay.stage(), b = a + 2 * kBlockBytes, bar = full + 8 * stage;
+                const uint32_t a = base + stage * lay.stage(), b = a + lay.x_at(), bar = full + 8 * stage;
                 mbar_expect(bar, bytes);
-                if (LAST) {
-                    for (int i = 0; i < a_blocks; ++i) tile_load(a + i * kBlockBytes, &q.dz, o0 + 64 * i, p0, bar);
-                    for (int i = 0; i < b_blocks; ++i) tile_load(b + i * kBlockBytes, &q.x, i0 + 64 * i, p0, bar);
-                } else {
-                    tile_load(a, &q.dz, p0, o0, sample, bar);
-                    tile_load(b, &q.x, p0, i0, sample, bar);
+                for (int part = 0; part < q.parts; ++part) {
+                    const CUtensorMap *dz = part ? &q.dz_rest : &q.dz;
+                    const uint32_t to = a + part * 2 * kBlockBytes;
+                    if (LAST)
+                        for (int i = 0; i < a_blocks; ++i) tile_load(to + i * kBlockBytes, dz, o0 + 64 * i, p0, bar);
+                    else tile_load(to, dz, p0, o0, sample, bar);
                 }
+                if (LAST)
+                    for (int i = 0; i < b_blocks; ++i) tile_load(b + i * kBlockBytes, &q.x, i0 + 64 * i, p0, bar);
+                else tile_load(b, &q.x, p0, i0, sample, bar);
                 if (++stage == (uint32_t)q.stages) {
                     stage = 0;
                     phase ^= 1;
@@ -392,11 +406,13 @@ __global__ void __launch_bounds__(kWeightThreads) pointwise_weight_mma_kernel(co
             for (int64_t slice = first; slice < last; ++slice) {
                 if (!wait(full + 8 * stage, phase)) break;
                 tmem_acquire();
-                const uint32_t a = base + stage * lay.stage(), b = a + 2 * kBlockBytes;
+                const uint32_t a = base + stage * lay.stage(), b = a + lay.x_at();
 #pragma unroll
-                for (int k = 0; k < 64; k += 16)
-                    mma(tmem, LAST ? mn_major(a, k, kBlockBytes) : k_major(a, k), LAST ? mn_major(b, k, kBlockBytes) : k_major(b, k), q.instruction,
-                        slice > first || k);
+                for (int k = 0; k < 64; k += 16) {
+                    const uint64_t x = LAST ? mn_major(b, k, kBlockBytes) : k_major(b, k), dz = LAST ? mn_major(a, k, kBlockBytes) : k_major(a, k);
+                    mma(tmem, dz, x, q.instruction, slice > first || k);
+                    if (q.parts == 2) mma(tmem, further(dz, 2 * kBlockBytes), x, q.instruction, true);
+                }
                 mma_commit(empty + 8 * stage);
                 if (++stage == (uint32_t)q.stages) {
                     stage = 0;
@@ -420,12 +436,13 @@ __global__ void __launch_bounds__(kWeightThreads) pointwise_weight_mma_kernel(co
                     const int k = 8 * j + pixel;
                     const char *from = LAST ? a + (group >> 3) * kBlockBytes + k * 128 + (((group & 7) ^ (k & 7)) << 4)
                                             : a + threadIdx.x * 128 + ((j ^ (threadIdx.x & 7)) << 4);
-                    if (LAST ? o0 + 8 * group < q.Co : o0 + (int)threadIdx.x < q.Co) {
-                        float v[8];
-                        unpack<T>(*reinterpret_cast<const uint4 *>(from), v);
+                    if (LAST ? o0 + 8 * group < q.Co : o0 + (int)threadIdx.x < q.Co)
+                        for (int part = 0; part < q.parts; ++part) {
+                            float v[8];
+                            unpack<T>(*reinterpret_cast<const uint4 *>(from + part * 2 * kBlockBytes), v);
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) total[i] += v[i];
-                    }
+                            for (int i = 0; i < 8; ++i) total[i] += v[i];
+                        }
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(empty + 8 * stage);
@@ -515,7 +532,7 @@ bool plan_product(const PointwiseShape &s, int K, int Cn, int mode, Plan *plan)
 }
 
 template <int MODE>
-int launch_mma(const PointwiseShape &s, const Plan &plan, MmaProduct q, const void *a, const void *w, cudaStream_t stream)
+int launch_mma(const PointwiseShape &s, const Plan &plan, MmaProduct q, const void *a, const void *a_rest, const void *w, cudaStream_t stream)
 {
     const bool bf16 = s.io_kind == BC_IO_BF16;
     q.samples = s.last ? 1 : s.N;
@@ -530,8 +547,13 @@ int launch_mma(const PointwiseShape &s, const Plan &plan, MmaProduct q, const vo
         const uint64_t last_sizes[2] = {(uint64_t)q.K, (uint64_t)q.P}, last_strides[1] = {(uint64_t)q.K};
         const uint64_t sizes[3] = {(uint64_t)q.P, (uint64_t)q.K, (uint64_t)q.samples}, strides[2] = {(uint64_t)q.P, (uint64_t)q.P * q.K};
         const uint32_t last_box[2] = {64, 128}, box[3] = {64, 64, 1};
-        if (const int e = s.last ? make_map(&q.a, a, bf16, 2, last_sizes, last_strides, last_box) : make_map(&q.a, a, bf16, 3, sizes, strides, box))
-            return e;
+        auto map = [&](CUtensorMap *to, const void *from) {
+            return s.last ? make_map(to, from, bf16, 2, last_sizes, last_strides, last_box) : make_map(to, from, bf16, 3, sizes, strides, box);
+        };
+        if (const int e = map(&q.a, a)) return e;
+        q.parts = a_rest ? 2 : 1;
+        if (a_rest)
+            if (const int e = map(&q.a_rest, a_rest)) return e;
         const uint64_t w_sizes[2] = {(uint64_t)s.Ci, (uint64_t)s.Co}, w_strides[1] = {(uint64_t)s.Ci};
         const uint32_t w_box[2] = {64, MODE == INPUT ? 64u : (uint32_t)plan.bn};
         if (const int e = make_map(&q.w, w, bf16, 2, w_sizes, w_strides, w_box)) return e;
@@ -591,10 +613,10 @@ int launch_pointwise_mma_forward(const PointwiseShape &s, const void *x, const v
     q.out = out;
     q.K = s.Ci;
     q.Cn = s.Co;
-    return launch_mma<FORWARD>(s, plan, q, x, weight, stream);
+    return launch_mma<FORWARD>(s, plan, q, x, nullptr, weight, stream);
 }
 int launch_pointwise_mma_slope(const PointwiseShape &s, const void *x, const void *weight, const void *bias, const void *residual,
-                               const void *grad, void *dz, float *sums, cudaStream_t stream)
+                               const void *grad, void *dz, void *rest, float *sums, cudaStream_t stream)
 {
     Plan plan;
     plan_product(s, s.Ci, s.Co, SLOPE, &plan);
@@ -603,12 +625,14 @@ int launch_pointwise_mma_slope(const PointwiseShape &s, const void *x, const voi
     q.residual = residual;
     q.grad = grad;
     q.out = dz;
+    q.rest = rest;
     q.sums = sums;
     q.K = s.Ci;
     q.Cn = s.Co;
-    return launch_mma<SLOPE>(s, plan, q, x, weight, stream);
+    return launch_mma<SLOPE>(s, plan, q, x, nullptr, weight, stream);
 }
-int launch_pointwise_mma_input(const PointwiseShape &s, const void *dz, const void *weight, void *grad_input, cudaStream_t stream)
+int launch_pointwise_mma_input(const PointwiseShape &s, const void *dz, const void *rest, const void *weight, void *grad_input,
+                               cudaStream_t stream)
 {
     Plan plan;
     plan_product(s, s.Co, s.Ci, INPUT, &plan);
@@ -616,7 +640,7 @@ int launch_pointwise_mma_input(const PointwiseShape &s, const void *dz, const vo
     q.out = grad_input;
     q.K = s.Co;
     q.Cn = s.Ci;
-    return launch_mma<INPUT>(s, plan, q, dz, weight, stream);
+    return launch_mma<INPUT>(s, plan, q, dz, rest, weight, stream);
 }
 
 // ---- grad_weight: rows of pointwise_partial_stride() floats, to be added
@@ -626,7 +650,7 @@ struct WeightPlan {
     int64_t slices, per;
     uint32_t smem;
 };
-bool plan_weight(const PointwiseShape &s, WeightPlan *plan)
+bool plan_weight(const PointwiseShape &s, int parts, WeightPlan *plan)
 {
     if (!rows_aligned(s)) return false;
     const int64_t P = s.last ? s.N * s.P : s.P, samples = s.last ? 1 : s.N;
@@ -639,7 +663,7 @@ bool plan_weight(const PointwiseShape &s, WeightPlan *plan)
     r.columns = 32;
     while (r.columns < r.bn) r.columns *= 2;
     for (r.stages = kMostStages; r.stages > 2; --r.stages) {
-        r.smem = WeightLayout{r.bn, r.stages, s.last}.bytes();
+        r.smem = WeightLayout{r.bn, r.stages, parts, s.last}.bytes();
         if (r.smem <= 200 << 10) break;
     }
     r.slices = ceil_div(P, 64);
@@ -656,12 +680,13 @@ bool plan_weight(const PointwiseShape &s, WeightPlan *plan)
 int pointwise_mma_weight_splits(const PointwiseShape &s)
 {
     WeightPlan plan;
-    return plan_weight(s, &plan) ? plan.splits : 0;
+    return plan_weight(s, 1, &plan) ? plan.splits : 0;      // (as many in two parts)
 }
-int launch_pointwise_mma_weight(const PointwiseShape &s, const void *dz, const void *x, float *partial, bool sums, cudaStream_t stream)
+int launch_pointwise_mma_weight(const PointwiseShape &s, const void *dz, const void *rest, const void *x, float *partial, bool sums,
+                                cudaStream_t stream)
 {
     WeightPlan plan;
-    plan_weight(s, &plan);
+    plan_weight(s, rest ? 2 : 1, &plan);
     const bool bf16 = s.io_kind == BC_IO_BF16;
     WeightMma q{};
     q.partial = partial;
@@ -684,7 +709,10 @@ int launch_pointwise_mma_weight(const PointwiseShape &s, const void *dz, const v
         const uint32_t last_box[2] = {64, 64}, box[3] = {64, rows, 1};
         return s.last ? make_map(to, from, bf16, 2, last_sizes, last_strides, last_box) : make_map(to, from, bf16, 3, sizes, strides, box);
     };
+    q.parts = rest ? 2 : 1;
     if (const int e = map(&q.dz, dz, s.Co, q.rows)) return e;
+    if (rest)
+        if (const int e = map(&q.dz_rest, rest, s.Co, q.rows)) return e;
     if (const int e = map(&q.x, x, s.Ci, plan.bn)) return e;
     auto go = [&](auto kernel) {
         if (const int e = raise_smem_limit((const void *)kernel, 200 << 10)) return e;

@@ -30,6 +30,7 @@ constexpr int kParts = sizeof(T) == 4 ? 3 : 1;
 struct SplitProduct {
     const void *a, *w, *bias, *residual, *grad;
     void *out;
+    void *rest;              // 16-bit.  INPUT: null, or what `a` lacks of dz; SLOPE: where that goes, or null
     float *sums;             // SLOPE: [CTA / tiles_n][Cn] sums of dz over the CTA's pixels, or null
     int64_t P;               // pixels of a sample (of all of them together, channels last)
     int K, Cn, samples;
@@ -116,7 +117,7 @@ __global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const Spli
     extern __shared__ char raw_smem[];
     const uint32_t raw = smem_u32(raw_smem), base = (raw + 1023) & ~1023u;
     char *smem = raw_smem + (base - raw);
-    const int chunks = (q.K + 63) / 64;
+    const int chunks = (q.K + 63) / 64, sources = PARTS == 1 && MODE == INPUT && q.rest ? 2 : 1;      // tensors that A is the sum of
     const SplitLayout lay{q.bn, q.stages, chunks, PARTS, LAST};
     float *bias_smem = reinterpret_cast<float *>(smem + lay.bias()), *sums_smem = reinterpret_cast<float *>(smem + lay.sums());
     const uint32_t full = base + lay.barriers(), empty = full + 8 * q.stages, ready = empty + 8 * q.stages, drained = ready + 16;
@@ -145,13 +146,13 @@ __global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const Spli
     for (int i = threadIdx.x; i < q.bn; i += kThreads)
         bias_smem[i] = MODE != INPUT && q.bias && n0 + i < q.Cn ? to_float(static_cast<const T *>(q.bias)[n0 + i]) : 0.f;
     for (int i = threadIdx.x; i < 4 * q.bn; i += kThreads) sums_smem[i] = 0.f;
-    // A producer's way through this CTA's slices.
+    // A producer's way through this CTA's slices, the sources of a slice in turn.
     struct Cursor {
         unsigned tile;
         int c;
     };
     auto advance = [&](Cursor &at) {
-        if (++at.c == chunks) {
+        if (++at.c == sources * chunks) {
             at.c = 0;
             at.tile += walkers;
         }
@@ -242,11 +243,12 @@ __global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const Spli
         Cursor at{walker, 0};
         if (group) advance(at);
         for (; at.tile < tiles; advance(at), advance(at)) {
-            const int c = at.c;
+            const int c = sources == 2 ? at.c >> 1 : at.c;
             const unsigned sample = at.tile / (unsigned)q.tiles_p;
             const int64_t p0 = (int64_t)(at.tile - sample * q.tiles_p) * 128;
             const int pixels = (int)min((int64_t)128, q.P - p0), k_left = q.K - 64 * c, k_used = (k_left + 15) / 16 * 16;
-            const T *a = a_all + (LAST ? p0 * q.K + 64 * c : ((int64_t)sample * q.K + 64 * c) * q.P + p0);
+            const T *a = (sources == 2 && (at.c & 1) ? static_cast<const T *>(q.rest) : a_all) +
+                         (LAST ? p0 * q.K + 64 * c : ((int64_t)sample * q.K + 64 * c) * q.P + p0);
             // a vector: planes, eight pixels of a k; last, eight k of a pixel.  `inner` of it are there.
             uint4 raw_v[8];
 #pragma unroll
@@ -282,9 +284,10 @@ __global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const Spli
             for (unsigned tile = walker; tile < tiles; tile += walkers) {
                 if (!wait(drained + 8 * set, set_phase ^ 1)) break;
                 tmem_acquire();
-                for (int c = 0; c < chunks; ++c) {
+                for (int piece = 0; piece < sources * chunks; ++piece) {
                     if (!wait(full + 8 * stage, phase)) break;
                     tmem_acquire();
+                    const int c = sources == 2 ? piece >> 1 : piece;
                     const uint64_t a = further(ring, stage * PARTS * kPart);
                     const uint64_t w = further(weights, c * PARTS * lay.slice());
                     const int k_used = q.K - 64 * c;
@@ -295,7 +298,7 @@ __global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const Spli
                             const uint64_t ak = further(a, (LAST ? 2 : 128) * k), wk = further(w, 2 * k);
                             if (PARTS == 3 && q.merged) {
                                 // the weights' parts in a row are one operand: an instruction takes some 90 cycles at any width here
-                                mma(d, ak, wk, q.instruction, c || k);
+                                mma(d, ak, wk, q.instruction, piece || k);
                                 mma(d + q.bn, further(ak, kPart), wk, q.instruction - (q.bn >> 3 << 17), true);
                                 mma(d + 2 * q.bn, further(ak, 2 * kPart), wk, q.instruction - (2 * q.bn >> 3 << 17), true);
                             } else {
@@ -304,7 +307,7 @@ __global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const Spli
 #pragma unroll
                                     for (int j = 0; j < PARTS - i; ++j)
                                         mma(i + j ? d + q.columns : d, further(ak, i * kPart), further(wk, j * lay.slice()), q.instruction,
-                                            c || k || i + j > 1 || i > 0);
+                                            piece || k || i + j > 1 || i > 0);
                             }
                         }
                     mma_commit(empty + 8 * stage);
@@ -322,7 +325,7 @@ __global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const Spli
         float *staging = reinterpret_cast<float *>(smem + lay.staging()) + warp * 32 * kPitch;
         const int quarter = warp & 3, half = warp >> 2, blocks = q.bn / 16;
         const T *residual = static_cast<const T *>(q.residual), *grad = static_cast<const T *>(q.grad);
-        T *out = static_cast<T *>(q.out);
+        T *out = static_cast<T *>(q.out), *rest = static_cast<T *>(q.rest);
         uint32_t set = 0, set_phase = 0;
         for (unsigned tile = walker; tile < tiles; tile += walkers) {
             const unsigned sample = tile / (unsigned)q.tiles_p;
@@ -410,8 +413,13 @@ __global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const Spli
                     }
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        if (there(i + h)) out[at + (i + h) * step] = from_float<T>(v[i + h]);
-                        else v[i + h] = 0.f;
+                        if (there(i + h)) {
+                            const T rounded = from_float<T>(v[i + h]);
+                            out[at + (i + h) * step] = rounded;
+                            if (PARTS == 1 && MODE == SLOPE && rest) rest[at + (i + h) * step] = from_float<T>(left_by_rounding(v[i + h], rounded));
+                        } else {
+                            v[i + h] = 0.f;
+                        }
                         if (LAST) total += v[i + h];
                     }
                 }
@@ -451,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const Spli
 constexpr int kWeightEpilogue = 4, kWeightThreads = 32 * (kWeightEpilogue + kGroups * kGroupWarps + 1);
 
 struct WeightSplit {
-    const void *dz, *x;
+    const void *dz, *rest, *x;      // (rest: 16-bit, what dz lacks, or null)
     float *partial;          // a row a split: Co * Ci sums, then Co sums of dz
     int64_t P;
     int per, slices;         // slices of a split; of a sample
@@ -463,13 +471,14 @@ struct WeightSplit {
 };
 
 struct WeightSplitLayout {
-    int rows, bn, stages, slots, parts;
+    int rows, bn, stages, slots, parts, sources;      // (sources: tensors that dz is the sum of)
     bool last;
     __host__ __device__ uint32_t bytes_of(int channels) const { return last ? (uint32_t)((channels + 63) / 64) * kBlockBytes : (uint32_t)channels * 128; }
     // (M is 128 whatever there is of dz: what lies behind its rows is read as well, and leads nowhere)
     __host__ __device__ uint32_t dz_part() const { return bytes_of(rows); }
     __host__ __device__ uint32_t x_part() const { return bytes_of(bn); }
-    __host__ __device__ uint32_t stage() const { return (parts * (dz_part() + x_part()) + 1023) / 1024 * 1024; }
+    __host__ __device__ uint32_t x_at() const { return parts * sources * dz_part(); }
+    __host__ __device__ uint32_t stage() const { return (x_at() + parts * x_part() + 1023) / 1024 * 1024; }
     __host__ __device__ uint32_t copies() const { return stages * stage() + 2 * kBlockBytes; }
     __host__ __device__ int each() const { return ((rows + bn) * 16 + kProducers - 1) / kProducers; }      // vectors of a thread
     __host__ __device__ uint32_t barriers() const { return copies() + slots * each() * 16 * kProducers; }
@@ -484,7 +493,8 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
     __shared__ float sums_smem[kGroups][128];
     const uint32_t raw = smem_u32(raw_smem), base = (raw + 1023) & ~1023u;
     char *smem = raw_smem + (base - raw);
-    const WeightSplitLayout lay{q.rows, q.bn, q.stages, q.slots, PARTS, LAST};
+    const int sources = PARTS == 1 && q.rest ? 2 : 1;
+    const WeightSplitLayout lay{q.rows, q.bn, q.stages, q.slots, PARTS, sources, LAST};
     const uint32_t full = base + lay.barriers(), empty = full + 8 * q.stages, ready = empty + 8 * q.stages;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + lay.barriers() + (2 * q.stages + 1) * 8);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -552,7 +562,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
         for (int slice = first; slice < last; ++slice) {
             copies_wait(q.slots);
             if (!wait(empty + 8 * stage, phase ^ 1)) break;
-            char *const dz_to = smem + stage * lay.stage(), *const x_to = dz_to + PARTS * lay.dz_part();
+            char *const dz_to = smem + stage * lay.stage(), *const x_to = dz_to + lay.x_at();
             const char *from = own + (q.slots > 1 ? (uint32_t)(slice - first & 1) * slot_bytes : 0);
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
@@ -615,13 +625,13 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
         }
     } else if (warp >= kWeightEpilogue && warp < kWeightEpilogue + kGroups * kGroupWarps) {
         const int group = (warp - kWeightEpilogue) / kGroupWarps, me = threadIdx.x - 32 * (kWeightEpilogue + group * kGroupWarps);
-        const int of_dz = q.rows * 8, total = of_dz + q.bn * 8;      // vectors of a slice
-        float sum[8] = {};      // planes: of the channel of vector me + 128 j; last: of the channels of every vector of dz
+        const int of_source = q.rows * 8, of_dz = sources * of_source, total = of_dz + q.bn * 8;      // vectors of a slice
+        float sum[8] = {};      // planes: of the channel of vector me + 128 j of a source; last: of the channels of every vector of dz
         for (int slice = first + group; slice < last; slice += kGroups) {
             const unsigned nth = slice - first, stage = nth % (unsigned)q.stages, phase = nth / (unsigned)q.stages & 1;
             const int64_t sample = (unsigned)slice / (unsigned)q.slices, p0 = (slice - sample * q.slices) * 64;
             const int pixels = (int)min((int64_t)64, q.P - p0);
-            char *const dz_to = smem + stage * lay.stage(), *const x_to = dz_to + PARTS * lay.dz_part();
+            char *const dz_to = smem + stage * lay.stage(), *const x_to = dz_to + lay.x_at();
             bool waited = false;
             for (int v0 = me; v0 < total; v0 += 8 * 128) {
                 uint4 v[8];
@@ -629,9 +639,9 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
                 for (int j = 0; j < 8; ++j) {
                     const int e = v0 + 128 * j;
                     if (e >= total) break;
-                    const bool dz = e < of_dz;
-                    const int f = dz ? e : e - of_dz, C = dz ? q.Co : q.Ci, c0 = dz ? o0 : i0, wide = (dz ? q.rows : q.bn) / 8;
-                    const T *from = dz ? dz_all : x_all;
+                    const bool dz = e < of_dz, more = dz && e >= of_source;
+                    const int f = dz ? more ? e - of_source : e : e - of_dz, C = dz ? q.Co : q.Ci, c0 = dz ? o0 : i0, wide = (dz ? q.rows : q.bn) / 8;
+                    const T *from = dz ? more ? static_cast<const T *>(q.rest) : dz_all : x_all;
                     if (LAST) {      // eight channels of a pixel
                         const int p = (unsigned)f / (unsigned)wide, c = c0 + 8 * (f - p * wide);
                         if constexpr (PARTS == 1) v[j] = load8<T, VEC>(from + (p0 + p) * C + c, p < pixels ? C - c : 0);
@@ -648,10 +658,10 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
                 for (int j = 0; j < 8; ++j) {
                     const int e = v0 + 128 * j;
                     if (e >= total) break;
-                    const bool dz = e < of_dz;
-                    const int f = dz ? e : e - of_dz, wide = (dz ? q.rows : q.bn) / 8;
+                    const bool dz = e < of_dz, more = dz && e >= of_source;
+                    const int f = dz ? more ? e - of_source : e : e - of_dz, wide = (dz ? q.rows : q.bn) / 8;
                     const int outer = LAST ? (unsigned)f / (unsigned)wide : f >> 3, chunk = LAST ? f - outer * wide : f & 7;
-                    char *to = (dz ? dz_to : x_to) + (LAST ? (chunk >> 3) * kBlockBytes : 0) + outer * 128 + (((chunk & 7) ^ (outer & 7)) << 4);
+                    char *to = (dz ? more ? dz_to + lay.dz_part() : dz_to : x_to) + (LAST ? (chunk >> 3) * kBlockBytes : 0) + outer * 128 + (((chunk & 7) ^ (outer & 7)) << 4);
                     *reinterpret_cast<uint4 *>(to) = v[j];
                     if (sums && dz) {
                         float g[8] = {};
@@ -682,6 +692,13 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
                     asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
                 }
             } else {
+                // (rows of less than 128: the second source's vectors come as later j)
+                if (sources == 2)
+#pragma unroll
+                    for (int j = 1; j < 8; j *= 2)
+                        if (16 * j == q.rows)
+#pragma unroll
+                            for (int i = 0; i < j; ++i) sum[i] += sum[j + i];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     float g = sum[j];
@@ -697,7 +714,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
         if (lane == 0) {
             uint64_t a[PARTS], b[PARTS];
             for (int i = 0; i < PARTS; ++i) {
-                const uint32_t dz = base + i * lay.dz_part(), x = base + PARTS * lay.dz_part() + i * lay.x_part();
+                const uint32_t dz = base + i * lay.dz_part(), x = base + lay.x_at() + i * lay.x_part();
                 a[i] = LAST ? mn_major(dz, 0, kBlockBytes) : k_major(dz, 0);
                 b[i] = LAST ? mn_major(x, 0, kBlockBytes) : k_major(x, 0);
             }
@@ -707,13 +724,16 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
                 tmem_acquire();
                 const uint32_t stage_at = stage * lay.stage();
 #pragma unroll
-                for (int k = 0; k < 64; k += 16)
+                for (int k = 0; k < 64; k += 16) {
 #pragma unroll
                     for (int i = 0; i < PARTS; ++i)
 #pragma unroll
                         for (int j = 0; j < PARTS - i; ++j)
                             mma(i + j ? tmem + q.columns : tmem, further(a[i], stage_at + (LAST ? 128 : 2) * k), further(b[j], stage_at + (LAST ? 128 : 2) * k),
                                 q.instruction, slice > first || k || i + j > 1 || i > 0);
+                    if (PARTS == 1 && sources == 2)
+                        mma(tmem, further(a[0], stage_at + lay.dz_part() + (LAST ? 128 : 2) * k), further(b[0], stage_at + (LAST ? 128 : 2) * k), q.instruction, true);
+                }
                 mma_commit(empty + 8 * stage);
                 if (++stage == (uint32_t)q.stages) {
                     stage = 0;
@@ -858,20 +878,21 @@ int launch_pointwise_split_forward(const PointwiseShape &s, const void *x, const
 {
     SplitPlan plan;
     plan_split(s, s.Ci, s.Co, &plan);
-    return launch_split<FORWARD>(s, plan, {x, weight, bias, residual, nullptr, out, nullptr, 0, s.Ci, s.Co, 0, s.Ci, 1}, stream);
+    return launch_split<FORWARD>(s, plan, {x, weight, bias, residual, nullptr, out, nullptr, nullptr, 0, s.Ci, s.Co, 0, s.Ci, 1}, stream);
 }
 int launch_pointwise_split_slope(const PointwiseShape &s, const void *x, const void *weight, const void *bias, const void *residual,
-                                 const void *grad, void *dz, float *sums, cudaStream_t stream)
+                                 const void *grad, void *dz, void *rest, float *sums, cudaStream_t stream)
 {
     SplitPlan plan;
     plan_split(s, s.Ci, s.Co, &plan);
-    return launch_split<SLOPE>(s, plan, {x, weight, bias, residual, grad, dz, sums, 0, s.Ci, s.Co, 0, s.Ci, 1}, stream);
+    return launch_split<SLOPE>(s, plan, {x, weight, bias, residual, grad, dz, rest, sums, 0, s.Ci, s.Co, 0, s.Ci, 1}, stream);
 }
-int launch_pointwise_split_input(const PointwiseShape &s, const void *dz, const void *weight, void *grad_input, cudaStream_t stream)
+int launch_pointwise_split_input(const PointwiseShape &s, const void *dz, const void *rest, const void *weight, void *grad_input,
+                                 cudaStream_t stream)
 {
     SplitPlan plan;
     plan_split(s, s.Co, s.Ci, &plan);
-    return launch_split<INPUT>(s, plan, {dz, weight, nullptr, nullptr, nullptr, grad_input, nullptr, 0, s.Co, s.Ci, 0, 1, s.Ci}, stream);
+    return launch_split<INPUT>(s, plan, {dz, weight, nullptr, nullptr, nullptr, grad_input, const_cast<void *>(rest), nullptr, 0, s.Co, s.Ci, 0, 1, s.Ci}, stream);
 }
 
 // ---- grad_weight: rows of pointwise_partial_stride() floats, to be added
@@ -881,7 +902,7 @@ struct WeightSplitPlan {
     int64_t slices, per;
     uint32_t smem;
 };
-bool plan_weight_split(const PointwiseShape &s, WeightSplitPlan *plan)
+bool plan_weight_split(const PointwiseShape &s, int sources, WeightSplitPlan *plan)
 {
     const int parts = s.io_kind == BC_IO_F32 ? 3 : 1, Ci = std::max(1, s.Ci);      // (no input channels: the sums of dz alone)
     const int64_t P = s.last ? s.N * s.P : s.P, samples = s.last ? 1 : s.N;
@@ -898,7 +919,7 @@ bool plan_weight_split(const PointwiseShape &s, WeightSplitPlan *plan)
         auto fits = [&](int stages, int slots) {
             r.stages = stages;
             r.slots = slots;
-            r.smem = WeightSplitLayout{r.rows, r.bn, stages, slots, parts, s.last}.bytes();
+            r.smem = WeightSplitLayout{r.rows, r.bn, stages, slots, parts, sources, s.last}.bytes();
             return r.smem <= kMostShared - 2048;
         };
         if (parts == 3 ? fits(2, 2) || fits(2, 1) : fits(4, 0) || fits(3, 0) || fits(2, 0)) break;
@@ -915,17 +936,19 @@ bool plan_weight_split(const PointwiseShape &s, WeightSplitPlan *plan)
 }
 }  // namespace
 
-int pointwise_split_weight_splits(const PointwiseShape &s)
+int pointwise_split_weight_splits(const PointwiseShape &s, bool rest)
 {
     WeightSplitPlan plan;
-    return plan_weight_split(s, &plan) ? plan.splits : 0;
+    return plan_weight_split(s, rest ? 2 : 1, &plan) ? plan.splits : 0;
 }
-int launch_pointwise_split_weight(const PointwiseShape &s, const void *dz, const void *x, float *partial, bool sums, cudaStream_t stream)
+int launch_pointwise_split_weight(const PointwiseShape &s, const void *dz, const void *rest, const void *x, float *partial, bool sums,
+                                  cudaStream_t stream)
 {
     WeightSplitPlan plan;
-    plan_weight_split(s, &plan);
+    plan_weight_split(s, rest ? 2 : 1, &plan);
     WeightSplit q{};
     q.dz = dz;
+    q.rest = rest;
     q.x = x;
     q.partial = partial;
     q.P = s.last ? s.N * s.P : s.P;

@@ -257,7 +257,8 @@ int bc_pack_parameters(const void *x_min, const void *x_max, const void *y_min, 
  *
  * Tensors of N samples of `pixels` = h*w pixels: planes (N, C, pixels), or channels last (N, pixels, C) with
  * channels_last nonzero, all tensors of a call alike; every array of type io_kind (BC_IO_*) unless stated.  Sums, statistics
- * and products are float; results are rounded once.  activation: BC_ACT_*, GELU is the one with the error function.
+ * and products are float; results are rounded once (a 16-bit gradient behind an activation enters its products as two
+ * values of its type, its rounding and what that leaves).  activation: BC_ACT_*, GELU is the one with the error function.
  * Workspaces: 256-byte aligned, may be NULL where the query says 0; calls that are not ordered by a stream need
  * workspaces of their own.  Sums are taken in a fixed order: the same call gives the same bits. */
 enum { BC_ACT_NONE = 0, BC_ACT_RELU = 1, BC_ACT_SILU = 2, BC_ACT_GELU = 3 };

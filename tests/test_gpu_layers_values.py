@@ -1,0 +1,60 @@
+"""pointwise_conv2d and group_norm where values, sums or strides are unusual: slopes that enter products.
+Definitions in 64 bits and tolerances as in test_gpu_layers.py."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_layers import TINY, U, bc, maps, slope64, slope_error, within  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+LAYOUTS = pytest.mark.parametrize("last", [False, True], ids=["planes", "last"])
+NARROW = [torch.float16, torch.bfloat16]
+
+
+# ---- products of a slope ---------------------------------------------------------------------------------
+
+# one product a value, tiles of TMA (several slices of channels, one CTA an SM and two), rows that it does not take, weights
+# that only multiply-adds hold (of grad_input; of the slope)
+SLOPES = [(2, 8, 1, 4, 6), (2, 1, 1, 5, 7), (2, 16, 24, 8, 16), (1, 256, 72, 8, 16), (1, 64, 200, 9, 16), (2, 17, 33, 3, 43), (1, 60, 130, 7, 9),
+          (1, 40, 2500, 4, 8), (1, 41, 2500, 3, 7), (1, 4609, 24, 3, 7), (300, 24, 40, 1, 1)]
+
+
+@LAYOUTS
+@pytest.mark.parametrize("dtype", NARROW, ids=str)
+@pytest.mark.parametrize("shape", SLOPES, ids=str)
+def test_a_slope_enters_its_products_unrounded(bc, shape, dtype, last):  # noqa: F811
+    """dz = grad * slope is not rounded to the tensors' type before grad_input, grad_weight and grad_bias are made of it: it
+    is held in two parts of that type, the second a rounding of u of what the first leaves (u |dz|)."""
+    N, Ci, Co, h, w = shape
+    u, gen = U[dtype], torch.Generator(device="cuda").manual_seed(Ci + Co)
+    for act in ("silu", "gelu", "relu"):
+        x, r, g = maps(gen, (N, Ci, h, w), dtype, last), maps(gen, (N, Co, h, w), dtype, last), maps(gen, (N, Co, h, w), dtype, last)
+        weight = (torch.randn(Co, Ci, device="cuda", generator=gen) / math.sqrt(Ci)).to(dtype)
+        bias = torch.randn(Co, device="cuda", generator=gen).to(dtype)
+        X, W = x.double().permute(0, 2, 3, 1).reshape(-1, Ci), weight.double()
+        R, G = (t.double().permute(0, 2, 3, 1).reshape(-1, Co) for t in (r, g))
+        z = X @ W.T + bias.double() + R
+        dz_arg = (Ci + 2) * 2.0 ** -23 * (X.abs() @ W.abs().T + bias.double().abs() + R.abs())
+        dz = G * slope64(z, act)
+        near = G.abs() * slope_error(z, dz_arg, act) + 2.0 ** -23 * dz.abs()
+        off = near + u * u * dz.abs() + TINY[dtype]
+        # two parts in every product: twice the additions
+        rows, size = X.shape[0], dz.abs() + off
+        planes = lambda t: t.reshape(N, h, w, -1).permute(0, 3, 1, 2)  # noqa: E731
+        for of_residual in (True, False):      # (dz is the residual's gradient as well, or nobody's)
+            leaves = [t.detach().requires_grad_() for t in (x, weight, bias)]
+            rr = r.detach().requires_grad_(of_residual)
+            out = bc.pointwise_conv2d(*leaves, activation=act, residual=rr)
+            got = torch.autograd.grad(out, leaves + [rr] * of_residual, g)
+            within(got[0], planes(dz @ W), planes(off @ W.abs() + (2 * Co + 2) * 2.0 ** -23 * (size @ W.abs())), dtype, "grad_input")
+            within(got[1], dz.T @ X, off.T @ X.abs() + (2 * rows + 2) * 2.0 ** -23 * (size.T @ X.abs()), dtype, "grad_weight")
+            within(got[2], dz.sum(0), off.sum(0) + (2 * rows + 2) * 2.0 ** -23 * size.sum(0), dtype, "grad_bias")
+            if of_residual:
+                within(got[3], planes(dz), planes(near), dtype, "grad_residual")
+
+
+def test_no_wait_has_expired():
+    from box_convolution import _cabi
+    assert _cabi.wait_timeouts() == 0
