@@ -14,22 +14,25 @@ namespace bc {
 // Which part a launch does: both readings (a cluster), the sums, the results.
 enum { NORM_WHOLE, NORM_SUMS, NORM_RESULTS };
 
-// Count, mean and sum of squares about the mean: two of them make the third's without cancellation wherever the mean lies.
+// Count, mean and variance: two of them make the third's without cancellation wherever the mean lies.  (The variance and not
+// the sum of squares, which may be no float where the variance is one.)
 struct Moments {
-    float n, mean, m2;
+    float n, mean, var;
 };
 __device__ __forceinline__ Moments merged(const Moments &a, const Moments &b)
 {
+    // (nothing on either side leaves the other as it is: its mean's square, which has no part in this, may be no float)
     if (a.n == 0.f) return b;
+    if (b.n == 0.f) return a;
     const float n = a.n + b.n, d = b.mean - a.mean, share = __fdividef(b.n, n);
-    return {n, fmaf(d, share, a.mean), a.m2 + b.m2 + d * d * a.n * share};
+    return {n, fmaf(d, share, a.mean), fmaf(share, fmaf(d * d, 1.f - share, b.var - a.var), a.var)};
 }
 __device__ __forceinline__ Moments warp_merged(Moments v)
 {
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
         const Moments w{__shfl_down_sync(0xffffffffu, v.n, o), __shfl_down_sync(0xffffffffu, v.mean, o),
-                        __shfl_down_sync(0xffffffffu, v.m2, o)};
+                        __shfl_down_sync(0xffffffffu, v.var, o)};
         v = merged(v, w);
     }
     return v;      // lane 0's

@@ -163,11 +163,12 @@ __global__ void __launch_bounds__(THREADS) norm_rows_forward_kernel(const T *__r
         // Neighbours of a group become one in the thread, where vectors and groups end together: their counts are equal.
         const int run = s.C % V == 0 && (D % V == 0 || V % D == 0) ? min(D, V) : 1;
         if (threadIdx.x < plan.active) {
-            float mj[V], qj[V];
+            float mj[V], qj[V];      // means and variances
+            const f2_t share = both(have > 0.f ? __frcp_rn(have) : 0.f);
 #pragma unroll
             for (int j = 0; j < V; j += 2) {
                 unpack2(mean[j / 2], mj[j], mj[j + 1]);
-                unpack2(m2[j / 2], qj[j], qj[j + 1]);
+                unpack2(mul2(m2[j / 2], share), qj[j], qj[j + 1]);
             }
 #pragma unroll
             for (int w = 1; w < V; w *= 2)
@@ -176,7 +177,7 @@ __global__ void __launch_bounds__(THREADS) norm_rows_forward_kernel(const T *__r
                     for (int j = 0; j < V; j += 2 * w) {
                         const float d = mj[j + w] - mj[j];
                         mj[j] = fmaf(0.5f, d, mj[j]);
-                        qj[j] += fmaf(d * d, 0.5f * w * have, qj[j + w]);
+                        qj[j] = fmaf(0.25f * d, d, 0.5f * (qj[j] + qj[j + w]));
                     }
 #pragma unroll
             for (int j = 0; j < V; ++j)
@@ -206,7 +207,7 @@ __global__ void __launch_bounds__(THREADS) norm_rows_forward_kernel(const T *__r
                 float *to = STEP == NORM_SUMS ? ws + ((unit * plan.k + rank) * groups + g) * 3 : moments + 3 * g;
                 to[0] = m.n;
                 to[1] = m.mean;
-                to[2] = m.m2;
+                to[2] = m.var;
             }
         }
         if (STEP == NORM_SUMS) return;
@@ -225,8 +226,8 @@ __global__ void __launch_bounds__(THREADS) norm_rows_forward_kernel(const T *__r
             }
             for (int o = 1; o < plan.k; o *= 2)
                 m = merged(m, {__shfl_down_sync(0xffffffffu, m.n, o), __shfl_down_sync(0xffffffffu, m.mean, o),
-                               __shfl_down_sync(0xffffffffu, m.m2, o)});
-            if (g < groups && i == g * plan.k) results[g] = make_float2(m.mean, rsqrtf(__fdiv_rn(m.m2, m.n) + s.eps));
+                               __shfl_down_sync(0xffffffffu, m.var, o)});
+            if (g < groups && i == g * plan.k) results[g] = make_float2(m.mean, rsqrtf(m.var + s.eps));
         }
         if (plan.k > 1) cluster_sync();      // (nobody leaves while its moments are read)
         else __syncthreads();
@@ -238,7 +239,7 @@ __global__ void __launch_bounds__(THREADS) norm_rows_forward_kernel(const T *__r
                 m = merged(m, {__ldg(from), __ldg(from + 1), __ldg(from + 2)});
             }
             m = warp_merged(m);
-            if (lane == 0) results[g] = make_float2(m.mean, rsqrtf(__fdiv_rn(m.m2, m.n) + s.eps));
+            if (lane == 0) results[g] = make_float2(m.mean, rsqrtf(m.var + s.eps));
         }
         __syncthreads();
     }

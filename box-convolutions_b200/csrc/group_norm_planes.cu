@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(512, 2) norm_planes_forward_kernel(const T *__
                         squares = fma2(d, d, squares);
                     }
                     unpack2(squares, a, b);
-                    m = merged(m, {(float)V, mean, a + b});
+                    m = merged(m, {(float)V, mean, (a + b) * (1.f / V)});
                 }
             });
             const int64_t at = piece.edge(lane);
@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(512, 2) norm_planes_forward_kernel(const T *__
         if (lane == 0) {
             warp_moments[warp][0] = m.n;
             warp_moments[warp][1] = m.mean;
-            warp_moments[warp][2] = m.m2;
+            warp_moments[warp][2] = m.var;
         }
         __syncthreads();
         if (threadIdx.x == 0) {
@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(512, 2) norm_planes_forward_kernel(const T *__
             float *to = STEP == NORM_SUMS ? ws + (unit * plan.k + rank) * 3 : own;
             to[0] = m.n;
             to[1] = m.mean;
-            to[2] = m.m2;
+            to[2] = m.var;
         }
         if (STEP == NORM_SUMS) return;
     }
@@ -120,7 +120,7 @@ __global__ void __launch_bounds__(512, 2) norm_planes_forward_kernel(const T *__
                     m = merged(m, {cluster_load(at), cluster_load(at + 4), cluster_load(at + 8)});
                 }
             }
-            result = make_float2(m.mean, rsqrtf(__fdiv_rn(m.m2, m.n) + s.eps));
+            result = make_float2(m.mean, rsqrtf(m.var + s.eps));
         }
         if (plan.k > 1) cluster_sync();      // (nobody leaves while its moments are read)
         else __syncthreads();
@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(512, 2) norm_planes_forward_kernel(const T *__
                 m = merged(m, {__ldg(from), __ldg(from + 1), __ldg(from + 2)});
             }
             m = warp_merged(m);
-            if (lane == 0) result = make_float2(m.mean, rsqrtf(__fdiv_rn(m.m2, m.n) + s.eps));
+            if (lane == 0) result = make_float2(m.mean, rsqrtf(m.var + s.eps));
         }
         __syncthreads();
     }

@@ -1,11 +1,11 @@
-"""pointwise_conv2d and group_norm where values, sums or strides are unusual: slopes that enter products.
+"""pointwise_conv2d and group_norm where values, sums or strides are unusual: slopes that enter products, groups far from zero.
 Definitions in 64 bits and tolerances as in test_gpu_layers.py."""
 import math
 
 import pytest
 import torch
 
-from test_gpu_layers import TINY, U, bc, maps, slope64, slope_error, within  # noqa: F401
+from test_gpu_layers import TINY, U, bc, check_norm, maps, slope64, slope_error, within  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -53,6 +53,27 @@ def test_a_slope_enters_its_products_unrounded(bc, shape, dtype, last):  # noqa:
             within(got[2], dz.sum(0), off.sum(0) + (2 * rows + 2) * 2.0 ** -23 * size.sum(0), dtype, "grad_bias")
             if of_residual:
                 within(got[3], planes(dz), planes(near), dtype, "grad_residual")
+
+
+# ---- groups far from zero --------------------------------------------------------------------------------
+
+@LAYOUTS
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("shape", [(2, 8, 2, 8, 8), (2, 8, 8, 8, 8), (1, 64, 16, 2, 2), (1, 16, 1, 1, 3), (3, 24, 3, 5, 7), (1, 32, 1, 64, 96),
+                                   (1, 8, 1, 250, 251), (2, 20, 4, 16, 24), (1, 2048, 2, 1, 3)], ids=str)
+def test_norm_of_groups_whose_squares_are_near_the_largest(bc, shape, dtype, last):  # noqa: F811
+    """Means of 1e19 with a spread of 1e17, of either sign: mean^2 times a few values is no float, the sum of squares about the
+    mean is.  Lanes, warps and CTAs without a value take part in such a group as well."""
+    N, C, G, h, w = shape
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    g = maps(gen, (N, C, h, w), dtype, last)
+    for sign in (1.0, -1.0):
+        x = maps(gen, (N, C, h, w), dtype, last, 1e17, sign * 1e19)
+        check_norm(bc, x, G, None, None, g, "silu" if sign > 0 else None)
+    # one value far off among many
+    x = maps(gen, (N, C, h, w), dtype, last)
+    x[0, 0, 0, 0] = 1e18
+    check_norm(bc, x, G, None, None, g, None)
 
 
 def test_no_wait_has_expired():
