@@ -1,11 +1,11 @@
-"""pointwise_conv2d and group_norm where values, sums or strides are unusual: slopes that enter products, groups far from zero.
+"""pointwise_conv2d and group_norm where values, sums or strides are unusual: slopes that enter products, groups far from zero, tails of SiLU.
 Definitions in 64 bits and tolerances as in test_gpu_layers.py."""
 import math
 
 import pytest
 import torch
 
-from test_gpu_layers import TINY, U, bc, check_norm, maps, slope64, slope_error, within  # noqa: F401
+from test_gpu_layers import DTYPES, FN, TINY, U, act64, bc, check_norm, maps, slope64, slope_error, within  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -74,6 +74,50 @@ def test_norm_of_groups_whose_squares_are_near_the_largest(bc, shape, dtype, las
     x = maps(gen, (N, C, h, w), dtype, last)
     x[0, 0, 0, 0] = 1e18
     check_norm(bc, x, G, None, None, g, None)
+
+
+# ---- SiLU far below zero ---------------------------------------------------------------------------------
+
+SMALLEST = {torch.float32: 2.0 ** -149, torch.float16: 2.0 ** -24, torch.bfloat16: 2.0 ** -133}      # steps of subnormal numbers
+
+
+def close(got, ref, relative, what):
+    """Within a relative error, and a step of the type's smallest numbers."""
+    off, bound = (got.double() - ref).abs(), relative * ref.abs() + 1.01 * SMALLEST[got.dtype]
+    bad = ~(off <= bound)
+    assert not bad.any(), "%s: %d of %d; first %r instead of %r" % (what, int(bad.sum()), bad.numel(), float(got[bad][0]), float(ref[bad][0]))
+
+
+@LAYOUTS
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("count", [512, 509])
+def test_silu_keeps_its_tails(bc, dtype, last, count):  # noqa: F811
+    """z from -104 to 104, relative errors of value and slope: sigmoid(z) is a normal number down to -87.3 and z sigmoid(z) to
+    -91.8.  float: half a step of its own, 2^-24, in each of the dozen operations, 2^-22 in the power of two: 2^-20.  16-bit: u,
+    that, and an exponent z log2(e) of at most 151 that is rounded to half of 2^-16, times log(2): 2^-17."""
+    z = torch.linspace(-104, 104, count, device="cuda").to(dtype)
+    ref, slope = act64(z.double(), "silu"), slope64(z.double(), "silu")
+    # what is there of a slope near its zero (-1.278): the error of its argument, none, and of its terms
+    parts = torch.sigmoid(z.double()) * (1 + z.double().abs() * torch.sigmoid(-z.double()))
+    tol = FN + (U[dtype] + 2.0 ** -17 if dtype != torch.float32 else 0)
+    # z as a residual, and its slope as the residual's gradient
+    shape = (1, 8, count, 1) if not last else (1, 8, 1, count)
+    r = z.view(shape[2:]).expand(shape).contiguous(memory_format=torch.channels_last if last else torch.contiguous_format).requires_grad_()
+    x, w = torch.zeros(1, 8, *shape[2:], device="cuda", dtype=dtype), torch.zeros(8, 8, device="cuda", dtype=dtype)
+    out = bc.pointwise_conv2d(x.contiguous(memory_format=torch.channels_last) if last else x, w, activation="silu", residual=r)
+    close(out[0].flatten(1), ref.expand(8, -1), tol, "pointwise")
+    grad = torch.autograd.grad(out, r, torch.ones_like(out))[0]
+    assert ((grad[0].flatten(1).double() - slope).abs() <= tol * parts + 1.01 * SMALLEST[dtype]).all()
+    # z as a normalisation's bias, and its slope as the gradient of that
+    x = torch.randn(1, count, 1, 1, device="cuda").to(dtype)
+    for gx in (x, x.expand(1, count, 1, 9).contiguous(memory_format=torch.channels_last if last else torch.contiguous_format)):
+        b = z.clone().requires_grad_()
+        out = bc.group_norm(gx, 1, torch.zeros_like(z), b, activation="silu")
+        close(out[0].flatten(1), ref[:, None].expand(-1, gx.shape[3]), tol, "group_norm")
+        g = torch.zeros_like(out)
+        g[..., 0] = 1
+        grad = torch.autograd.grad(out, b, g)[0]
+        assert ((grad.double() - slope).abs() <= tol * parts + 1.01 * SMALLEST[dtype]).all()
 
 
 def test_no_wait_has_expired():
