@@ -92,6 +92,8 @@ __device__ __forceinline__ void fold(float (&v)[N], int lane, int mask, int half
 }
 
 // A wait whose expiry ends all further ones of the thread: a lost arrival is counted (bc_wait_timeouts), and nothing hangs.
+// Threads learn of a loss each for itself, so one that works alone may leave its loop on it; whoever shares barriers (of a
+// warp, a pair, a group) goes round to the loop's end, where further waits return at once and values mean nothing.
 struct Waiter {
     bool lost = false;
     __device__ __forceinline__ bool operator()(uint32_t mbar, uint32_t parity)
@@ -103,7 +105,7 @@ struct Waiter {
         return false;
     }
 };
-// Before a CTA that has lost an arrival leaves: time for its copies in flight, far more than any takes.
+// Before a CTA that has lost an arrival leaves: time for its copies and products in flight, far more than any takes.
 __device__ __forceinline__ void let_copies_land()
 {
     for (const long long t0 = clock64(); clock64() - t0 < 20000000LL;) __nanosleep(1000);

@@ -292,7 +292,6 @@ __global__ void __launch_bounds__(32 * (kEpilogue * PAIR + 2), PAIR == 1 ? 2 : 1
             tmem_release();
             __syncwarp();
             if (lane == 0) mbar_arrive(drained + 8 * set);
-            if (wait.lost) break;
             if (set ^= 1; set == 0) set_phase ^= 1;
         }
     }
@@ -429,7 +428,7 @@ __global__ void __launch_bounds__(kWeightThreads) pointwise_weight_mma_kernel(co
             uint32_t stage = 0, phase = 0;
             const int group = threadIdx.x & 15, pixel = threadIdx.x >> 4;
             for (int64_t slice = first; slice < last; ++slice) {
-                if (!wait(full + 8 * stage, phase)) break;
+                wait(full + 8 * stage, phase);
                 const char *a = smem + stage * lay.stage();
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
@@ -464,7 +463,7 @@ __global__ void __launch_bounds__(kWeightThreads) pointwise_weight_mma_kernel(co
                 partial[(int64_t)q.Co * q.Ci + o0 + threadIdx.x] = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
             }
         }
-        if (!wait.lost) wait(ready, 0);
+        wait(ready, 0);
         __syncwarp();
         tmem_acquire();
         const int o = o0 + warp * 32 + lane;

@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const Spli
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] = *reinterpret_cast<const float4 *>(own + 4096 * j);
             copy();
-            if (!wait(empty + 8 * stage, phase ^ 1)) break;
+            wait(empty + 8 * stage, phase ^ 1);
             char *to = smem + lay.ring() + stage * PARTS * kPart + (in & 4) * 2;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const Spli
                 const T *from = a + outer * (LAST ? (int64_t)q.K : q.P) + in;
                 if constexpr (PARTS == 1) raw_v[j] = load8<T, VEC>(from, inner);
             }
-            if (!wait(empty + 8 * stage, phase ^ 1)) break;
+            wait(empty + 8 * stage, phase ^ 1);
             char *to = smem + lay.ring() + stage * PARTS * kPart;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -439,10 +439,10 @@ __global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const Spli
             tmem_release();
             __syncwarp();
             if (lane == 0) mbar_arrive(drained + 8 * set);
-            if (wait.lost) break;
             if (set ^= 1; set == 0) set_phase ^= 1;
         }
     }
+    if (wait.lost) let_copies_land();
     __syncwarp();
     tmem_release();
     __syncthreads();
@@ -561,7 +561,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
         uint32_t stage = 0, phase = 0;
         for (int slice = first; slice < last; ++slice) {
             copies_wait(q.slots);
-            if (!wait(empty + 8 * stage, phase ^ 1)) break;
+            wait(empty + 8 * stage, phase ^ 1);
             char *const dz_to = smem + stage * lay.stage(), *const x_to = dz_to + lay.x_at();
             const char *from = own + (q.slots > 1 ? (uint32_t)(slice - first & 1) * slot_bytes : 0);
 #pragma unroll
@@ -652,7 +652,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
                 }
                 if (!waited) {
                     waited = true;
-                    if (!wait(empty + 8 * stage, phase ^ 1)) break;
+                    wait(empty + 8 * stage, phase ^ 1);
                 }
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
@@ -675,7 +675,6 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
                     }
                 }
             }
-            if (wait.lost) break;
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(full + 8 * stage);
@@ -786,6 +785,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
                     if (i0 + b + j < q.Ci) partial[(int64_t)o * q.Ci + i0 + b + j] = v[j];
         }
     }
+    if (wait.lost) let_copies_land();
     __syncwarp();
     tmem_release();
     __syncthreads();
