@@ -41,6 +41,13 @@ __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t
     asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
                  ::"r"(d), "l"(a), "l"(b), "r"(instruction), "r"((uint32_t)add) : "memory");
 }
+// The same of operands in two words, the address in the lower one.
+__device__ __forceinline__ void mma(uint32_t d, uint32_t a, uint32_t a_high, uint32_t b, uint32_t b_high, uint32_t instruction, bool add)
+{
+    asm volatile("{\n .reg .pred p;\n .reg .b64 x, y;\n setp.ne.b32 p, %6, 0;\n mov.b64 x, {%1, %2};\n mov.b64 y, {%3, %4};\n"
+                 " tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %5, p;\n}"
+                 ::"r"(d), "r"(a), "r"(a_high), "r"(b), "r"(b_high), "r"(instruction), "r"((uint32_t)add) : "memory");
+}
 // Arrives once everything issued so far by this thread is done (and has been read).
 __device__ __forceinline__ void mma_commit(uint32_t mbar)
 {
@@ -63,6 +70,20 @@ __device__ __forceinline__ void tile_load(uint32_t dst, const CUtensorMap *map, 
 }
 __device__ __forceinline__ void map_prefetch(const CUtensorMap *map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 
+// The tensor memory of such sums: one or two sets of accumulators of `columns` (a power of two), two where there is room, and
+// behind them `width` columns of totals.
+struct SumColumns {
+    int sets, all;
+};
+inline SumColumns sum_columns(bool several, int columns, int width)
+{
+    if (!several) return {1, columns};
+    const int sets = 2 * columns + width <= 512 ? 2 : 1;
+    int all = 32;
+    while (all < sets * columns + width) all *= 2;
+    return {sets, all};
+}
+
 // 16 accumulators of each of the warp's lanes.
 __device__ __forceinline__ void accumulators16(uint32_t at, float (&v)[16])
 {
@@ -78,6 +99,20 @@ __device__ __forceinline__ void accumulators16(uint32_t at, float (&v)[16])
     }
 }
 
+__device__ __forceinline__ void store16(uint32_t at, const float (&v)[16])
+{
+#pragma unroll
+    for (int i = 0; i < 16; i += 8)
+        tmem_store8(at + i, make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]), make_float4(v[i + 4], v[i + 5], v[i + 6], v[i + 7]));
+}
+__device__ __forceinline__ void add16(uint32_t at, float (&v)[16])
+{
+    float u[16];
+    accumulators16(at, u);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] += u[j];
+}
+
 // Halves the values of the two lanes that `mask` tells apart: the one without the bit goes on with the lower half of both's sums.
 template <int N>
 __device__ __forceinline__ void fold(float (&v)[N], int lane, int mask, int half)
@@ -91,9 +126,28 @@ __device__ __forceinline__ void fold(float (&v)[N], int lane, int mask, int half
         }
 }
 
+// Slices of 64 pixels that an accumulator of grad_weight takes before its sum goes on to another part of tensor memory.  An
+// accumulator rounds towards zero with every addition (two an instruction of 16 pixels, as measured: 28340 instructions lost 2.8e-3
+// of a sum of one sign), which adds up, so a sum is of 128 additions for float tensors and 512 for 16-bit ones: they lose 2^-17
+// and 2^-15 of a sum that grows evenly, whatever the number of pixels.  What follows is rounded to nearest: kMostSums of them in
+// a row of partial sums, and the rows in double.  Kernels, one accumulator throughout and so: (64,128->128,64,128) f32 291 us
+// and 289, channels last 504 and 516; (1,16->16,2048,2048) f32 432 and 513; (16,128->32,64,128) f32 43.5 and 47.6.
+template <typename T>
+constexpr int kSumSlices = sizeof(T) == 4 ? 16 : 64;
+template <typename T>
+constexpr int kMostSums = sizeof(T) == 4 ? 16 : 64;
+// Slices of a CTA, `most` or less: a CTA an SM with four at least, else as few rounds of them as will do.
+inline int64_t slices_of_split(int64_t all, int64_t tiles, int64_t most)
+{
+    const int64_t walkers = std::max<int64_t>(1, 148 / tiles), per = std::max<int64_t>(std::min<int64_t>(4, all), (all + walkers - 1) / walkers);
+    const int64_t rounds = (per + most - 1) / most;
+    return rounds > 1 ? (all + walkers * rounds - 1) / (walkers * rounds) : per;
+}
+
 // A wait whose expiry ends all further ones of the thread: a lost arrival is counted (bc_wait_timeouts), and nothing hangs.
-// Threads learn of a loss each for itself, so one that works alone may leave its loop on it; whoever shares barriers (of a
-// warp, a pair, a group) goes round to the loop's end, where further waits return at once and values mean nothing.
+// Threads learn of a loss each for itself, so one that works alone may leave its loop on it, and a warp as a whole whose loop
+// has no other warps' barriers; whoever shares those goes round to the loop's end, where further waits return at once and
+// values mean nothing.
 struct Waiter {
     bool lost = false;
     __device__ __forceinline__ bool operator()(uint32_t mbar, uint32_t parity)

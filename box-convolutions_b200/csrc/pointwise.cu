@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(kThreads, BN == 64 ? 3 : 4) pointwise_kernel(P
     }
 }
 
-// Rows of partial sums, added in a fixed order, rounded once: `count` columns, `stride` floats from row to row.
+// Rows of partial sums, added in a fixed order (in double: there may be thousands), rounded once: `count` columns, `stride` floats from row to row.
 struct Partials {
     const float *from;
     int64_t stride, count;
@@ -270,11 +270,11 @@ constexpr int kFinishRows = 8;
 template <typename T>
 __global__ void __launch_bounds__(32 * kFinishRows) pointwise_finish_kernel(Partials weights, Partials sums, unsigned blocks)
 {
-    __shared__ float part[kFinishRows][32];
+    __shared__ double part[kFinishRows][32];
     const Partials &q = blockIdx.x < blocks ? weights : sums;
     const int64_t e = (int64_t)(blockIdx.x < blocks ? blockIdx.x : blockIdx.x - blocks) * 32 + threadIdx.x;
     grid_dependency_wait();
-    float v = 0.f;
+    double v = 0;
     if (e < q.count) {
 #pragma unroll 8
         for (int i = threadIdx.y; i < q.rows; i += kFinishRows) v += q.from[i * q.stride + e];
@@ -283,7 +283,7 @@ __global__ void __launch_bounds__(32 * kFinishRows) pointwise_finish_kernel(Part
     __syncthreads();
     if (threadIdx.y || e >= q.count) return;
     for (int i = 1; i < kFinishRows; ++i) v += part[i][threadIdx.x];
-    static_cast<T *>(q.to)[e] = from_float<T>(v);
+    static_cast<T *>(q.to)[e] = from_float<T>((float)v);
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }

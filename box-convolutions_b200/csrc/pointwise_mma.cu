@@ -320,8 +320,8 @@ struct WeightMma {
     int64_t slices;          // of a sample
     int samples, Ci, Co;
     int tiles_i;
-    int bn, rows, stages, columns;      // input channels of a tile; rows of dz that are loaded (planes); ring; tensor memory
-    int parts;               // tensors that dz is the sum of
+    int bn, rows, stages, columns;      // input channels of a tile; rows of dz that are loaded (planes); ring; tensor memory of a set of sums
+    SumColumns sums_at;
     bool sums;
     uint32_t instruction;
 };
@@ -334,20 +334,20 @@ struct WeightLayout {
     __host__ __device__ uint32_t x_at() const { return parts * 2 * kBlockBytes; }
     __host__ __device__ uint32_t stage() const { return x_at() + x_bytes(); }
     __host__ __device__ uint32_t barriers() const { return stages * stage(); }
-    __host__ __device__ uint32_t bytes() const { return barriers() + (2 * stages + 1) * 8 + 8 + 1024; }
+    __host__ __device__ uint32_t bytes() const { return barriers() + (2 * stages + 4) * 8 + 8 + 1024; }
 };
 
-// Four warps of the epilogue also add up dz, from the slices as they pass, for grad_bias.
-template <typename T, bool LAST>
+// Four warps of the epilogue also add up dz, from the slices as they pass, for grad_bias.  PARTS: tensors that dz is the sum of.
+template <typename T, bool LAST, int PARTS>
 __global__ void __launch_bounds__(kWeightThreads) pointwise_weight_mma_kernel(const __grid_constant__ WeightMma q)
 {
     extern __shared__ char raw_smem[];
     __shared__ float part[128][9];
     const uint32_t raw = smem_u32(raw_smem), base = (raw + 1023) & ~1023u;
     char *smem = raw_smem + (base - raw);
-    const WeightLayout lay{q.bn, q.stages, q.parts, LAST};
-    const uint32_t full = base + lay.barriers(), empty = full + 8 * q.stages, ready = empty + 8 * q.stages;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + lay.barriers() + (2 * q.stages + 1) * 8);
+    const WeightLayout lay{q.bn, q.stages, PARTS, LAST};
+    const uint32_t full = base + lay.barriers(), empty = full + 8 * q.stages, ready = empty + 8 * q.stages, drained = ready + 16;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + lay.barriers() + (2 * q.stages + 4) * 8);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int tiles_o = (q.Co + 127) / 128, tiles = tiles_o * q.tiles_i;
     const int split = (int)(blockIdx.x / (unsigned)tiles), t = (int)blockIdx.x - split * tiles;
@@ -360,13 +360,16 @@ __global__ void __launch_bounds__(kWeightThreads) pointwise_weight_mma_kernel(co
             mbar_init(full + 8 * i, 1);
             mbar_init(empty + 8 * i, sums ? 5 : 1);
         }
-        mbar_init(ready, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(ready + 8 * i, 1);
+            mbar_init(drained + 8 * i, 4);
+        }
         fence_mbar_init();
         map_prefetch(&q.dz);
         map_prefetch(&q.x);
     }
     grid_dependency_wait();
-    if (warp == 5) tmem_alloc(tmem_slot, q.columns);
+    if (warp == 5) tmem_alloc(tmem_slot, q.sums_at.all);
     tmem_release();
     __syncthreads();
     tmem_acquire();
@@ -376,14 +379,15 @@ __global__ void __launch_bounds__(kWeightThreads) pointwise_weight_mma_kernel(co
     if (warp == 4) {
         if (lane == 0) {
             const int a_blocks = LAST ? (o0 + 64 < q.Co ? 2 : 1) : 0, b_blocks = (q.bn + 63) / 64;
-            const uint32_t bytes = q.parts * (LAST ? a_blocks * kBlockBytes : (uint32_t)q.rows * 128) + lay.x_bytes();
+            const uint32_t bytes = PARTS * (LAST ? a_blocks * kBlockBytes : (uint32_t)q.rows * 128) + lay.x_bytes();
             uint32_t stage = 0, phase = 0;
             for (int64_t slice = first; slice < last; ++slice) {
                 if (!wait(empty + 8 * stage, phase ^ 1)) break;
                 const int sample = (int)(slice / q.slices), p0 = (int)(slice - sample * q.slices) * 64;
                 const uint32_t a = base + stage * lay.stage(), b = a + lay.x_at(), bar = full + 8 * stage;
                 mbar_expect(bar, bytes);
-                for (int part = 0; part < q.parts; ++part) {
+#pragma unroll
+                for (int part = 0; part < PARTS; ++part) {
                     const CUtensorMap *dz = part ? &q.dz_rest : &q.dz;
                     const uint32_t to = a + part * 2 * kBlockBytes;
                     if (LAST)
@@ -401,55 +405,100 @@ __global__ void __launch_bounds__(kWeightThreads) pointwise_weight_mma_kernel(co
         }
     } else if (warp == 5) {
         if (lane == 0) {
-            uint32_t stage = 0, phase = 0;
-            for (int64_t slice = first; slice < last; ++slice) {
-                if (!wait(full + 8 * stage, phase)) break;
-                tmem_acquire();
-                const uint32_t a = base + stage * lay.stage(), b = a + lay.x_at();
+            constexpr uint32_t step = LAST ? 128 : 2;      // bytes from k to k
+            const uint64_t dz = LAST ? mn_major(base, 0, kBlockBytes) : k_major(base, 0), x = further(dz, lay.x_at());
+            const uint32_t a_high = (uint32_t)(dz >> 32), b_high = (uint32_t)(x >> 32);
+            uint32_t stage = 0, phase = 0, set = 0, set_phase = 0;
+            int64_t begin = first, end;      // a sum's slices
+            do {
+                end = min(last, begin + kSumSlices<T>);
+                if (!wait(drained + 8 * set, set_phase ^ 1)) break;
+                const uint32_t d = tmem + set * q.columns;
+                for (int64_t slice = begin; slice < end; ++slice) {
+                    if (!wait(full + 8 * stage, phase)) break;
+                    tmem_acquire();
+                    const uint32_t at = stage * lay.stage() >> 4, a = (uint32_t)dz + at, b = (uint32_t)x + at;
 #pragma unroll
-                for (int k = 0; k < 64; k += 16) {
-                    const uint64_t x = LAST ? mn_major(b, k, kBlockBytes) : k_major(b, k), dz = LAST ? mn_major(a, k, kBlockBytes) : k_major(a, k);
-                    mma(tmem, dz, x, q.instruction, slice > first || k);
-                    if (q.parts == 2) mma(tmem, further(dz, 2 * kBlockBytes), x, q.instruction, true);
+                    for (int k = 0; k < 64; k += 16) {
+                        mma(d, a + (step * k >> 4), a_high, b + (step * k >> 4), b_high, q.instruction, slice > begin || k);
+                        if (PARTS == 2) mma(d, a + (2 * kBlockBytes + step * k >> 4), a_high, b + (step * k >> 4), b_high, q.instruction, true);
+                    }
+                    mma_commit(empty + 8 * stage);
+                    if (++stage == (uint32_t)q.stages) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
                 }
-                mma_commit(empty + 8 * stage);
-                if (++stage == (uint32_t)q.stages) {
-                    stage = 0;
-                    phase ^= 1;
+                if (wait.lost) break;
+                mma_commit(ready + 8 * set);
+                if (++set == (uint32_t)q.sums_at.sets) {
+                    set = 0;
+                    set_phase ^= 1;
                 }
-            }
-            if (!wait.lost) mma_commit(ready);
+            } while ((begin = end) < last);
         }
     } else {
         float *partial = q.partial + split * pointwise_partial_stride(q.Co, q.Ci);
-        if (sums) {
+        const int o = o0 + warp * 32 + lane, group = threadIdx.x & 15, pixel = threadIdx.x >> 4;
+        float total[8] = {};
+        uint32_t stage = 0, phase = 0, set = 0, set_phase = 0;
+        for (int64_t from = first; from < last; from += kSumSlices<T>) {
             // planes: a thread a channel, its 64 pixels.  last: a thread 8 channels of 8 pixels.
-            float total[8] = {};
-            uint32_t stage = 0, phase = 0;
-            const int group = threadIdx.x & 15, pixel = threadIdx.x >> 4;
-            for (int64_t slice = first; slice < last; ++slice) {
-                wait(full + 8 * stage, phase);
-                const char *a = smem + stage * lay.stage();
+            float sum[8] = {};
+            if (sums)
+                for (int64_t slice = from; slice < min(last, from + kSumSlices<T>); ++slice) {
+                    wait(full + 8 * stage, phase);
+                    const char *a = smem + stage * lay.stage();
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int k = 8 * j + pixel;
-                    const char *from = LAST ? a + (group >> 3) * kBlockBytes + k * 128 + (((group & 7) ^ (k & 7)) << 4)
-                                            : a + threadIdx.x * 128 + ((j ^ (threadIdx.x & 7)) << 4);
-                    if (LAST ? o0 + 8 * group < q.Co : o0 + (int)threadIdx.x < q.Co)
-                        for (int part = 0; part < q.parts; ++part) {
-                            float v[8];
-                            unpack<T>(*reinterpret_cast<const uint4 *>(from + part * 2 * kBlockBytes), v);
+                    for (int j = 0; j < 8; ++j) {
+                        const int k = 8 * j + pixel;
+                        const char *at = LAST ? a + (group >> 3) * kBlockBytes + k * 128 + (((group & 7) ^ (k & 7)) << 4)
+                                                : a + threadIdx.x * 128 + ((j ^ (threadIdx.x & 7)) << 4);
+                        if (LAST ? o0 + 8 * group < q.Co : o0 + (int)threadIdx.x < q.Co)
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) total[i] += v[i];
-                        }
+                            for (int part = 0; part < PARTS; ++part) {
+                                float v[8];
+                                unpack<T>(*reinterpret_cast<const uint4 *>(at + part * 2 * kBlockBytes), v);
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) sum[i] += v[i];
+                            }
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(empty + 8 * stage);
+                    if (++stage == (uint32_t)q.stages) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
                 }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(empty + 8 * stage);
-                if (++stage == (uint32_t)q.stages) {
-                    stage = 0;
-                    phase ^= 1;
-                }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) total[i] += sum[i];
+            wait(ready + 8 * set, set_phase);
+            __syncwarp();
+            tmem_acquire();
+            const bool ends = last - from <= kSumSlices<T>;
+            for (int b = 0; b < q.bn; b += 16) {
+                const uint32_t at = tmem + b + ((uint32_t)warp << 21);
+                const uint32_t total = at + q.sums_at.sets * q.columns;
+                float v[16];
+                accumulators16(at + set * q.columns, v);
+                if (from > first) add16(total, v);
+                if (!ends) store16(total, v);
+                float *to = partial + (int64_t)o * q.Ci + i0 + b;
+#pragma unroll
+                for (int j = 0; j < 16; j += 4)
+                    if (ends && o < q.Co && i0 + b + j < q.Ci) *reinterpret_cast<float4 *>(to + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
             }
+            if (ends) break;
+            tmem_wait_store();
+            tmem_release();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(drained + 8 * set);
+            if (++set == (uint32_t)q.sums_at.sets) {
+                set = 0;
+                set_phase ^= 1;
+            }
+        }
+        if (sums) {
             if (LAST) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) part[8 * group + i][pixel] = total[i];
@@ -463,25 +512,12 @@ __global__ void __launch_bounds__(kWeightThreads) pointwise_weight_mma_kernel(co
                 partial[(int64_t)q.Co * q.Ci + o0 + threadIdx.x] = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
             }
         }
-        wait(ready, 0);
-        __syncwarp();
-        tmem_acquire();
-        const int o = o0 + warp * 32 + lane;
-        if (!__any_sync(0xffffffffu, wait.lost))
-            for (int b = 0; b < q.bn; b += 16) {
-                float v[16];
-                accumulators16(tmem + b + ((uint32_t)warp << 21), v);
-                float *to = partial + (int64_t)o * q.Ci + i0 + b;
-#pragma unroll
-                for (int j = 0; j < 16; j += 4)
-                    if (o < q.Co && i0 + b + j < q.Ci) *reinterpret_cast<float4 *>(to + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-            }
     }
     if (wait.lost) let_copies_land();
     __syncwarp();
     tmem_release();
     __syncthreads();
-    if (warp == 5) tmem_free(tmem, q.columns);
+    if (warp == 5) tmem_free(tmem, q.sums_at.all);
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -667,8 +703,7 @@ bool plan_weight(const PointwiseShape &s, int parts, WeightPlan *plan)
     }
     r.slices = ceil_div(P, 64);
     const int64_t all = r.slices * samples, tiles = (int64_t)r.tiles_o * r.tiles_i;
-    // a CTA an SM, of four slices at least
-    r.per = std::max<int64_t>(std::min<int64_t>(4, all), ceil_div(all, std::max<int64_t>(1, 148 / tiles)));
+    r.per = slices_of_split(all, tiles, kSumSlices<__half> * kMostSums<__half>);
     r.splits = (int)ceil_div(all, r.per);
     if (r.splits * tiles > INT32_MAX) return false;
     *plan = r;
@@ -708,7 +743,7 @@ int launch_pointwise_mma_weight(const PointwiseShape &s, const void *dz, const v
         const uint32_t last_box[2] = {64, 64}, box[3] = {64, rows, 1};
         return s.last ? make_map(to, from, bf16, 2, last_sizes, last_strides, last_box) : make_map(to, from, bf16, 3, sizes, strides, box);
     };
-    q.parts = rest ? 2 : 1;
+    q.sums_at = sum_columns(plan.per > kSumSlices<__half>, plan.columns, plan.bn);
     if (const int e = map(&q.dz, dz, s.Co, q.rows)) return e;
     if (rest)
         if (const int e = map(&q.dz_rest, rest, s.Co, q.rows)) return e;
@@ -719,8 +754,12 @@ int launch_pointwise_mma_weight(const PointwiseShape &s, const void *dz, const v
         launch_overlapped(kernel, (unsigned)(plan.splits * plan.tiles_o * plan.tiles_i), kWeightThreads, plan.smem, stream, q);
         return check_launch("pointwise_weight_mma_kernel");
     };
-    if (bf16) return s.last ? go(pointwise_weight_mma_kernel<__nv_bfloat16, true>) : go(pointwise_weight_mma_kernel<__nv_bfloat16, false>);
-    return s.last ? go(pointwise_weight_mma_kernel<__half, true>) : go(pointwise_weight_mma_kernel<__half, false>);
+    auto of = [&](auto t, auto parts) {
+        using T = decltype(t);
+        return s.last ? go(pointwise_weight_mma_kernel<T, true, decltype(parts)::value>) : go(pointwise_weight_mma_kernel<T, false, decltype(parts)::value>);
+    };
+    auto of_parts = [&](auto parts) { return bf16 ? of(__nv_bfloat16(), parts) : of(__half(), parts); };
+    return rest ? of_parts(std::integral_constant<int, 2>()) : of_parts(std::integral_constant<int, 1>());
 }
 
 int read_wait_timeouts_mma(int *count) { return read_wait_timeouts_here(count); }

@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const Spli
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] = *reinterpret_cast<const float4 *>(own + 4096 * j);
             copy();
-            wait(empty + 8 * stage, phase ^ 1);
+            if (__any_sync(0xffffffffu, !wait(empty + 8 * stage, phase ^ 1))) break;
             char *to = smem + lay.ring() + stage * PARTS * kPart + (in & 4) * 2;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const Spli
                 const T *from = a + outer * (LAST ? (int64_t)q.K : q.P) + in;
                 if constexpr (PARTS == 1) raw_v[j] = load8<T, VEC>(from, inner);
             }
-            wait(empty + 8 * stage, phase ^ 1);
+            if (__any_sync(0xffffffffu, !wait(empty + 8 * stage, phase ^ 1))) break;
             char *to = smem + lay.ring() + stage * PARTS * kPart;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -439,6 +439,7 @@ __global__ void __launch_bounds__(kThreads, 1) pointwise_split_kernel(const Spli
             tmem_release();
             __syncwarp();
             if (lane == 0) mbar_arrive(drained + 8 * set);
+            if (__any_sync(0xffffffffu, wait.lost)) break;
             if (set ^= 1; set == 0) set_phase ^= 1;
         }
     }
@@ -466,6 +467,7 @@ struct WeightSplit {
     int samples, Ci, Co;
     int tiles_i;
     int rows, bn, stages, slots, columns;      // output and input channels of a tile; ring; floats' slices on their way
+    SumColumns sums_at;
     bool sums;
     uint32_t instruction;
 };
@@ -482,7 +484,7 @@ struct WeightSplitLayout {
     __host__ __device__ uint32_t copies() const { return stages * stage() + 2 * kBlockBytes; }
     __host__ __device__ int each() const { return ((rows + bn) * 16 + kProducers - 1) / kProducers; }      // vectors of a thread
     __host__ __device__ uint32_t barriers() const { return copies() + slots * each() * 16 * kProducers; }
-    __host__ __device__ uint32_t bytes() const { return barriers() + (2 * stages + 1) * 8 + 8 + 1024; }
+    __host__ __device__ uint32_t bytes() const { return barriers() + (2 * stages + 4) * 8 + 8 + 1024; }
 };
 
 template <typename T, bool LAST, bool VEC>
@@ -495,8 +497,8 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
     char *smem = raw_smem + (base - raw);
     const int sources = PARTS == 1 && q.rest ? 2 : 1;
     const WeightSplitLayout lay{q.rows, q.bn, q.stages, q.slots, PARTS, sources, LAST};
-    const uint32_t full = base + lay.barriers(), empty = full + 8 * q.stages, ready = empty + 8 * q.stages;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + lay.barriers() + (2 * q.stages + 1) * 8);
+    const uint32_t full = base + lay.barriers(), empty = full + 8 * q.stages, ready = empty + 8 * q.stages, drained = ready + 16;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + lay.barriers() + (2 * q.stages + 4) * 8);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int tiles_o = (q.Co + q.rows - 1) / q.rows, tiles = tiles_o * q.tiles_i;
     const int split = (int)(blockIdx.x / (unsigned)tiles), t = (int)blockIdx.x - split * tiles;
@@ -511,11 +513,14 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
             mbar_init(full + 8 * i, PARTS == 3 ? kGroups * kGroupWarps : kGroupWarps);
             mbar_init(empty + 8 * i, 1);
         }
-        mbar_init(ready, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(ready + 8 * i, 1);
+            mbar_init(drained + 8 * i, kWeightEpilogue);
+        }
         fence_mbar_init();
     }
     grid_dependency_wait();
-    if (warp == kWeightEpilogue + kGroups * kGroupWarps) tmem_alloc(tmem_slot, columns);
+    if (warp == kWeightEpilogue + kGroups * kGroupWarps) tmem_alloc(tmem_slot, q.sums_at.all);
     tmem_release();
     __syncthreads();
     tmem_acquire();
@@ -561,9 +566,10 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
         uint32_t stage = 0, phase = 0;
         for (int slice = first; slice < last; ++slice) {
             copies_wait(q.slots);
-            wait(empty + 8 * stage, phase ^ 1);
+            if (__any_sync(0xffffffffu, !wait(empty + 8 * stage, phase ^ 1))) break;
             char *const dz_to = smem + stage * lay.stage(), *const x_to = dz_to + lay.x_at();
             const char *from = own + (q.slots > 1 ? (uint32_t)(slice - first & 1) * slot_bytes : 0);
+            float here[4] = {};
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 float4 v[8];
@@ -579,17 +585,20 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
                                (w.in & 4) * 2;
                     place4(to, w.dz ? lay.dz_part() : lay.x_part(), v[j]);
                     if (half == 0 && sums && w.dz) {      // (dz has 2048 vectors at most)
-                        if (LAST) {
-                            sum[0] += v[j].x;
-                            sum[1] += v[j].y;
-                            sum[2] += v[j].z;
-                            sum[3] += v[j].w;
+                        if (LAST) {      // (a slice's by itself first: fewer additions to a long sum)
+                            here[0] += v[j].x;
+                            here[1] += v[j].y;
+                            here[2] += v[j].z;
+                            here[3] += v[j].w;
                         } else {
                             sum[j] += (v[j].x + v[j].y) + (v[j].z + v[j].w);
                         }
                     }
                 }
             }
+            if (LAST)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[i] += here[i];
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(full + 8 * stage);
@@ -626,7 +635,8 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
     } else if (warp >= kWeightEpilogue && warp < kWeightEpilogue + kGroups * kGroupWarps) {
         const int group = (warp - kWeightEpilogue) / kGroupWarps, me = threadIdx.x - 32 * (kWeightEpilogue + group * kGroupWarps);
         const int of_source = q.rows * 8, of_dz = sources * of_source, total = of_dz + q.bn * 8;      // vectors of a slice
-        float sum[8] = {};      // planes: of the channel of vector me + 128 j of a source; last: of the channels of every vector of dz
+        // planes: of the channel of vector me + 128 j of a source; last: of the channels of every vector of dz.  Of kSumSlices, of all.
+        float sum[8] = {}, total_of[8] = {};
         for (int slice = first + group; slice < last; slice += kGroups) {
             const unsigned nth = slice - first, stage = nth % (unsigned)q.stages, phase = nth / (unsigned)q.stages & 1;
             const int64_t sample = (unsigned)slice / (unsigned)q.slices, p0 = (slice - sample * q.slices) * 64;
@@ -678,6 +688,12 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(full + 8 * stage);
+            if (sums && (nth % kSumSlices<T> >= kSumSlices<T> - kGroups || slice + kGroups >= last))
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    total_of[j] += sum[j];
+                    sum[j] = 0.f;
+                }
         }
         if (sums) {
             // (rows are a power of two: a thread's vectors of dz are all at one place among the channels, or eight lanes' of a channel)
@@ -687,7 +703,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
                 for (int turn = 0; turn < 128 / wide; ++turn) {
                     if (me / wide == turn)
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) sums_smem[group][8 * place + i] = turn ? sums_smem[group][8 * place + i] + sum[i] : sum[i];
+                        for (int i = 0; i < 8; ++i) sums_smem[group][8 * place + i] = turn ? sums_smem[group][8 * place + i] + total_of[i] : total_of[i];
                     asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
                 }
             } else {
@@ -697,10 +713,10 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
                     for (int j = 1; j < 8; j *= 2)
                         if (16 * j == q.rows)
 #pragma unroll
-                            for (int i = 0; i < j; ++i) sum[i] += sum[j + i];
+                            for (int i = 0; i < j; ++i) total_of[i] += total_of[j + i];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    float g = sum[j];
+                    float g = total_of[j];
                     g += __shfl_xor_sync(0xffffffffu, g, 1);
                     g += __shfl_xor_sync(0xffffffffu, g, 2);
                     g += __shfl_xor_sync(0xffffffffu, g, 4);
@@ -711,54 +727,94 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
         }
     } else if (warp == kWeightEpilogue + kGroups * kGroupWarps) {
         if (lane == 0) {
-            uint64_t a[PARTS], b[PARTS];
+            constexpr uint32_t step = LAST ? 128 : 2;      // bytes from k to k
+            const uint64_t dz = LAST ? mn_major(base, 0, kBlockBytes) : k_major(base, 0), x = further(dz, lay.x_at());
+            const uint32_t a_high = (uint32_t)(dz >> 32), b_high = (uint32_t)(x >> 32);
+            uint32_t a[PARTS], b[PARTS];
             for (int i = 0; i < PARTS; ++i) {
-                const uint32_t dz = base + i * lay.dz_part(), x = base + lay.x_at() + i * lay.x_part();
-                a[i] = LAST ? mn_major(dz, 0, kBlockBytes) : k_major(dz, 0);
-                b[i] = LAST ? mn_major(x, 0, kBlockBytes) : k_major(x, 0);
+                a[i] = (uint32_t)further(dz, i * lay.dz_part());
+                b[i] = (uint32_t)further(x, i * lay.x_part());
             }
-            uint32_t stage = 0, phase = 0;
-            for (int slice = first; slice < last; ++slice) {
-                if (!wait(full + 8 * stage, phase)) break;
+            uint32_t stage = 0, phase = 0, set = 0, set_phase = 0;
+            int begin = first, end;      // a sum's slices
+            do {
+                end = min(last, begin + kSumSlices<T>);
+                if (!wait(drained + 8 * set, set_phase ^ 1)) break;
                 tmem_acquire();
-                const uint32_t stage_at = stage * lay.stage();
+                const uint32_t d = tmem + set * columns;
+                for (int slice = begin; slice < end; ++slice) {
+                    if (!wait(full + 8 * stage, phase)) break;
+                    tmem_acquire();
+                    const uint32_t at = stage * lay.stage() >> 4;
 #pragma unroll
-                for (int k = 0; k < 64; k += 16) {
+                    for (int k = 0; k < 64; k += 16) {
 #pragma unroll
-                    for (int i = 0; i < PARTS; ++i)
+                        for (int i = 0; i < PARTS; ++i)
 #pragma unroll
-                        for (int j = 0; j < PARTS - i; ++j)
-                            mma(i + j ? tmem + q.columns : tmem, further(a[i], stage_at + (LAST ? 128 : 2) * k), further(b[j], stage_at + (LAST ? 128 : 2) * k),
-                                q.instruction, slice > first || k || i + j > 1 || i > 0);
-                    if (PARTS == 1 && sources == 2)
-                        mma(tmem, further(a[0], stage_at + lay.dz_part() + (LAST ? 128 : 2) * k), further(b[0], stage_at + (LAST ? 128 : 2) * k), q.instruction, true);
+                            for (int j = 0; j < PARTS - i; ++j)
+                                mma(i + j ? d + q.columns : d, a[i] + at + (step * k >> 4), a_high, b[j] + at + (step * k >> 4), b_high,
+                                    q.instruction, slice > begin || k || i + j > 1 || i > 0);
+                        if (PARTS == 1 && sources == 2)
+                            mma(d, a[0] + at + (lay.dz_part() + step * k >> 4), a_high, b[0] + at + (step * k >> 4), b_high, q.instruction, true);
+                    }
+                    mma_commit(empty + 8 * stage);
+                    if (++stage == (uint32_t)q.stages) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
                 }
-                mma_commit(empty + 8 * stage);
-                if (++stage == (uint32_t)q.stages) {
-                    stage = 0;
-                    phase ^= 1;
+                if (wait.lost) break;
+                mma_commit(ready + 8 * set);
+                if (++set == (uint32_t)q.sums_at.sets) {
+                    set = 0;
+                    set_phase ^= 1;
                 }
-            }
-            if (!wait.lost) mma_commit(ready);
+            } while ((begin = end) < last);
         }
     } else {
         float *partial = q.partial + split * pointwise_partial_stride(q.Co, q.Ci);
-        wait(ready, 0);
-        __syncwarp();
-        tmem_acquire();
         const int row = warp * 32 + lane, o = o0 + row;
         const bool mine = row < q.rows && o < q.Co;
+        uint32_t set = 0, set_phase = 0;
+        auto arrived = [&] {
+            wait(ready + 8 * set, set_phase);
+            __syncwarp();
+            tmem_acquire();
+        };
+        auto sum16 = [&](int b, bool begun, float (&v)[16]) {
+            const uint32_t at = tmem + b + ((uint32_t)warp << 21);
+            accumulators16(at + set * columns, v);
+            if (PARTS == 3) add16(at + set * columns + q.columns, v);
+            if (begun) add16(at + q.sums_at.sets * columns, v);
+        };
+        int begin = first;
+#pragma unroll 1
+        for (; last - begin > kSumSlices<T>; begin += kSumSlices<T>) {
+            arrived();
+#pragma unroll 1
+            for (int b = 0; b < q.bn; b += 16) {
+                float v[16];
+                sum16(b, begin > first, v);
+                store16(tmem + q.sums_at.sets * columns + b + ((uint32_t)warp << 21), v);
+            }
+            tmem_wait_store();
+            tmem_release();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(drained + 8 * set);
+            if (++set == (uint32_t)q.sums_at.sets) {
+                set = 0;
+                set_phase ^= 1;
+            }
+        }
+        arrived();
         for (int b = 0; b < q.bn; b += 16) {
             float v[16];
-            accumulators16(tmem + b + ((uint32_t)warp << 21), v);
+            sum16(b, begin > first, v);
             if constexpr (PARTS == 3) {
                 float u[16], finite = 0.f;
-                accumulators16(tmem + q.columns + b + ((uint32_t)warp << 21), u);
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    v[j] += u[j];
+                for (int j = 0; j < 16; ++j)
                     if (i0 + b + j < q.Ci) finite = fmaf(v[j], 0.f, finite);
-                }
                 if (finite != 0.f && mine) {      // (a NaN: some value is not finite)
 #pragma unroll
                     for (int j = 0; j < 16; ++j) u[j] = 0.f;
@@ -789,7 +845,7 @@ __global__ void __launch_bounds__(kWeightThreads, 1) pointwise_weight_split_kern
     __syncwarp();
     tmem_release();
     __syncthreads();
-    if (warp == kWeightEpilogue + kGroups * kGroupWarps) tmem_free(tmem, columns);
+    if (warp == kWeightEpilogue + kGroups * kGroupWarps) tmem_free(tmem, q.sums_at.all);
     if (sums && (int)threadIdx.x < q.rows && o0 + (int)threadIdx.x < q.Co)
         q.partial[split * pointwise_partial_stride(q.Co, q.Ci) + (int64_t)q.Co * q.Ci + o0 + threadIdx.x] =
             PARTS == 1 && last - first > 1 ? sums_smem[0][threadIdx.x] + sums_smem[1][threadIdx.x] : sums_smem[0][threadIdx.x];
@@ -928,7 +984,7 @@ bool plan_weight_split(const PointwiseShape &s, int sources, WeightSplitPlan *pl
     while (r.columns < r.bn) r.columns *= 2;
     r.slices = ceil_div(P, 64);
     const int64_t all = r.slices * samples, tiles = (int64_t)r.tiles_o * r.tiles_i;
-    r.per = std::max<int64_t>(std::min<int64_t>(4, all), ceil_div(all, std::max<int64_t>(1, 148 / tiles)));
+    r.per = slices_of_split(all, tiles, parts == 3 ? kSumSlices<float> * kMostSums<float> : kSumSlices<__half> * kMostSums<__half>);
     r.splits = (int)ceil_div(all, r.per);
     if (all >= 1 << 30 || r.splits * tiles > INT32_MAX) return false;
     *plan = r;
@@ -963,6 +1019,8 @@ int launch_pointwise_split_weight(const PointwiseShape &s, const void *dz, const
     q.stages = plan.stages;
     q.slots = plan.slots;
     q.columns = plan.columns;
+    q.sums_at = s.io_kind == BC_IO_F32 ? sum_columns(plan.per > kSumSlices<float>, 2 * plan.columns, plan.bn)
+                                       : sum_columns(plan.per > kSumSlices<__half>, plan.columns, plan.bn);
     q.sums = sums;
     q.instruction = mma_instruction(s.io_kind != BC_IO_F16, s.last, s.last, plan.bn);
     const int each = 16 / io_size(s.io_kind);

@@ -1,4 +1,4 @@
-"""pointwise_conv2d and group_norm where values, sums or strides are unusual: slopes that enter products, groups far from zero, tails of SiLU.
+"""pointwise_conv2d and group_norm where values, sums or strides are unusual: slopes that enter products, groups far from zero, tails of SiLU, sums that are very long.
 Definitions in 64 bits and tolerances as in test_gpu_layers.py."""
 import math
 
@@ -118,6 +118,39 @@ def test_silu_keeps_its_tails(bc, dtype, last, count):  # noqa: F811
         g[..., 0] = 1
         grad = torch.autograd.grad(out, b, g)[0]
         assert ((grad.double() - slope).abs() <= tol * parts + 1.01 * SMALLEST[dtype]).all()
+
+
+# ---- long sums of one sign -------------------------------------------------------------------------------
+
+@LAYOUTS
+@pytest.mark.parametrize("shape, dtype", [((1, 16, 16, 2048, 2048), torch.float32), ((1, 1, 1, 8192, 8192), torch.float32), ((1, 3, 2, 4001, 4003), torch.float32),
+                                          ((1, 8, 8, 8192, 4096), torch.float16), ((1, 3, 5, 4096, 4099), torch.float16), ((1, 8, 8, 4096, 4096), torch.bfloat16)], ids=str)
+def test_sums_of_millions_of_one_sign(bc, shape, dtype, last):  # noqa: F811
+    """An accumulator's additions round towards zero, so what they lose of a sum of one sign adds up: it must not grow with the
+    pixels.  n additions that are each off by less than a step of a sum that grows evenly lose less than n / 2 steps of 2^-23.  A
+    sum in an accumulator is of 128 additions at most (16-bit tensors 512): 2^-17 (2^-15).  16 (64) of those make a row, rounded
+    to nearest, half a step: 2^-21 (2^-19), and the rows are added in double.  grad_bias: 256 (512) additions, 8 (64) of or in
+    those, up to 64 threads' in order, rounded to nearest: less than 2^-16 (2^-14)."""
+    N, Ci, Co, h, w = shape
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    layout = torch.channels_last if last else torch.contiguous_format
+    x = torch.empty(N, Ci, h, w, device="cuda", dtype=dtype, memory_format=layout).uniform_(0.5, 1.5, generator=gen)
+    g = torch.empty(N, Co, h, w, device="cuda", dtype=dtype, memory_format=layout).uniform_(0.5, 1.5, generator=gen)
+    weight, bias = torch.zeros(Co, Ci, device="cuda", dtype=dtype).requires_grad_(), torch.zeros(Co, device="cuda", dtype=dtype).requires_grad_()
+    # (16-bit: an eighth of a small power of two, so that sums of 2^25 are in float16's range)
+    scale = 2.0 ** -12 if dtype == torch.float16 else 1.0
+    g = g * scale
+    out = bc.pointwise_conv2d(x, weight, bias)
+    gw, gb = torch.autograd.grad(out, (weight, bias), g)
+    W, B = torch.zeros(Co, Ci, device="cuda").double(), torch.zeros(Co, device="cuda").double()
+    for rows in range(0, h, 256):
+        X, G = x[0, :, rows:rows + 256].double().flatten(1), g[0, :, rows:rows + 256].double().flatten(1)
+        W += G @ X.T
+        B += G.sum(1)
+    once = 0 if dtype == torch.float32 else U[dtype]
+    tol = 2.0 ** -16 if dtype == torch.float32 else 2.0 ** -14 + 2.0 ** -18
+    assert float(((gw.double() - W).abs() / W).max()) <= once + tol
+    assert float(((gb.double() - B).abs() / B).max()) <= once + tol
 
 
 def test_no_wait_has_expired():

@@ -1,6 +1,7 @@
 """Expired waits in the pointwise convolutions' kernels, read from their sources: a thread learns of a loss by itself, so
-its partners at a barrier need not know.  A loop is left on a loss only by a thread that works alone (`lane == 0`);
-elsewhere one thread would go on to the kernel's last barrier while its partners waited at the loop's."""
+its partners at a barrier need not know.  A loop is left on a loss only by a thread that works alone (`lane == 0`), or by a
+whole warp (`__any_sync`) whose loop has no other warps' barriers; elsewhere one thread would go on to the kernel's last
+barrier while its partners waited at the loop's."""
 import os
 import re
 
@@ -8,37 +9,52 @@ import pytest
 
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "box-convolutions_b200", "csrc")
 # a jump or a wait that depends on a loss
-ON_LOSS = re.compile(r"if \((?:!wait\(.*\)|!?wait\.lost|.*wait\.lost.*)\) (break|return|continue|wait\()")
+ON_LOSS = re.compile(r"if \([^;\n]*(?:!wait\(|wait\.lost)[^;\n]*\) (?:break|return|continue|wait\()")
+OTHER_WARPS = re.compile(r"bar\.sync|__syncthreads|together\(")
+
+
+def without_comments(text):
+    return re.sub(r"//[^\n]*", "", text)
 
 
 def scopes(text):
-    """(position, headers of the braces that are open there) of every character that opens or closes one."""
-    open_at, out, start = [], [], 0
-    for m in re.finditer(r"[{};]", text):
-        if m.group() == "{":
-            open_at.append(text[start:m.start()])
-        elif m.group() == "}" and open_at:
-            open_at.pop()
+    """(start, end, what stands in front of it) of every pair of braces."""
+    text = re.sub(r"\w\{[^{};]*\}", lambda m: " " * len(m.group()), text)      # (initial values)
+    open_at, out, start, depth = [], [], 0, 0
+    for m in re.finditer(r"[(){};]", text):
+        c = m.group()
+        depth += (c == "(") - (c == ")")
+        if c in "()" or c == ";" and depth:
+            continue
+        if c == "{":
+            open_at.append((m.start(), text[start:m.start()], depth))
+            depth = 0
+        elif c == "}" and open_at:
+            begin, head, depth = open_at.pop()
+            out.append((begin, m.end(), head))
         start = m.end()
-        out.append((m.end(), list(open_at)))
     return out
 
 
 def shared_exits(text):
-    text = re.sub(r"//[^\n]*", "", text)
+    text = without_comments(text)
     places = scopes(text)
     found = []
     for m in ON_LOSS.finditer(text):
-        at = max((p for p in places if p[0] <= m.start()), default=(0, []), key=lambda p: p[0])[1]
-        if not any(re.search(r"\blane == 0\b", h) for h in at):
-            found.append(text[:m.start()].count("\n") + 1)
+        around = [p for p in places if p[0] < m.start() < p[1]]
+        if any(re.search(r"\blane == 0\b", head) for _, _, head in around):
+            continue
+        loops = [text[a:b] for a, b, head in around if re.search(r"\b(for|while|do)\b", head)]
+        if "__any_sync" in m.group() and loops and not any(OTHER_WARPS.search(t) for t in loops):
+            continue
+        found.append(text[:m.start()].count("\n") + 1)
     return found
 
 
 @pytest.mark.parametrize("name", ["pointwise_mma.cu", "pointwise_split.cu"])
 def test_only_a_thread_alone_leaves_its_loop_on_a_loss(name):
     text = open(os.path.join(CSRC, name)).read()
-    assert len(ON_LOSS.findall(re.sub(r"//[^\n]*", "", text))) >= 4      # (of the threads that issue copies and products)
+    assert len(ON_LOSS.findall(without_comments(text))) >= 4      # (of the threads that issue copies and products)
     assert shared_exits(text) == []
 
 
@@ -54,4 +70,6 @@ def test_a_block_that_lost_an_arrival_waits_before_it_frees_what_products_write(
 def test_the_reader_finds_a_shared_exit():
     alone = "void f() { if (lane == 0) { for (;;) { if (!wait(full, 0)) break; } } }"
     shared = "void f() { for (;;) { if (!wait(full, 0)) break; __syncwarp(); } }"
-    assert shared_exits(alone) == [] and shared_exits(shared) == [1]
+    warp = "void f() { for (;;) { if (__any_sync(all, !wait(full, 0))) break; __syncwarp(); } }"
+    pair = "void f() { for (;;) { if (__any_sync(all, wait.lost)) break; together(); } }"
+    assert shared_exits(alone) == [] and shared_exits(shared) == [1] and shared_exits(warp) == [] and shared_exits(pair) == [1]
