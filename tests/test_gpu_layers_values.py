@@ -1,4 +1,4 @@
-"""pointwise_conv2d and group_norm where values, sums or strides are unusual: slopes that enter products, groups far from zero, tails of SiLU, sums that are very long.
+"""pointwise_conv2d and group_norm where values, sums or strides are unusual: slopes that enter products, groups far from zero, tails of SiLU, sums that are very long, sums that are exact.
 Definitions in 64 bits and tolerances as in test_gpu_layers.py."""
 import math
 
@@ -118,6 +118,35 @@ def test_silu_keeps_its_tails(bc, dtype, last, count):  # noqa: F811
         g[..., 0] = 1
         grad = torch.autograd.grad(out, b, g)[0]
         assert ((grad.double() - slope).abs() <= tol * parts + 1.01 * SMALLEST[dtype]).all()
+
+
+# ---- exact sums over many pixels -------------------------------------------------------------------------
+
+@LAYOUTS
+@pytest.mark.parametrize("act", [None, "relu"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("shape", [(2, 24, 40, 311, 328), (2, 25, 37, 311, 331), (1, 264, 136, 161, 168), (3, 130, 20, 101, 171)], ids=str)
+def test_sums_of_whole_numbers_are_exact(bc, shape, act, dtype, last):  # noqa: F811
+    """Small whole numbers, whose sums are exact in any order: a slice of pixels that is lost or taken twice shows, with some
+    twenty slices and more for every partial sum (rings go round several times)."""
+    N, Ci, Co, h, w = shape
+    gen = torch.Generator(device="cuda").manual_seed(Ci)
+
+    def whole(size, most):
+        t = torch.randint(-most, most + 1, size, device="cuda", generator=gen).to(dtype)
+        return t.contiguous(memory_format=torch.channels_last if last else torch.contiguous_format) if len(size) == 4 else t
+
+    x, g = whole((N, Ci, h, w), 2).requires_grad_(), whole((N, Co, h, w), 2)
+    weight, bias = whole((Co, Ci), 1).requires_grad_(), (whole((Co,), 3) + 0.5).requires_grad_()
+    out = bc.pointwise_conv2d(x, weight, bias, activation=act)
+    got = torch.autograd.grad(out, (x, weight, bias), g)
+    X, G = (t.detach().double().permute(0, 2, 3, 1).reshape(-1, t.shape[1]) for t in (x, g))
+    z = X @ weight.detach().double().T + bias.detach().double()
+    dz = G * (z > 0) if act else G
+    planes = lambda t: t.reshape(N, h, w, -1).permute(0, 3, 1, 2)  # noqa: E731
+    for name, a, b in (("out", out, planes(act64(z, act))), ("grad_input", got[0], planes(dz @ weight.detach().double())),
+                       ("grad_weight", got[1], dz.T @ X), ("grad_bias", got[2], dz.sum(0))):
+        assert torch.equal(a, b.to(dtype)), name
 
 
 # ---- long sums of one sign -------------------------------------------------------------------------------
