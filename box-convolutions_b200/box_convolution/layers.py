@@ -11,7 +11,9 @@ group of planes, so that a step does not depend on how the batch is sharded.
 
 Inputs are float32, float16 or bfloat16, all tensors of a call alike, ``(N, C, h, w)`` in planes (contiguous: what a box
 convolution reads and writes) or channels last; outputs and gradients come in the input's layout.  Tensors of other
-strides are copied first.  Sums, statistics and activations are float32 whatever the type, results are rounded once (a
+strides are copied first.  The fastest kernels want arrays on 16 bytes, 16-bit convolutions also rows of a multiple of 16 bytes; a
+normalisation of a view that starts elsewhere (or, channels last, of channels that take more than 1024 vectors of 16 bytes to
+repeat their place in one) runs value by value, many times slower.  Sums, statistics and activations are float32 whatever the type, results are rounded once (a
 16-bit gradient through an activation enters its products as two values of that type, off by 2^-16 or 2^-22 of it).  Results
 are the same bits from call to call.  Activations: None, "relu", "silu", "gelu" (the one with the error function).  The backward pass computes the
 activation's argument again from what the forward pass was given: nothing but the inputs is kept (and two

@@ -138,7 +138,7 @@ std::vector<Tensor> run_pointwise_backward(const Tensor &x, const Tensor &weight
     if (mask & BC_NEED_PW_INPUT) g[0] = new_maps(x.sizes(), s.last, x);
     if (mask & BC_NEED_PW_WEIGHT) g[1] = new_tensor(weight.sizes(), x.scalar_type(), x);
     if (mask & BC_NEED_PW_BIAS) g[2] = new_tensor({s.Co}, x.scalar_type(), x);
-    if (mask & BC_NEED_PW_RESIDUAL) g[3] = s.act == BC_ACT_NONE ? grad_output : new_maps(s.out_sizes, s.last, x);
+    if (mask & BC_NEED_PW_RESIDUAL) g[3] = s.act == BC_ACT_NONE ? grad : new_maps(s.out_sizes, s.last, x);
     const int kind = io_kind(x.scalar_type());
     const size_t bytes = bc_pointwise_backward_workspace(kind, s.N, s.Ci, s.Co, s.P, s.last, s.act, mask);
     Tensor ws;

@@ -1,11 +1,11 @@
-"""pointwise_conv2d and group_norm where values, sums or strides are unusual: slopes that enter products, groups far from zero, tails of SiLU, sums that are very long, sums that are exact.
+"""pointwise_conv2d and group_norm where values, sums or strides are unusual: slopes that enter products, groups far from zero, tails of SiLU, sums that are very long, sums that are exact, layouts of gradients.
 Definitions in 64 bits and tolerances as in test_gpu_layers.py."""
 import math
 
 import pytest
 import torch
 
-from test_gpu_layers import DTYPES, FN, TINY, U, act64, bc, check_norm, maps, slope64, slope_error, within  # noqa: F401
+from test_gpu_layers import DTYPES, FN, TINY, U, act64, bc, check_norm, maps, same_layout, slope64, slope_error, within  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -180,6 +180,23 @@ def test_sums_of_millions_of_one_sign(bc, shape, dtype, last):  # noqa: F811
     tol = 2.0 ** -16 if dtype == torch.float32 else 2.0 ** -14 + 2.0 ** -18
     assert float(((gw.double() - W).abs() / W).max()) <= once + tol
     assert float(((gb.double() - B).abs() / B).max()) <= once + tol
+
+
+# ---- layouts ---------------------------------------------------------------------------------------------
+
+@LAYOUTS
+@pytest.mark.parametrize("act", [None, "silu"])
+def test_every_gradient_has_the_inputs_layout(bc, act, last):  # noqa: F811
+    x, r = (maps(torch.Generator(device="cuda").manual_seed(s), (2, c, 6, 10), torch.float32, last).requires_grad_() for s, c in ((1, 24), (2, 40)))
+    w = torch.randn(40, 24, device="cuda")
+    other = torch.contiguous_format if last else torch.channels_last
+    for g in (torch.randn(2, 40, 6, 10, device="cuda").contiguous(memory_format=other), torch.randn(1, 40, 1, 1, device="cuda").expand(2, 40, 6, 10),
+              torch.randn(2, 40, 10, 6, device="cuda").transpose(2, 3)):
+        for leaves in ((x, r), (r,)):
+            got = torch.autograd.grad(bc.pointwise_conv2d(x, w, activation=act, residual=r), leaves, g)
+            assert all(same_layout(t, last) for t in got)
+            if act is None:
+                assert torch.equal(got[-1], g)
 
 
 def test_no_wait_has_expired():
