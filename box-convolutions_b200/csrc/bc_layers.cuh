@@ -114,9 +114,11 @@ __device__ __forceinline__ uint4 left_by_rounding(const f2_t (&v)[kVec<T> / 2], 
 // ---- activations (BC_ACT_*), of two values at a time.  A NaN stays one in all of them; the ReLU's slope at zero and at NaN
 // is 0, as PyTorch's.  Exponentials and quotients are the hardware's powers of two and reciprocals (2^-22 and 2^-23): with
 // CUDA's own functions a normalisation of float planes with SiLU was bound by instructions, (256,32,64,128) forward 148 us.
-// Float tensors carry the rounding of the exponent along; 16-bit ones, whose results are rounded to 2^-9 or 2^-12, do not, and
-// take the normal distribution function from Abramowitz and Stegun's 7.1.26: five terms of 1 / (1 + 0.3275911 |x|) times
-// exp(-x^2), x = z / sqrt(2), off by 7.5e-8 at most.
+// Float tensors carry the rounding of the exponent along; 16-bit ones, whose results are rounded to 2^-9 or 2^-12, do not.
+// Their normal distribution function, below zero, is exp(-z^2 / 2) times t (c1 + ... + c6 t^5), t = 1 / (1 + 0.29 |z|): the form of
+// Abramowitz and Stegun's 7.1.26 with a term more, its coefficients fitted by weighted least squares (Lawson's iteration) to errors of
+// 4.8e-8 or, in the tail down to -13, 2^-13 of the function.  (7.1.26 itself is off by 7.5e-8, and by 4 % of the tail.)  With the
+// arithmetic's errors it is off by 2.5e-7 and 10^-4 at most over all 16-bit arguments.
 __device__ __forceinline__ float power_of_two(float v)
 {
     float r;
@@ -188,15 +190,18 @@ __device__ __forceinline__ f2_t normal2(f2_t z, f2_t &density)
 {
     if constexpr (sizeof(T) == 4) {
         density = of_each(z, [](float v) { return expf(-0.5f * v * v); });
+        // (off by 2^-24 of 1, so that the tail's digits are lost from -3 on, as PyTorch's; with erfcf in its place, or below -2.5
+        // alone, (256,32,64,128) planes took 166 to 175 us forward instead of 138, and 326 to 331 backward instead of 244)
         return of_each(z, [](float v) { return 0.5f * (1.f + erff(v * 0.70710678118654752f)); });
     }
     density = of_each(mul2(mul2(z, z), both(-0.5f * 1.4426950408889634f)), power_of_two);
     const f2_t size = of_each(z, [](float v) { return fabsf(v); });
-    const f2_t t = of_each(fma2(size, both(0.3275911f * 0.70710678118654752f), both(1.f)), reciprocal);
-    f2_t p = fma2(both(0.5f * 1.061405429f), t, both(0.5f * -1.453152027f));
-    p = fma2(p, t, both(0.5f * 1.421413741f));
-    p = fma2(p, t, both(0.5f * -0.284496736f));
-    p = fma2(p, t, both(0.5f * 0.254829592f));
+    const f2_t t = of_each(fma2(size, both(0.29f), both(1.f)), reciprocal);
+    f2_t p = fma2(both(-0.0896348559f), t, both(0.287845366f));
+    p = fma2(p, t, both(-0.0973541001f));
+    p = fma2(p, t, both(0.182338251f));
+    p = fma2(p, t, both(0.0998317281f));
+    p = fma2(p, t, both(0.116973562f));
     p = mul2(mul2(p, t), density);      // the smaller of the two tails
     float z0, z1, p0, p1;
     unpack2(z, z0, z1);

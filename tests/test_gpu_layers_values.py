@@ -1,5 +1,5 @@
-"""pointwise_conv2d and group_norm where values, sums or strides are unusual: slopes that enter products, groups far from zero, tails of SiLU, sums that are very long, sums that are exact, layouts of gradients.
-Definitions in 64 bits and tolerances as in test_gpu_layers.py."""
+"""pointwise_conv2d and group_norm where values, sums or strides are unusual: slopes that enter products, groups far from zero,
+tails of SiLU and GELU, very long sums and exact ones, layouts of gradients.  Definitions in 64 bits and tolerances as in test_gpu_layers.py."""
 import math
 
 import pytest
@@ -114,6 +114,39 @@ def test_silu_keeps_its_tails(bc, dtype, last, count):  # noqa: F811
         b = z.clone().requires_grad_()
         out = bc.group_norm(gx, 1, torch.zeros_like(z), b, activation="silu")
         close(out[0].flatten(1), ref[:, None].expand(-1, gx.shape[3]), tol, "group_norm")
+        g = torch.zeros_like(out)
+        g[..., 0] = 1
+        grad = torch.autograd.grad(out, b, g)[0]
+        assert ((grad.double() - slope).abs() <= tol * parts + 1.01 * SMALLEST[dtype]).all()
+
+
+# ---- GELU far below zero ---------------------------------------------------------------------------------
+
+@LAYOUTS
+@pytest.mark.parametrize("dtype", NARROW, ids=str)
+@pytest.mark.parametrize("count", [512, 509])
+def test_gelu_of_16_bits_keeps_its_tails(bc, dtype, last, count):  # noqa: F811
+    """z from -13 to 13, where z times the normal distribution function is a normal number of bfloat16, relative errors of value and
+    slope: u, 2^-13 of the function, and an argument z^2 / 2 of the exponential that is rounded to half a step, which moves it by up
+    to z^2 2^-24 relatively, twice that with a dozen other steps."""
+    z = torch.linspace(-13, 13, count, device="cuda").to(dtype)
+    Z = z.double()
+    P, density = 0.5 * torch.erfc(-Z / math.sqrt(2)), torch.exp(-0.5 * Z * Z) / math.sqrt(2 * math.pi)
+    ref, slope, parts = Z * P, P + Z * density, P + Z.abs() * density
+    tol = 2.0 ** -23 * (Z * Z + 16) + U[dtype] + 2.0 ** -13
+    shape = (1, 8, count, 1) if not last else (1, 8, 1, count)
+    layout = torch.channels_last if last else torch.contiguous_format
+    r = z.view(shape[2:]).expand(shape).contiguous(memory_format=layout).requires_grad_()
+    x, w = torch.zeros(1, 8, *shape[2:], device="cuda", dtype=dtype).contiguous(memory_format=layout), torch.zeros(8, 8, device="cuda", dtype=dtype)
+    out = bc.pointwise_conv2d(x, w, activation="gelu", residual=r)
+    close(out[0].flatten(1), ref.expand(8, -1), tol, "pointwise")
+    grad = torch.autograd.grad(out, r, torch.ones_like(out))[0]
+    assert ((grad[0].flatten(1).double() - slope).abs() <= tol * parts + 1.01 * SMALLEST[dtype]).all()
+    x = torch.randn(1, count, 1, 1, device="cuda").to(dtype)
+    for gx in (x, x.expand(1, count, 1, 9).contiguous(memory_format=layout)):
+        b = z.clone().requires_grad_()
+        out = bc.group_norm(gx, 1, torch.zeros_like(z), b, activation="gelu")
+        close(out[0].flatten(1), ref[:, None].expand(-1, gx.shape[3]), tol[:, None], "group_norm")
         g = torch.zeros_like(out)
         g[..., 0] = 1
         grad = torch.autograd.grad(out, b, g)[0]
