@@ -531,8 +531,10 @@ bool plan_rows(const NormShape &s, NormRows *plan)
     r.width = s.C;
     r.slabs = 1;
     const int64_t sample = s.P * s.C * size;
-    // Parts of the channels as units of their own: down to 64 bytes a pixel where the GPU would not fill, to 128 where slices
-    // would be long ((16,128,64,128) bf16: forward 37 us at 64 bytes, 33 at 128; (1,64,256,512) f32 the other way round, 17 and 19).
+    // Parts of the channels as units of their own: down to 64 bytes a pixel where the GPU would not fill ((1,64,256,512) f32 forward
+    // 17 us, 19 at 128 bytes), to 128 where slices would be long.  us forward + backward of that against no parts there, and
+    // against 64 bytes there too: (16,128,64,128) bf16 35 + 48, 35 + 48, 41 + 54; f32 43 + 99, 58 + 101, 43 + 101; (24,256,64,128) bf16
+    // 78 + 146, 132 + 177, 82 + 154; (64,64,64,128) bf16 68 + 103, 68 + 101, 62 + 105; (24,64,128,128) f32 56 + 199, 72 + 203, 66 + 170.
     while (r.width % 2 == 0 && r.width / 2 % D == 0 && r.width / 2 * size % 64 == 0 &&
            (s.N * r.slabs * kNormCluster < 148 || (sample / r.slabs > kNormCluster * kNormSlice && r.width / 2 * size % 128 == 0))) {
         r.width /= 2;

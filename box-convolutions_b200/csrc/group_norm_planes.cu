@@ -11,9 +11,16 @@ namespace {
 
 constexpr int kPiece = 256;            // vectors: eight a lane
 constexpr int kMostPieces = 2048;      // of a CTA: their sums are kept in shared memory
-// Bytes that are worth a CTA: (256,32,64,128) f32, 8 groups, SiLU, forward 112 us with a group of 128 KB a CTA, 145 with a
-// cluster of two, 137 of four; backward 182, 185, 182.
-constexpr int64_t kPlaneSlice = 128 << 10;
+// Bytes that are worth a CTA.  A CTA a group, or a cluster of two where a group is longer than that; 256 samples, 8 groups, SiLU, f32,
+// us forward and backward by the size of a group:
+//     128 KB  119 + 191 (one), 156 + 201 (two)     136 KB  185 + 308, 256 + 355     192 KB  176 + 312, 215 + 307
+//     256 KB  243 + 407 (one), 245 + 403 (two)     384 KB  366 + 622 (two), 366 + 622 (four), 435 + 615 (eight)
+// and bf16, 160 KB, 178 + 328 and 235 + 348: up to 256 KB one is as fast or faster, beyond they are alike.
+constexpr int64_t kPlaneSlice = 256 << 10;
+// Bytes of a CTA up to which a cluster of eight serves a group where that leaves SMs without work: (2,64,256,512) bf16, 8 groups of
+// 2 MB, SiLU: 41 us forward and 61 backward with 256 KB a CTA; in two launches over the whole GPU 22 + 22 and 31 + 31, each timed
+// by itself, of which some 5 are the timing.
+constexpr int64_t kClusterSlice = 128 << 10;
 
 // Where a piece lies: values [a, b) of the tensor, whole vectors [v0, v1) of those.
 template <typename T>
@@ -352,7 +359,7 @@ void plan_planes(const NormShape &s, NormPlanes *plan)
     int64_t k = norm_ceil(bytes, kPlaneSlice);
     if (units * k < kNormFill) k = norm_ceil(kNormFill, units);
     k = std::min(k, norm_ceil(bytes, (int64_t)8 << 10));
-    if (k > kNormCluster && (units * kNormCluster >= 148 || bytes <= kNormCluster * kPlaneSlice)) k = kNormCluster;
+    if (k > kNormCluster && (units * kNormCluster >= 148 || bytes <= kNormCluster * kClusterSlice)) k = kNormCluster;
     k = std::max<int64_t>(1, std::min(k, pieces));
     if (k <= kNormCluster) {
         int p = 1;
