@@ -5,8 +5,8 @@
 // number is a multiple of the vectors after which the places repeat (60 channels: 15 vectors of 8 are 2 pixels).  The
 // values in front of a slice's first whole vector and behind its last are dealt with one by one.
 //
-// Measured on B200, (16,128,64,128) bf16 with SiLU: forward 26 us, backward 40 (the bytes at the copy bandwidth: 10 and 15): two
-// powers of two and reciprocals a value and reading are half of it, the exchange of the clusters most of the rest.
+// Measured on B200, (16,128,64,128) bf16 with SiLU: forward 30 us, backward 43 (the bytes at the copy bandwidth: 10 and 15).  256 CTAs of
+// 256 threads are fewer than two an SM: what a reading waits for has little beside it, nor has the exchange of the clusters.
 //
 // Position q of a CTA's vectors (thread q / V, value q % V) holds channel (phase + q) % width: reductions walk positions.
 //

@@ -343,7 +343,7 @@ size_t sums_bytes(const PointwiseShape &s)
 bool own_dz(const PointwiseShape &s, int need_mask) { return s.act != BC_ACT_NONE && !(need_mask & BC_NEED_PW_RESIDUAL); }
 // A 16-bit dz goes into its products as its rounding (grad_residual) and what that leaves, rounded: off by u^2 of it.  With
 // the rounding alone grad_input and grad_weight were 1.4 times as far from their definition as one rounding puts them; a step of
-// (64,256->256,64,128) bf16 last with GELU took 706 us, and takes 864.
+// (64,256->256,64,128) bf16 last with GELU took 706 us, and takes 831 to 883.
 bool keeps_rest(const PointwiseShape &s, int need_mask)
 {
     return s.act != BC_ACT_NONE && s.io_kind != BC_IO_F32 && (need_mask & (BC_NEED_PW_INPUT | BC_NEED_PW_WEIGHT | BC_NEED_PW_BIAS));

@@ -8,10 +8,12 @@
 // residuals and gradients and writes results 16 bytes a lane, 64 bytes in a row, along whichever index runs in memory.  Where a
 // CTA has its SM to itself, the next block's are on their way while a block is dealt with.
 //
-// Measured on B200, (64,256->256,64,128) bf16 last: grad_input 97 us, 5.4 TB/s or 0.83 of the copy bandwidth; forward with residual
-// and GELU 182, slope 249, bound by the epilogue's instructions (grad_input of one tensor; the slope without storing what its rounding leaves).
+// Measured on B200, (64,256->256,64,128) bf16 last: grad_input 97 us, 5.4 TB/s or 0.83 of the copy bandwidth, and 151 where dz is two
+// tensors (5.3); forward with residual and GELU 182, slope that stores two tensors 291.  Those two wait for memory and shared memory with a
+// CTA an SM: 0.41 and 0.47 instructions a cycle and scheduler, 1.5 and 1.4 times what their bytes take.
 //
-// pointwise_weight_mma_kernel: grad_weight, D[o, i] = sum_p dz[o, p] x[i, p], 128 x up to 256 weights, split over the pixels; 96 us there.
+// pointwise_weight_mma_kernel: grad_weight, D[o, i] = sum_p dz[o, p] x[i, p], 128 x up to 256 weights, split over the pixels; 94 us there, 129
+// of two tensors.
 #include "bc_mma.cuh"
 
 namespace bc {

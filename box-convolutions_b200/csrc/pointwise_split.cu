@@ -6,9 +6,10 @@
 // of nine pairs; the six are made that reach above 2^-26 of it: the upper ones into one accumulator, the others into a second or a
 // third, added at the end.  (An accumulator's additions round towards zero: the others stay 2^-8 of the first, which sees a
 // sixth of the additions.)  Measured against multiply-adds, which wait for shared memory here ((16,128->32,64,128) planes: 38 us).
-// With them 26 us forward, 34 with the slope, 34 grad_input, 38 grad_weight (13 to 15 at the copy bandwidth): an instruction takes
+// With them 26 us forward, 34 with the slope, 35 grad_input, 42 grad_weight (13 to 15 at the copy bandwidth): an instruction takes
 // some 90 cycles here whether it is 32 or 128 columns wide, and splitting the operands about as long as the products.
-// Infinities and NaN have no such sum: a result that is not finite is computed again by multiply-adds.
+// Infinities and NaN have no such sum: a result that is not finite is computed again by multiply-adds.  (Parts end at 2^-133, bf16's
+// smallest number: operands below 2^-110 lose digits.)
 #include "bc_mma.cuh"
 
 namespace bc {
@@ -870,7 +871,9 @@ bool plan_split(const PointwiseShape &s, int K, int Cn, SplitPlan *plan)
     // channels of a tile: what shared memory holds of the weights, and tensor memory of the sums
     const uint32_t others = SplitLayout{16, r.stages, 0, parts, s.last}.bytes() + 8192;
     const int64_t most = std::min<int64_t>(parts == 3 ? 128 : 256, (int64_t)(kMostShared - others) / (parts * chunks * 128) / 16 * 16);
-    if (most < 32 && Cn > most) return false;      // (every tile splits the operand again: multiply-adds are as fast)
+    // (every tile splits the operand again.  f32, 16 samples of 64 x 128 pixels, forward: 400 -> 400 channels in tiles of 32 641 us, by
+    // multiply-adds 1168; 512 -> 512, where tiles would be of 16, by multiply-adds 1675)
+    if (most < 32 && Cn > most) return false;
     if (most < 16) return false;
     r.tiles_n = (int)ceil_div(Cn, most);
     r.bn = (int)ceil_div(ceil_div(Cn, r.tiles_n), 16) * 16;
